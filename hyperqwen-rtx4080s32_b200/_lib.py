@@ -52,6 +52,11 @@ SIGNATURES = {
                                          _i64, _i64, _vp]),
     "gq_gemv_grouped_allreduce_silu_mul": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i32, _i32, _vp,
                                                   _i64, _i64, _vp]),
+    "gq_low_rank_workspace_bytes": (_i64, [_vp]),
+    "gq_low_rank_add": (_i32, [_vp, _vp]),
+    "gq_head_norm_rope": (_i32, [_vp, _vp]),
+    "gq_attention_workspace_bytes": (_i64, [_vp]),
+    "gq_paged_attention": (_i32, [_vp, _vp]),
     "gq_prefill_plan": (_i32, [_i64, _i64, _i64, _i32, _vp]),
     "gq_prefill_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64]),
     "gq_gemm_prefill": (_i32, [_vp, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _vp]),

@@ -14,12 +14,16 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB = os.path.join(_HERE, "libgq_b200.so")
 EXT = os.path.join(_HERE, "_gq_torch.so")
-SOURCES = ["gq_b200.cu"]
+SOURCES = ["gq_b200.cu", "gq_block.cu"]     # translation units: the quantized layers, the operators beside them
+OBJ_DIR = os.path.join(CSRC, "_generated")
 EXT_SOURCE = os.path.join(CSRC, "gq_torch.cpp")
 EXT_STAMP = os.path.join(CSRC, "_generated", "gq_torch.stamp")     # what the extension was compiled against
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))) + [os.path.join("..", "..", "include", "gq_b200.h")]
+BLOCK_HEADERS = ["gq_adapters.cuh", "gq_heads.cuh", "gq_paged.cuh"]      # read by gq_block.cu alone
+UNIT_HEADERS = {"gq_b200.cu": [h for h in HEADERS if h not in BLOCK_HEADERS],
+                "gq_block.cu": BLOCK_HEADERS + ["gq_common.cuh", "gq_host.h", "gq_layout.h", HEADERS[-1]]}
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "--expt-relaxed-constexpr", "-diag-suppress", "177",
-              "-shared", "-Xcompiler", "-fPIC"]
+              "-Xcompiler", "-fPIC"]
 
 
 def _newest(paths):
@@ -33,10 +37,13 @@ def build(force: bool = False, verbose: bool = False) -> str:
     finally:
         sys.path.pop(0)
     table_h = gen_tables.generate()
-    srcs = [os.path.join(CSRC, s) for s in SOURCES]
-    deps = srcs + [os.path.join(CSRC, h) for h in HEADERS] + [table_h]
-    if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < _newest(deps):
-        _build_lib(srcs, verbose)
+    stale = []
+    for src in SOURCES:
+        deps = [os.path.join(CSRC, d) for d in [src] + UNIT_HEADERS[src]] + [table_h]
+        if force or not os.path.exists(_object(src)) or os.path.getmtime(_object(src)) < _newest(deps):
+            stale.append(src)
+    if stale or not os.path.exists(LIB) or os.path.getmtime(LIB) < _newest([_object(s) for s in SOURCES]):
+        _build_lib(stale, verbose)
     if force or not _ext_current():
         _build_ext()
     return LIB
@@ -61,10 +68,19 @@ def _ext_current() -> bool:
         return False
 
 
-def _build_lib(srcs, verbose: bool) -> None:
+def _object(src: str) -> str:
+    return os.path.join(OBJ_DIR, os.path.splitext(src)[0] + ".o")
+
+
+def _build_lib(stale, verbose: bool) -> None:
+    """Compiles the units that are out of date, side by side, and links the library."""
     nvcc = os.environ.get("NVCC") or ("/usr/local/cuda/bin/nvcc" if os.path.exists("/usr/local/cuda/bin/nvcc") else "nvcc")
-    cmd = [nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-o", LIB] + srcs
-    subprocess.check_call(cmd, cwd=CSRC)
+    cmds = [[nvcc] + NVCC_FLAGS + (["-Xptxas", "-v"] if verbose else []) + ["-c", os.path.join(CSRC, src), "-o", _object(src)] for src in stale]
+    runs = [subprocess.Popen(cmd, cwd=CSRC) for cmd in cmds]
+    for cmd, code in zip(cmds, [r.wait() for r in runs]):
+        if code:
+            raise subprocess.CalledProcessError(code, cmd)
+    subprocess.check_call([nvcc, "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-Xcompiler", "-fPIC", "-o", LIB] + [_object(s) for s in SOURCES], cwd=CSRC)
 
 
 def _build_ext() -> None:

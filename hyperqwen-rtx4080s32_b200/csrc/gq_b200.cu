@@ -8,6 +8,7 @@
 #include <mutex>
 #include <unordered_map>
 #include "../../include/gq_b200.h"
+#include "gq_host.h"
 #include "gq_decode.cuh"
 #include "gq_decode8.cuh"
 #include "gq_scale16.cuh"
@@ -22,21 +23,11 @@ using namespace gq;
 static thread_local char g_cuda_err[256] = "";
 static std::atomic<long long> g_launches{0};
 
-static int cuda_fail(cudaError_t e, const char *what) {
+int gq::cuda_fail(cudaError_t e, const char *what) {
     snprintf(g_cuda_err, sizeof g_cuda_err, "%s: %s", what, cudaGetErrorString(e));
     return GQ_ERR_CUDA;
 }
-#define GQ_CUDA(call)                                          \
-    do {                                                       \
-        cudaError_t e_ = (call);                               \
-        if (e_ != cudaSuccess) return cuda_fail(e_, #call);    \
-    } while (0)
-#define GQ_LAUNCHED()                                                    \
-    do {                                                                 \
-        cudaError_t e_ = cudaGetLastError();                             \
-        if (e_ != cudaSuccess) return cuda_fail(e_, "kernel launch");    \
-        g_launches.fetch_add(1, std::memory_order_relaxed);              \
-    } while (0)
+void gq::count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
 extern "C" const char *gq_last_cuda_error(void) { return g_cuda_err; }
 extern "C" int64_t gq_launch_count(void) { return (int64_t)g_launches.load(); }
@@ -2150,15 +2141,18 @@ extern "C" int gq_gemm_prefill(const void *x_dev, int64_t M, int64_t K, int64_t 
 }
 
 extern "C" int gq_device_status(int clear, void *stream) {
-    int v = 0;
-    GQ_CUDA(cudaMemcpyFromSymbolAsync(&v, g_sticky_status, sizeof v, 0, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
-    GQ_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
-    if (clear && v != 0) {
+    const cudaStream_t st = (cudaStream_t)stream;
+    int v = 0, b = 0;                      // the word of this unit's kernels, and that of the operators beside the layers
+    GQ_CUDA(cudaMemcpyFromSymbolAsync(&v, g_sticky_status, sizeof v, 0, cudaMemcpyDeviceToHost, st));
+    GQ_CUDA(block_status_read(&b, st));
+    GQ_CUDA(cudaStreamSynchronize(st));
+    if (clear && (v != 0 || b != 0)) {
         const int zero = 0;
-        GQ_CUDA(cudaMemcpyToSymbolAsync(g_sticky_status, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, (cudaStream_t)stream));
-        GQ_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+        GQ_CUDA(cudaMemcpyToSymbolAsync(g_sticky_status, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, st));
+        GQ_CUDA(block_status_clear(st));
+        GQ_CUDA(cudaStreamSynchronize(st));
     }
-    return v;
+    return v > b ? v : b;
 }
 
 extern "C" int gq_set_peer_wait_limit_ns(int64_t ns) {

@@ -1,0 +1,116 @@
+// The operators beside the quantized layers of a decoder block: low-rank adapters of many requests beside a layer, norms and rotation of
+// queries and keys with the store into a paged cache, attention over that cache.  C ABI in include/gq_b200.h.
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include "gq_host.h"
+#include "gq_adapters.cuh"
+#include "gq_heads.cuh"
+#include "gq_paged.cuh"
+
+using namespace gq;
+
+// the largest status code a kernel of this unit reported since it was last read
+__device__ int g_block_status;
+
+cudaError_t gq::block_status_read(int *code, cudaStream_t s) { return cudaMemcpyFromSymbolAsync(code, g_block_status, sizeof(int), 0, cudaMemcpyDeviceToHost, s); }
+cudaError_t gq::block_status_clear(cudaStream_t s) {
+    static const int zero = 0;
+    return cudaMemcpyToSymbolAsync(g_block_status, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, s);
+}
+
+static bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+static int status_word(int **p) {
+    GQ_CUDA(cudaGetSymbolAddress((void **)p, g_block_status));
+    return GQ_OK;
+}
+
+// ---- low-rank adapters -------------------------------------------------------------------------------
+
+static int check_low_rank(const gq_low_rank_args *p, int64_t *n_total) {
+    if (!p || p->M < 0 || p->M > INT32_MAX || p->K <= 0 || p->K % GQ_QK || p->rank <= 0 || p->rank % 8 || p->n_adapters <= 0) return p ? GQ_ERR_SHAPE : GQ_ERR_ARG;
+    if (p->rank > GQ_MAX_RANK || p->n_shards < 1 || p->n_shards > GQ_MAX_DEVICE_SHARDS) return GQ_ERR_LIMIT;
+    *n_total = 0;
+    for (int s = 0; s < p->n_shards; ++s) {
+        if (p->n_outs[s] < 0 || p->n_outs[s] > INT32_MAX) return GQ_ERR_SHAPE;
+        *n_total += p->n_outs[s];
+    }
+    return *n_total > INT32_MAX ? GQ_ERR_SHAPE : GQ_OK;
+}
+extern "C" int64_t gq_low_rank_workspace_bytes(const gq_low_rank_args *p) {
+    int64_t n = 0;
+    if (const int rc = check_low_rank(p, &n)) return rc;
+    return p->M * p->n_shards * p->rank * 4;
+}
+extern "C" int gq_low_rank_add(const gq_low_rank_args *p, void *stream) {
+    int64_t n = 0;
+    if (const int rc = check_low_rank(p, &n)) return rc;
+    if (p->M == 0 || n == 0) return GQ_OK;
+    if (!p->base || !p->x || !p->a || !p->b || !p->scales || !p->ids || !p->out || (p->ids_bytes != 4 && p->ids_bytes != 8)) return GQ_ERR_ARG;
+    if (!aligned(p->x, 16) || !aligned(p->a, 16) || !aligned(p->b, 16) || p->ldx % 8 || p->ldx < p->K || p->ld_base < n || p->ld_out < n) return GQ_ERR_ARG;
+    if (p->workspace_bytes < gq_low_rank_workspace_bytes(p) || !p->workspace) return GQ_ERR_WORKSPACE;
+    int *status;
+    if (const int rc = status_word(&status)) return rc;
+    LowRankParams q{(const __nv_bfloat16 *)p->base, (const __nv_bfloat16 *)p->x, (const __nv_bfloat16 *)p->a, (const __nv_bfloat16 *)p->b, p->scales, p->ids,
+                    (__nv_bfloat16 *)p->out, (float *)p->workspace, p->K, p->ld_base, p->ldx, p->ld_out, n, {0},
+                    (int)p->M, p->n_shards, p->n_adapters, p->rank, p->ids_bytes == 8};
+    for (int s = 0; s < p->n_shards; ++s) q.edges[s + 1] = q.edges[s] + p->n_outs[s];
+    const int64_t values = p->M * p->n_shards * p->rank;
+    low_rank_inner_kernel<<<(unsigned)((values + 7) / 8), 256, 0, (cudaStream_t)stream>>>(q);
+    GQ_LAUNCHED();
+    low_rank_outer_kernel<<<dim3((unsigned)p->M, (unsigned)((n + 255) / 256)), 256, 0, (cudaStream_t)stream>>>(q, status);
+    GQ_LAUNCHED();
+    return GQ_OK;
+}
+
+// ---- norms and rotation of heads ---------------------------------------------------------------------
+
+extern "C" int gq_head_norm_rope(const gq_head_norm_args *p, void *stream) {
+    if (!p) return GQ_ERR_ARG;
+    const bool store = p->k_pages || p->v_pages;
+    if (p->T < 0 || p->T > INT32_MAX || p->n_heads < 1 || p->n_kv_heads < 1 || p->head_dim < 8 || p->head_dim % 8 || p->rotary_dim < 0 || p->rotary_dim % 2 ||
+        p->rotary_dim > p->head_dim) return GQ_ERR_SHAPE;
+    if (p->head_dim > 512 || (int64_t)p->n_heads + 2 * (int64_t)p->n_kv_heads > 65535) return GQ_ERR_LIMIT;
+    if (store && (p->page_size < 1 || p->n_pages < 0)) return GQ_ERR_SHAPE;
+    if (p->T == 0) return GQ_OK;
+    const int64_t width = ((int64_t)p->n_heads * (p->gated ? 2 : 1) + 2 * (int64_t)p->n_kv_heads) * p->head_dim;
+    if (!p->qkv || !p->q_out || !p->positions || (p->rotary_dim && !p->inv_freq) || (p->positions_bytes != 4 && p->positions_bytes != 8) || p->ld_qkv < width) return GQ_ERR_ARG;
+    if (!aligned(p->q_out, 16) || !aligned(p->q_norm, 16) || !aligned(p->k_norm, 16)) return GQ_ERR_ARG;
+    if (store) {
+        if (!p->k_pages || !p->v_pages || !p->slots || (p->slots_bytes != 4 && p->slots_bytes != 8) || p->k_out || !aligned(p->k_pages, 16) || !aligned(p->v_pages, 16)) return GQ_ERR_ARG;
+        for (int i = 0; i < 3; ++i)
+            if (p->k_strides[i] % 8 || p->v_strides[i] % 8) return GQ_ERR_ARG;
+    } else if (!p->k_out || !aligned(p->k_out, 16)) return GQ_ERR_ARG;
+    int *status;
+    if (const int rc = status_word(&status)) return rc;
+    head_norm_kernel<<<dim3((unsigned)p->T, p->n_heads + (store ? 2 : 1) * p->n_kv_heads), 64, 0, (cudaStream_t)stream>>>(*p, status);
+    GQ_LAUNCHED();
+    return GQ_OK;
+}
+
+// ---- attention over pages ----------------------------------------------------------------------------
+
+static int check_attention(const gq_attention_args *p) {
+    if (!p) return GQ_ERR_ARG;
+    if (p->T < 0 || p->T > INT32_MAX || p->n_seqs < 0 || p->n_seqs > INT32_MAX || p->table_width < 0 || p->n_pages < 0 || p->page_size < 1 || p->n_heads < 1 || p->n_kv_heads < 1 ||
+        p->n_heads % p->n_kv_heads || (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)) return GQ_ERR_SHAPE;
+    if (!p->q_starts && p->T && (p->n_seqs == 0 || p->T % p->n_seqs)) return GQ_ERR_SHAPE;
+    if (p->n_heads > 65535) return GQ_ERR_LIMIT;
+    return GQ_OK;
+}
+extern "C" int64_t gq_attention_workspace_bytes(const gq_attention_args *p) {
+    if (const int rc = check_attention(p)) return rc;
+    return 0;
+}
+extern "C" int gq_paged_attention(const gq_attention_args *p, void *stream) {
+    if (const int rc = check_attention(p)) return rc;
+    if (p->T == 0 || p->n_seqs == 0) return GQ_OK;
+    if (!p->q || !p->lens || !p->out || p->ld_table < p->table_width || (p->n_pages && (!p->k_pages || !p->v_pages)) || (p->table_width && !p->page_table)) return GQ_ERR_ARG;
+    if (!aligned(p->q, 16) || !aligned(p->k_pages, 16) || !aligned(p->v_pages, 16)) return GQ_ERR_ARG;
+    for (int i = 0; i < 3; ++i)
+        if (p->k_strides[i] % 8 || p->v_strides[i] % 8 || (i < 2 && p->q_strides[i] % 8)) return GQ_ERR_ARG;
+    int *status;
+    if (const int rc = status_word(&status)) return rc;
+    paged_attention_kernel<<<dim3((unsigned)p->T, p->n_heads), 128, 0, (cudaStream_t)stream>>>(*p, status);
+    GQ_LAUNCHED();
+    return GQ_OK;
+}

@@ -21,6 +21,8 @@
 #include <pybind11/stl.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/core/grad_mode.h>
+#include <cmath>
 #include <string>
 #include <vector>
 #include "../../include/gq_b200.h"
@@ -275,6 +277,264 @@ PyObject *dequantize_rows(py::handle rawh, int64_t type, py::handle idsh, bool b
     return THPVariable_Wrap(std::move(out));
 }
 
+// ---- the operators beside the quantized layers ---------------------------------------------------------
+// Arguments are checked here in full (shapes and types first, then devices and memory), then handed to the C ABI on the current stream of their device.
+
+[[noreturn]] void refuse(const char *op, const std::string &why) {
+    PyErr_SetString(g_error, (std::string(op) + ": " + why).c_str());
+    throw py::error_already_set();
+}
+std::string shape_of(const at::Tensor &t) {
+    std::string s = "[";
+    for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
+    return s + "] " + c10::toString(t.scalar_type());
+}
+// What all tensors of a call have in common: memory of one CUDA device that is what it says, and no gradient to keep
+class Checked {
+  public:
+    explicit Checked(const char *op) : op_(op) {}
+    void need(bool ok, const char *what) const { if (!ok) refuse(op_, what); }
+    void shaped(const at::Tensor &t, at::ScalarType type, std::initializer_list<int64_t> sizes, const char *what) const {      // -1: any size
+        bool ok = t.scalar_type() == type && t.dim() == (int64_t)sizes.size();
+        int64_t i = 0;
+        for (int64_t n : sizes) { ok = ok && (n < 0 || t.size(i) == n); ++i; }
+        if (!ok) refuse(op_, std::string(what) + ", got " + shape_of(t));
+    }
+    void add(const at::Tensor &t) { if (count_ < 16) all_[count_++] = &t; }
+    void devices() const {
+        for (int i = 0; i < count_; ++i) {
+            if (!all_[i]->is_cuda()) refuse(op_, "takes CUDA tensors (there is no CPU path)");
+            if (!plain_tensor(*all_[i])) refuse(op_, "takes tensors that are what their memory says (no negative views, wrappers or transforms)");
+            if (all_[i]->get_device() != all_[0]->get_device()) refuse(op_, "takes tensors of one device");
+            if (all_[i]->requires_grad() && at::GradMode::is_enabled()) refuse(op_, "has no backward pass: call it under torch.no_grad(), or detach its inputs");
+        }
+        if (!plain_thread()) refuse(op_, "was called inside a torch mode or function transform");
+    }
+  private:
+    const char *op_;
+    const at::Tensor *all_[16];
+    int count_ = 0;
+};
+inline bool on16(const at::Tensor &t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+// elements from a tensor's first to behind its last
+inline int64_t extent(const at::Tensor &t) {
+    int64_t n = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) { if (t.size(i) == 0) return 0; n += (t.size(i) - 1) * t.stride(i); }
+    return n;
+}
+// whether two tensors' ranges of memory meet; of rows with unit stride, whether the rows do
+bool meet(const at::Tensor &u, const at::Tensor &v) {
+    const char *a = (const char *)u.data_ptr(), *b = (const char *)v.data_ptr();
+    const int64_t na = extent(u) * u.element_size(), nb = extent(v) * v.element_size();
+    if (na == 0 || nb == 0 || a + na <= b || b + nb <= a) return false;
+    if (u.dim() == 2 && v.dim() == 2 && u.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16 && u.size(1) == v.size(1) && u.size(0) > 1 && v.size(0) > 1 &&
+        u.stride(0) >= u.size(1) && v.stride(0) >= v.size(1))
+        return may_overlap(a, u.size(0), u.stride(0), b, v.size(0), v.stride(0), u.size(1));
+    return true;
+}
+// rows that start at multiples of 16 bytes: the tensor itself, or a copy
+at::Tensor rows16(const at::Tensor &t) {
+    bool ok = t.stride(-1) == 1 && on16(t);
+    for (int64_t i = 0; ok && i + 1 < t.dim(); ++i) ok = t.size(i) == 1 || (t.stride(i) % 8 == 0 && t.stride(i) >= t.size(-1));
+    return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+// elements between rows; one row has none, and any number will do
+inline int64_t row_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+inline int id_bytes(const at::Tensor &t) { return t.scalar_type() == at::kLong ? 8 : 4; }
+inline bool integers(const at::Tensor &t) { return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt; }
+// scratch of a call: from torch's allocator, on the current stream
+c10::DataPtr scratch(int64_t bytes) { return bytes > 0 ? c10::cuda::CUDACachingAllocator::get()->allocate((size_t)bytes) : c10::DataPtr(); }
+
+at::Tensor low_rank_add(const at::Tensor &base0, const at::Tensor &x0, const at::Tensor &a, const at::Tensor &b, const at::Tensor &scales, const at::Tensor &ids0,
+                        const std::vector<int64_t> &n_outs, c10::optional<at::Tensor> out0) {
+    Checked c("low_rank_add");
+    gq_low_rank_args p{};
+    c.need(!n_outs.empty() && n_outs.size() <= GQ_MAX_DEVICE_SHARDS, "n_outs names one to eight shards");
+    int64_t n = 0;
+    for (size_t s = 0; s < n_outs.size(); ++s) { c.need(n_outs[s] >= 0, "n_outs holds the columns of each shard"); n += p.n_outs[s] = n_outs[s]; }
+    c.shaped(x0, at::kBFloat16, {-1, -1}, "x is bf16 [M, K]");
+    const int64_t m = x0.size(0), k = x0.size(1), shards = (int64_t)n_outs.size();
+    c.need(k > 0 && k % 256 == 0, "K is a multiple of 256");
+    c.shaped(base0, at::kBFloat16, {m, n}, "base is bf16 [M, sum(n_outs)]");
+    c.shaped(b, at::kBFloat16, {-1, n, -1}, "b is bf16 [adapters, sum(n_outs), rank]");
+    const int64_t bank = b.size(0), rank = b.size(2);
+    c.need(bank > 0 && rank > 0 && rank % 8 == 0 && rank <= GQ_MAX_RANK, "the rank is a multiple of 8 up to 128, of one adapter or more");
+    c.shaped(a, at::kBFloat16, {bank, shards * rank, k}, "a is bf16 [adapters, shards * rank, K]");
+    c.shaped(scales, at::kFloat, {bank, shards}, "scales is float32 [adapters, shards]");
+    c.need(ids0.dim() == 1 && ids0.size(0) == m && integers(ids0), "ids is int32 or int64 [M]");
+    c.need(a.is_contiguous() && b.is_contiguous() && scales.is_contiguous(), "a, b and scales are contiguous");
+    if (out0.has_value()) {
+        c.shaped(*out0, at::kBFloat16, {m, n}, "out is bf16 [M, sum(n_outs)]");
+        c.need(m == 0 || n == 0 || (out0->stride(1) == 1 && (m == 1 || out0->stride(0) >= n)), "out has unit column stride and rows of their own");
+    }
+    for (const at::Tensor *t : {&x0, &base0, &a, &b, &scales, &ids0}) c.add(*t);
+    if (out0.has_value()) c.add(*out0);
+    c.devices();
+    c.need(on16(a) && on16(b), "a and b start at multiples of 16 bytes");
+    if (out0.has_value() && m > 0 && n > 0) {
+        const bool in_place = out0->data_ptr() == base0.data_ptr() && base0.stride(1) == 1 && row_stride(*out0) == row_stride(base0);
+        c.need(in_place || !meet(*out0, base0), "out is base itself or shares no memory with it");
+        for (const at::Tensor *t : {&x0, &a, &b, &scales, &ids0}) c.need(!meet(*out0, *t), "out shares no memory with an input other than base");
+    }
+    Status status;
+    at::Tensor out;
+    {
+        py::gil_scoped_release unlocked;
+        c10::cuda::CUDAGuard guard((c10::DeviceIndex)x0.get_device());
+        out = out0.has_value() ? *out0 : at::detail::empty_cuda({m, n}, at::kBFloat16, x0.device(), c10::nullopt);
+        if (m > 0 && n > 0) {
+            const at::Tensor x = rows16(x0), ids = ids0.contiguous(), base = base0.stride(1) == 1 && (m == 1 || base0.stride(0) >= n) ? base0 : base0.contiguous();
+            p.base = base.data_ptr(); p.x = x.data_ptr(); p.a = a.data_ptr(); p.b = b.data_ptr(); p.scales = (const float *)scales.data_ptr();
+            p.ids = ids.data_ptr(); p.out = out.data_ptr(); p.M = m; p.K = k; p.ld_base = row_stride(base); p.ldx = row_stride(x); p.ld_out = row_stride(out);
+            p.n_shards = (int)shards; p.n_adapters = (int)bank; p.rank = (int)rank; p.ids_bytes = id_bytes(ids);
+            p.workspace_bytes = gq_low_rank_workspace_bytes(&p);
+            const c10::DataPtr ws = scratch(p.workspace_bytes);
+            p.workspace = ws.get();
+            status = p.workspace_bytes < 0 ? Status{p.workspace_bytes, "gq_low_rank_workspace_bytes"} : Status{gq_low_rank_add(&p, stream_of(x)), "gq_low_rank_add"};
+        }
+    }
+    status.check();
+    return out;
+}
+
+// the pages of a cache, [pages, rows, kv heads, head_dim] by strides
+void take_pages(const Checked &c, const at::Tensor &t, int64_t kv_heads, int64_t dim, const char *what, int64_t (&strides)[3]) {
+    c.shaped(t, at::kBFloat16, {-1, -1, kv_heads, dim}, what);
+    c.need(t.size(1) > 0, "a page holds one row or more");
+    c.need(t.numel() == 0 || t.stride(3) == 1, "the pages' head_dim has unit stride");
+    for (int i = 0; i < 3; ++i) {
+        c.need(t.size(i) <= 1 || (t.stride(i) % 8 == 0 && t.stride(i) >= dim), "the pages' rows and heads start at multiples of 16 bytes, each in memory of its own");
+        strides[i] = t.size(i) > 1 ? t.stride(i) : 0;
+    }
+}
+
+py::object qk_norm_rope(const at::Tensor &qkv0, const at::Tensor &positions0, const at::Tensor &inv_freq, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                        c10::optional<at::Tensor> q_norm, c10::optional<at::Tensor> k_norm, double eps, double amplitude, bool interleaved, bool gated,
+                        c10::optional<at::Tensor> k_pages, c10::optional<at::Tensor> v_pages, c10::optional<at::Tensor> slots0) {
+    const bool store = k_pages.has_value();
+    Checked c(store ? "qk_norm_rope_store" : "qk_norm_rope");
+    gq_head_norm_args p{};
+    c.need(n_heads > 0 && n_kv_heads > 0 && n_heads <= 16384 && n_kv_heads <= 16384, "one or more heads of queries and of keys");
+    c.need(head_dim >= 8 && head_dim % 8 == 0 && head_dim <= 512, "head_dim is a multiple of 8 up to 512");
+    const int64_t width = (n_heads * (gated ? 2 : 1) + 2 * n_kv_heads) * head_dim;
+    c.shaped(qkv0, at::kBFloat16, {-1, width}, "qkv is bf16 [T, all heads of q (each with its gate if gated), k and v]");
+    const int64_t t = qkv0.size(0);
+    c.need(positions0.dim() == 1 && positions0.size(0) == t && integers(positions0), "positions is int32 or int64 [T]");
+    c.shaped(inv_freq, at::kDouble, {-1}, "inv_freq is float64 [rotary_dim / 2]");
+    c.need(inv_freq.is_contiguous() && 2 * inv_freq.numel() <= head_dim, "inv_freq is contiguous, of at most head_dim / 2 values");
+    for (auto *w : {&q_norm, &k_norm})
+        if (w->has_value()) {
+            c.shaped(**w, at::kBFloat16, {head_dim}, "a norm weight is bf16 [head_dim]");
+            c.need((*w)->is_contiguous(), "a norm weight is contiguous");
+        }
+    if (store) {
+        take_pages(c, *k_pages, n_kv_heads, head_dim, "k_pages is bf16 [pages, rows, kv heads, head_dim]", p.k_strides);
+        take_pages(c, *v_pages, n_kv_heads, head_dim, "v_pages is bf16 [pages, rows, kv heads, head_dim]", p.v_strides);
+        c.need(k_pages->size(0) == v_pages->size(0) && k_pages->size(1) == v_pages->size(1), "k_pages and v_pages hold the same pages");
+        c.need(slots0->dim() == 1 && slots0->size(0) == t && integers(*slots0), "slots is int32 or int64 [T]");
+    }
+    for (const at::Tensor *x : {&qkv0, &positions0, &inv_freq}) c.add(*x);
+    for (auto *x : {&q_norm, &k_norm, &k_pages, &v_pages, &slots0})
+        if (x->has_value()) c.add(**x);
+    c.devices();
+    if (store) {
+        c.need(on16(*k_pages) && on16(*v_pages), "the pages start at multiples of 16 bytes");
+        for (auto *pages : {&*k_pages, &*v_pages})
+            for (const at::Tensor *x : std::initializer_list<const at::Tensor *>{&qkv0, &positions0, &inv_freq, &*slots0}) c.need(!meet(*pages, *x), "the pages share no memory with the other arguments");
+    }
+    Status status;
+    at::Tensor q, k;
+    {
+        py::gil_scoped_release unlocked;
+        c10::cuda::CUDAGuard guard((c10::DeviceIndex)qkv0.get_device());
+        q = at::detail::empty_cuda({t, n_heads, head_dim}, at::kBFloat16, qkv0.device(), c10::nullopt);
+        if (!store) k = at::detail::empty_cuda({t, n_kv_heads, head_dim}, at::kBFloat16, qkv0.device(), c10::nullopt);
+        if (t > 0) {
+            const at::Tensor qkv = rows16(qkv0), positions = positions0.contiguous(), slots = store ? slots0->contiguous() : at::Tensor();
+            auto weight = [](const c10::optional<at::Tensor> &w) { return !w.has_value() ? at::Tensor() : on16(*w) ? *w : w->clone(); };
+            const at::Tensor wq = weight(q_norm), wk = weight(k_norm);
+            p.qkv = qkv.data_ptr(); p.positions = positions.data_ptr(); p.inv_freq = (const double *)inv_freq.data_ptr();
+            p.q_norm = wq.defined() ? wq.data_ptr() : nullptr; p.k_norm = wk.defined() ? wk.data_ptr() : nullptr;
+            p.q_out = q.data_ptr(); p.k_out = store ? nullptr : k.data_ptr();
+            p.T = t; p.ld_qkv = row_stride(qkv);
+            p.n_heads = (int)n_heads; p.n_kv_heads = (int)n_kv_heads; p.head_dim = (int)head_dim; p.rotary_dim = (int)(2 * inv_freq.numel());
+            p.positions_bytes = id_bytes(positions); p.interleaved = interleaved; p.gated = gated; p.eps = (float)eps; p.amplitude = (float)amplitude;
+            if (store) {
+                p.k_pages = k_pages->data_ptr(); p.v_pages = v_pages->data_ptr(); p.slots = slots.data_ptr(); p.slots_bytes = id_bytes(slots);
+                p.n_pages = k_pages->size(0); p.page_size = (int)k_pages->size(1);
+            }
+            status = {gq_head_norm_rope(&p, stream_of(qkv)), "gq_head_norm_rope"};
+        }
+    }
+    status.check();
+    return store ? py::cast(q) : py::object(py::make_tuple(q, k));
+}
+
+at::Tensor paged_attention(const at::Tensor &q0, const at::Tensor &k_pages, const at::Tensor &v_pages, const at::Tensor &table0, const at::Tensor &lens0,
+                           c10::optional<at::Tensor> q_starts0, c10::optional<double> scale, c10::optional<at::Tensor> gate0, c10::optional<at::Tensor> out0) {
+    Checked c("paged_attention");
+    gq_attention_args p{};
+    c.shaped(q0, at::kBFloat16, {-1, -1, -1}, "q is bf16 [T, heads, head_dim]");
+    const int64_t t = q0.size(0), heads = q0.size(1), dim = q0.size(2);
+    c.need(dim == 64 || dim == 128 || dim == 256, "head_dim is 64, 128 or 256");
+    take_pages(c, k_pages, -1, dim, "k_pages is bf16 [pages, rows, kv heads, head_dim]", p.k_strides);
+    const int64_t kv_heads = k_pages.size(2);
+    take_pages(c, v_pages, kv_heads, dim, "v_pages is bf16 [pages, rows, kv heads, head_dim]", p.v_strides);
+    c.need(k_pages.size(0) == v_pages.size(0) && k_pages.size(1) == v_pages.size(1), "k_pages and v_pages hold the same pages");
+    c.need(heads > 0 && heads <= 65535 && kv_heads > 0 && heads % kv_heads == 0, "the query heads are a multiple of the key-value heads");
+    c.shaped(table0, at::kInt, {-1, -1}, "page_table is int32 [sequences, pages of the longest]");
+    const int64_t seqs = table0.size(0);
+    c.shaped(lens0, at::kInt, {seqs}, "lens is int32 [sequences]");
+    if (q_starts0.has_value()) c.shaped(*q_starts0, at::kInt, {seqs + 1}, "q_starts is int32 [sequences + 1]");
+    else c.need(seqs ? t % seqs == 0 : t == 0, "without q_starts every sequence has the same number of tokens");
+    for (auto *x : {&gate0, &out0})
+        if (x->has_value()) {
+            c.shaped(**x, at::kBFloat16, {t, heads, dim}, x == &gate0 ? "gate is bf16, of q's shape" : "out is bf16, of q's shape");
+            c.need((*x)->numel() == 0 || (*x)->stride(2) == 1, "gate and out have unit stride along head_dim");
+        }
+    if (out0.has_value())
+        c.need((t <= 1 || out0->stride(0) >= dim) && (heads <= 1 || out0->stride(1) >= dim), "out's rows and heads have memory of their own");
+    for (const at::Tensor *x : {&q0, &k_pages, &v_pages, &table0, &lens0}) c.add(*x);
+    for (auto *x : {&q_starts0, &gate0, &out0})
+        if (x->has_value()) c.add(**x);
+    c.devices();
+    c.need(on16(k_pages) && on16(v_pages), "the pages start at multiples of 16 bytes");
+    if (out0.has_value()) {
+        for (const at::Tensor *x : {&q0, &k_pages, &v_pages, &table0, &lens0}) c.need(!meet(*out0, *x), "out shares no memory with an input");
+        for (auto *x : {&q_starts0, &gate0})
+            if (x->has_value()) c.need(!meet(*out0, **x), "out shares no memory with an input");
+    }
+    Status status;
+    at::Tensor out;
+    {
+        py::gil_scoped_release unlocked;
+        c10::cuda::CUDAGuard guard((c10::DeviceIndex)q0.get_device());
+        if (out0.has_value()) out = *out0;
+        else {
+            out = at::detail::empty_cuda({t, heads, dim}, at::kBFloat16, q0.device(), c10::nullopt);
+            if (q_starts0.has_value()) out.zero_();                 // rows behind the last sequence
+        }
+        if (t > 0 && seqs > 0) {
+            const at::Tensor q = rows16(q0), lens = lens0.contiguous(), starts = q_starts0.has_value() ? q_starts0->contiguous() : at::Tensor();
+            const at::Tensor table = table0.size(1) == 0 || (table0.stride(1) == 1 && (seqs == 1 || table0.stride(0) >= table0.size(1))) ? table0 : table0.contiguous();
+            p.q = q.data_ptr(); p.k_pages = k_pages.data_ptr(); p.v_pages = v_pages.data_ptr(); p.page_table = (const int32_t *)table.data_ptr();
+            p.lens = (const int32_t *)lens.data_ptr(); p.q_starts = starts.defined() ? (const int32_t *)starts.data_ptr() : nullptr; p.out = out.data_ptr();
+            p.T = t; p.n_seqs = seqs; p.table_width = table.size(1); p.ld_table = row_stride(table); p.n_pages = k_pages.size(0); p.page_size = (int)k_pages.size(1);
+            p.n_heads = (int)heads; p.n_kv_heads = (int)kv_heads; p.head_dim = (int)dim;
+            p.scale = scale.has_value() ? (float)*scale : 1.0f / std::sqrt((float)dim);
+            auto strides = [](const at::Tensor &x, int64_t (&s)[2]) { for (int i = 0; i < 2; ++i) s[i] = x.size(i) > 1 ? x.stride(i) : 0; };
+            strides(q, p.q_strides); strides(out, p.out_strides);
+            if (gate0.has_value()) { p.gate = gate0->data_ptr(); strides(*gate0, p.gate_strides); }
+            p.workspace_bytes = gq_attention_workspace_bytes(&p);
+            const c10::DataPtr ws = scratch(p.workspace_bytes);
+            p.workspace = ws.get();
+            status = p.workspace_bytes < 0 ? Status{p.workspace_bytes, "gq_attention_workspace_bytes"} : Status{gq_paged_attention(&p, stream_of(q)), "gq_paged_attention"};
+        }
+    }
+    status.check();
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_gq_torch, m) {
@@ -286,6 +546,9 @@ PYBIND11_MODULE(_gq_torch, m) {
     m.def("dequantize_rows", [](py::handle raw, int64_t type, py::handle ids, bool bf16) {
         return py::reinterpret_steal<py::object>(dequantize_rows(raw, type, ids, bf16));
     });
+    m.def("low_rank_add", &low_rank_add);
+    m.def("qk_norm_rope", &qk_norm_rope);
+    m.def("paged_attention", &paged_attention);
     py::class_<Run>(m, "Run")
         .def(py::init<at::Tensor, std::vector<at::Tensor>, std::vector<int64_t>, std::vector<int64_t>, std::vector<int64_t>, int64_t, std::vector<int64_t>,
                       int64_t, int64_t>())

@@ -12,6 +12,7 @@ import contextlib
 
 import ctypes
 import functools
+import math
 from typing import Sequence
 
 import numpy as np
@@ -558,6 +559,89 @@ class NativeRun:
         if pre.kind == 1:
             return self._run.forward_silu_mul(x)
         return self._run.forward_add_rms_norm(x, pre.weight, pre.residual, pre.residual_out, pre.eps)
+
+
+# ---- beside the layers: adapters, norms and rotation of heads, attention over a paged cache ---------------
+#
+# Each is one call of the native extension, on the current stream of its tensors' device, safe to capture in a CUDA graph; arguments are checked
+# in full before anything is launched (GqError).  What only the device can see (an id, a slot, a page outside its range) sets device_status to 2.
+
+MAX_RANK = 128
+
+
+def low_rank_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, ids: torch.Tensor,
+                 n_outs: Sequence[int], *, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Low-rank adapters of many requests beside one (merged) layer: base [M, N] plus, for every row m with an adapter i = ids[m],
+    scales[i, s] * b[i] @ (a[i, s] @ x[m]) in the columns of each shard s.
+
+    x bf16 [M, K], base bf16 [M, N] (the layer's output), a bf16 [adapters, shards * rank, K], b bf16 [adapters, N, rank], scales float32
+    [adapters, shards], ids int32 or int64 [M], n_outs the shards' columns (N in all).  The rank is a multiple of 8 up to 128 (pad with zeros), K of 256.
+    ids[m] = -1: the row has no adapter and is base's.  Any other id outside the bank makes its row NaN and device_status 2.  `out` may be base
+    (in place); it is new memory if left out.  Sums in 32 bits, one rounding; a row's sums hold nothing of other rows' adapters."""
+    return native().low_rank_add(base, x, a, b, scales, ids, [int(n) for n in n_outs], out)
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0, original_context: int | None = None,
+                       beta_fast: float = 32.0, beta_slow: float = 1.0, device="cuda") -> tuple[torch.Tensor, float]:
+    """(inv_freq float64 [rotary_dim / 2], amplitude) for qk_norm_rope, made once per model: radians per position of each rotated pair.
+    `scaling`, the kinds a GGUF file names: None or "none"; "linear", positions divided by `factor`; "yarn", pairs that turn less than beta_slow times over
+    `original_context` tokens divided by `factor`, those above beta_fast kept, a ramp between, and values times 0.1 ln(factor) + 1."""
+    if rotary_dim < 0 or rotary_dim % 2 or base <= 0 or factor <= 0:
+        raise GqError(f"rotary_dim is even, base and factor are positive; got {rotary_dim}, {base}, {factor}")
+    inv = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / max(1, rotary_dim))
+    amplitude = 1.0
+    if scaling == "linear":
+        inv = inv / factor
+    elif scaling == "yarn":
+        if not original_context or original_context <= 0:
+            raise GqError("yarn needs the context the model was trained on")
+        pair = lambda turns: rotary_dim * math.log(original_context / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+        low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rotary_dim - 1)
+        kept = 1 - ((torch.arange(inv.numel(), dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)
+        inv = inv / factor * (1 - kept) + inv * kept
+        amplitude = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    elif scaling not in (None, "none"):
+        raise GqError(f"unknown rotary scaling {scaling!r}")
+    return inv.to(device), amplitude
+
+
+def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, *,
+                 q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, eps: float = 1e-6, amplitude: float = 1.0,
+                 interleaved: bool = False, gated: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rows of a merged qkv layer -> (q [T, n_heads, head_dim], k [T, n_kv_heads, head_dim]): RMS norm of every head (weights bf16
+    [head_dim]; None: no norm) and the rotation by the token's position, in one pass and one rounding.
+
+    The first 2 * len(inv_freq) dimensions of a head turn, as pairs half of them apart or, `interleaved`, side by side; inv_freq (float64) and amplitude as
+    rotary_frequencies makes them; angles are reduced in 64 bits.  positions int32 or int64 [T].  `gated`: every query head is followed
+    by an output gate of head_dim values, which stays where it is (paged_attention takes it)."""
+    return native().qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated, None, None, None)
+
+
+def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
+                       k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor, *, q_norm: torch.Tensor | None = None,
+                       k_norm: torch.Tensor | None = None, eps: float = 1e-6, amplitude: float = 1.0, interleaved: bool = False,
+                       gated: bool = False) -> torch.Tensor:
+    """qk_norm_rope, with keys and values written to the pages of a cache in the same pass; returns q.
+
+    k_pages, v_pages bf16 [pages, rows, n_kv_heads, head_dim] by strides; token t goes to slot slots[t] (int32 or int64) = page * rows + row.  A negative
+    slot stores nothing (padding); one beyond the cache stores nothing and makes device_status 2.  Of two tokens with one slot either may be kept."""
+    return native().qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated,
+                                 k_pages, v_pages, slots)
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, *,
+                    q_starts: torch.Tensor | None = None, scale: float | None = None, gate: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the newest tokens of every sequence (one in decode, a few in verification) over a paged key-value cache that
+    holds them already: q bf16 [T, heads, head_dim] -> the same shape.  Sequence s has lens[s] (int32) keys, key j in row j % rows of page
+    page_table[s, j // rows] (int32 [sequences, pages]); the i-th of its n tokens sees the keys up to lens[s] - n + i.  A token that sees none: zeros.
+
+    k_pages, v_pages bf16 [pages, rows, kv_heads, head_dim] by strides, head_dim 64, 128 or 256, heads a multiple of kv_heads.  q_starts (int32 [sequences + 1]):
+    the first token of each sequence, for batches of uneven numbers of tokens; rows behind the last sequence stay as they are in `out` (zeros without one).
+    scale: head_dim ** -0.5 if left out.  gate (q's shape, any strides over tokens and heads): the result is multiplied by sigmoid(gate).
+    A page outside the cache or a length beyond the table: NaN in the rows that see it, and device_status 2.  Probabilities, sums and the join of the
+    cache's parts in 32 bits, one rounding; the order of the sums does not depend on timing."""
+    return native().paged_attention(q, k_pages, v_pages, page_table, lens, q_starts, scale, gate, out)
 
 
 # ---- torch custom op (traceable boundary) ----------------------------------------------------------

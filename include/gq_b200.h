@@ -275,6 +275,84 @@ int gq_gemm_prefill(const void *x_dev, int64_t M, int64_t K, int64_t ldx, const 
                     int64_t n_desc, int run_info, void *y_dev, int64_t ldy, int64_t n_total, void *workspace_dev,
                     int64_t workspace_bytes, void *stream);
 
+/* ---- the operators beside the quantized layers of a decoder block ------------------------------------
+ * bf16 tensors, sums and statistics in 32 bits, one rounding at the end.  Each call takes its arguments in a struct; nothing is written
+ * before all of them have been checked (< 0: nothing was launched).  Reference: none — the reference leaves these steps to the engine
+ * around its linear method. */
+
+/* Low-rank adapters of many requests beside one (merged) layer, any number of rows:
+ *   out[m, n] = base[m, n] + scales[i, s] * sum_r b[i, n, r] * (sum_k a[i, s * rank + r, k] * x[m, k]),  i = ids[m], s the shard of column n
+ * ids[m] = -1: no adapter, out[m] = base[m].  Any other id outside the bank: out[m] is NaN and the device status becomes 2.  Rows of other
+ * adapters never enter a row's sums.  K is a multiple of 256, rank a multiple of 8 up to GQ_MAX_RANK, one to GQ_MAX_DEVICE_SHARDS shards.  a, b and x
+ * 16-byte aligned, ldx a multiple of 8; base and out start anywhere, and out may be base (in place), else it shares no memory with an input. */
+#define GQ_MAX_RANK 128
+typedef struct gq_low_rank_args {
+    const void *base;            /* bf16 [M, n_total], row stride ld_base elements */
+    const void *x;               /* bf16 [M, K], row stride ldx */
+    const void *a;               /* bf16 [n_adapters, n_shards * rank, K] */
+    const void *b;               /* bf16 [n_adapters, n_total, rank] */
+    const float *scales;         /* [n_adapters, n_shards] */
+    const void *ids;             /* int32 or int64 [M] */
+    void *out;                   /* bf16 [M, n_total], row stride ld_out */
+    int64_t M, K, ld_base, ldx, ld_out;
+    int64_t n_outs[8];           /* columns of each shard; their sum is n_total */
+    int32_t n_shards, n_adapters, rank, ids_bytes;
+    void *workspace;             /* gq_low_rank_workspace_bytes(args) bytes, 256-byte aligned; null if that is 0 */
+    int64_t workspace_bytes;
+} gq_low_rank_args;
+int64_t gq_low_rank_workspace_bytes(const gq_low_rank_args *args);
+int gq_low_rank_add(const gq_low_rank_args *args, void *stream);
+
+/* RMS norm of every query and key head and the rotation by the token's position, in one pass over the rows that a merged q / k / v layer
+ * wrote; with pages given, keys and values go to the cache in the same pass.
+ *   u = x * rsqrt(mean(x^2) + eps) * weight       (weight null: u = x)
+ *   (u_i, u_j) -> amplitude * (u_i cos f - u_j sin f, u_j cos f + u_i sin f),  f = position * inv_freq[p], for the pairs p of the first
+ *   rotary_dim dimensions: (p, p + rotary_dim / 2), or (2 p, 2 p + 1) if interleaved; the others are left as u.
+ * The angle is reduced in 64 bits, so positions may be large.  qkv holds n_heads heads of queries (each followed by a gate of the same
+ * size if gated: it is left alone), n_kv_heads of keys, n_kv_heads of values.  head_dim is a multiple of 8 up to 512, rotary_dim even (0: no rotation).
+ * A negative slot stores nothing; one beyond the cache stores nothing and sets device status 2.  Two tokens of one slot: either may be kept.
+ * out and the pages share no memory with qkv; pages and their strides start at multiples of 16 bytes. */
+typedef struct gq_head_norm_args {
+    const void *qkv;             /* bf16 [T, n_heads * head_dim * (gated ? 2 : 1) + 2 * n_kv_heads * head_dim], row stride ld_qkv */
+    const void *positions;       /* int32 or int64 [T] */
+    const double *inv_freq;      /* [rotary_dim / 2], radians per position */
+    const void *q_norm, *k_norm; /* bf16 [head_dim] or null */
+    void *q_out;                 /* bf16 [T, n_heads, head_dim], contiguous */
+    void *k_out;                 /* the same for keys, or null where pages are given */
+    void *k_pages, *v_pages;     /* bf16 [n_pages, page_size, n_kv_heads, head_dim] by strides, or null */
+    const void *slots;           /* int32 or int64 [T]: page * page_size + row */
+    int64_t T, ld_qkv, n_pages;
+    int64_t k_strides[3], v_strides[3];     /* elements between pages, rows, heads */
+    int32_t n_heads, n_kv_heads, head_dim, rotary_dim, page_size, positions_bytes, slots_bytes, interleaved, gated;
+    float eps, amplitude;
+} gq_head_norm_args;
+int gq_head_norm_rope(const gq_head_norm_args *args, void *stream);
+
+/* Attention of the newest tokens of n_seqs sequences over a paged key-value cache that holds them already:
+ *   o = sum_j softmax_j(scale * q . k_j) v_j over the keys j <= lens[s] - n + i of sequence s for the i-th of its n tokens,  o *= sigmoid(gate)
+ * A token that sees no key: zeros.  Tokens of sequence s are q_starts[s] .. q_starts[s + 1] - 1 (null: T / n_seqs each); rows behind the last
+ * sequence are left as they were.  Key j stands in row j % page_size of page page_table[s, j / page_size].  A page outside the cache, or a length beyond the table: the
+ * rows that see it are NaN and the device status becomes 2.  head_dim 64, 128 or 256; n_heads a multiple of n_kv_heads; every row, head and page starts
+ * at a multiple of 16 bytes (gate, and out: of 2).  out shares no memory with an input. */
+typedef struct gq_attention_args {
+    const void *q;               /* bf16 [T, n_heads, head_dim] by strides */
+    const void *k_pages, *v_pages;
+    const int32_t *page_table;   /* [n_seqs, table_width], row stride ld_table */
+    const int32_t *lens;         /* [n_seqs]: keys of the sequence, its new tokens' among them */
+    const int32_t *q_starts;     /* [n_seqs + 1] or null */
+    const void *gate;            /* as q, by strides of its own, or null */
+    void *out;                   /* as q, by strides of its own */
+    int64_t T, n_seqs, table_width, ld_table, n_pages;
+    int64_t q_strides[2], gate_strides[2], out_strides[2];      /* elements between tokens, heads */
+    int64_t k_strides[3], v_strides[3];                         /* elements between pages, rows, heads */
+    int32_t n_heads, n_kv_heads, head_dim, page_size;
+    float scale;
+    void *workspace;             /* gq_attention_workspace_bytes(args) bytes, 256-byte aligned; null if that is 0 */
+    int64_t workspace_bytes;
+} gq_attention_args;
+int64_t gq_attention_workspace_bytes(const gq_attention_args *args);
+int gq_paged_attention(const gq_attention_args *args, void *stream);
+
 /* Reads the device status word of the last call on this workspace (synchronises the stream): 0, or
  * a positive GQ_DEV_* code (1: a bounded wait ran out; 2: a shape or a tile's type contradicts the call's arguments —
  * an odd column count in the fused all-reduce, or a tile of a type that run_info leaves out and for which the call has no kernel (up to
