@@ -1,6 +1,7 @@
 // The operators beside the quantized layers of a decoder block: low-rank adapters of many requests beside a layer, norms and rotation of
 // queries and keys with the store into a paged cache, attention over that cache.  C ABI in include/gq_b200.h.
 #include <cuda_runtime.h>
+#include <atomic>
 #include <stdint.h>
 #include "gq_host.h"
 #include "gq_adapters.cuh"
@@ -97,9 +98,72 @@ static int check_attention(const gq_attention_args *p) {
     if (p->n_heads > 65535) return GQ_ERR_LIMIT;
     return GQ_OK;
 }
+static int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
+
+// Launches a kernel that begins with griddepcontrol.wait while the kernel in front of it ends.
+template <class... P, class... A> static cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, int smem, void *stream, A... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t)stream; cfg.attrs = &attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// blocks of a kernel that the current device holds at once; its shared memory is allowed on the way (asked once per device)
+template <auto KERNEL> static int resident_blocks(int threads, int smem, int *blocks) {
+    static std::atomic<int> known[64];
+    int dev = 0, sms = 0, per_sm = 0;
+    GQ_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && (*blocks = known[dev].load(std::memory_order_acquire))) return GQ_OK;
+    GQ_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    GQ_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    GQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, KERNEL, threads, smem));
+    *blocks = sms * (per_sm < 1 ? 1 : per_sm);
+    if (dev < 64) known[dev].store(*blocks, std::memory_order_release);
+    return GQ_OK;
+}
+
+// rows of a tile: those of a sequence's tokens under one kv head, as far as the batch's average tells
+static int row_groups(const gq_attention_args *p) {
+    const int64_t tokens = p->n_seqs ? (p->T + p->n_seqs - 1) / p->n_seqs : 1, rows = tokens * (p->n_heads / p->n_kv_heads);
+    return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+}
+template <int D, int RG> static int attention(const gq_attention_args *p, int64_t *bytes, int *status, void *stream) {
+    using Shape = PagedShape<D, RG>;
+    int blocks = 0;
+    if (const int rc = resident_blocks<paged_attention_kernel<D, RG>>(PA_THREADS, Shape::SMEM, &blocks)) return rc;
+    const int64_t slots = 2 * (int64_t)blocks * Shape::ROWS, at_stats = up256((p->n_seqs + 1) * 8), at_parts = at_stats + up256(slots * 8);
+    *bytes = at_parts + slots * D * 4;
+    if (!status) return GQ_OK;
+    if (!p->workspace || !aligned(p->workspace, 256) || p->workspace_bytes < *bytes) return GQ_ERR_WORKSPACE;
+    uint8_t *ws = (uint8_t *)p->workspace;
+    PagedParams q{*p, status, (int64_t *)ws, (float2 *)(ws + at_stats), (float *)(ws + at_parts), p->n_heads / p->n_kv_heads, blocks, p->scale * 1.4426950408889634f};
+    if (p->n_pages == 0) {       // every page is outside the cache: nothing is read, but addresses are formed
+        q.a.k_pages = q.a.v_pages = p->q;
+        for (int i = 0; i < 3; ++i) q.a.k_strides[i] = q.a.v_strides[i] = 0;
+    }
+    GQ_CUDA(launch_pdl(paged_attention_kernel<D, RG>, dim3(blocks), PA_THREADS, Shape::SMEM, stream, q));
+    GQ_LAUNCHED();
+    GQ_CUDA(launch_pdl(join_parts_kernel<D>, dim3((unsigned)p->T, p->n_heads), 128, 0, stream, q, Shape::ROWS, Shape::UNIT));
+    GQ_LAUNCHED();
+    return GQ_OK;
+}
+static int attention_by_shape(const gq_attention_args *p, int64_t *bytes, int *status, void *stream) {
+    const int rg = row_groups(p);
+#define GQ_HEAD(D) return rg == 1 ? attention<D, 1>(p, bytes, status, stream) : rg == 2 ? attention<D, 2>(p, bytes, status, stream) : attention<D, 4>(p, bytes, status, stream)
+    if (p->head_dim == 64) GQ_HEAD(64);
+    if (p->head_dim == 128) GQ_HEAD(128);
+    GQ_HEAD(256);
+#undef GQ_HEAD
+}
+
 extern "C" int64_t gq_attention_workspace_bytes(const gq_attention_args *p) {
+    int64_t bytes = 0;
     if (const int rc = check_attention(p)) return rc;
-    return 0;
+    if (p->T == 0 || p->n_seqs == 0) return 0;
+    const int rc = attention_by_shape(p, &bytes, nullptr, nullptr);
+    return rc ? rc : bytes;
 }
 extern "C" int gq_paged_attention(const gq_attention_args *p, void *stream) {
     if (const int rc = check_attention(p)) return rc;
@@ -110,7 +174,6 @@ extern "C" int gq_paged_attention(const gq_attention_args *p, void *stream) {
         if (p->k_strides[i] % 8 || p->v_strides[i] % 8 || (i < 2 && p->q_strides[i] % 8)) return GQ_ERR_ARG;
     int *status;
     if (const int rc = status_word(&status)) return rc;
-    paged_attention_kernel<<<dim3((unsigned)p->T, p->n_heads), 128, 0, (cudaStream_t)stream>>>(*p, status);
-    GQ_LAUNCHED();
-    return GQ_OK;
+    int64_t bytes;
+    return attention_by_shape(p, &bytes, status, stream);
 }
