@@ -17,18 +17,19 @@
 
 namespace gq {
 
-constexpr int PA_THREADS = 128, PA_STAGES = 3;
-
 struct PagedParams {
     gq_attention_args a;
     int *status;
     int64_t *first;         // workspace: [n_seqs] first unit of each sequence, then W
     float2 *stats;          // [2 G][rows of a tile]: maximum, sum
     float *parts;           // [2 G][rows of a tile][head_dim]
-    int group, blocks;
+    int group, blocks, max_keys;        // query heads of a kv head; blocks the GPU holds; keys that the page table has room for
+    uint32_t page_mul, page_shift;      // key / page_size = key * page_mul >> page_shift, for keys below 2^31
     float scale2;           // scale * log2 e
 };
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+// the same, or 16 zeros
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
@@ -62,12 +63,20 @@ __device__ __forceinline__ void bf16_parts(float lo, float hi, uint32_t &big, ui
     small = bf16_pair(lo - __uint_as_float(big << 16), hi - __uint_as_float(big & 0xffff0000u));
 }
 
+// an 8 x 8 tile of 16-bit values, a row to four lanes, turned over
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
 // A sequence's tokens and keys, and how its rows and keys are cut
 struct SeqSpan {
     int64_t tok0;     // its first token
     int n, len;       // new tokens, keys
 };
-__device__ __forceinline__ SeqSpan seq_span(const gq_attention_args &a, int64_t s) {
+__device__ __forceinline__ SeqSpan seq_span(const PagedParams &p, int64_t s) {
+    const gq_attention_args &a = p.a;
     SeqSpan v;
     if (a.q_starts) {
         const int64_t q0 = min(max((int64_t)a.q_starts[s], (int64_t)0), a.T), q1 = min(max((int64_t)a.q_starts[s + 1], q0), a.T);
@@ -75,7 +84,7 @@ __device__ __forceinline__ SeqSpan seq_span(const gq_attention_args &a, int64_t 
     } else {
         v.n = (int)(a.T / a.n_seqs); v.tok0 = s * v.n;
     }
-    v.len = max(a.lens[s], 0);
+    v.len = min(max(a.lens[s], 0), p.max_keys + v.n);      // with more keys than the table has, every token sees a missing one
     return v;
 }
 // keys that a tile's last row sees
@@ -110,7 +119,7 @@ template <int ROWS, int UNIT> __device__ __forceinline__ void next_segment(const
                 c.head = 0;
                 do {
                     if (++c.seq >= p.a.n_seqs) { c.units = 0; return; }
-                    c.v = seq_span(p.a, c.seq);
+                    c.v = seq_span(p, c.seq);
                     c.tiles = tiles_of(c.v, ROWS, p.group);
                 } while (c.tiles == 0);
             }
@@ -119,24 +128,24 @@ template <int ROWS, int UNIT> __device__ __forceinline__ void next_segment(const
     } while (c.units == 0);
 }
 
-template <int D, int RG> struct PagedShape {
-    static constexpr int KG = 4 / RG, ROWS = 16 * RG, UNIT = 16 * KG;
-    static constexpr int STAGE = 2 * 16 * D * 2;                                // keys and values of 16 keys, bytes
-    static constexpr int RING = KG * PA_STAGES * STAGE, Q = D > 128 ? ROWS * D * 2 : 0, MERGE = KG > 1 ? ROWS * D * 4 : 0;
-    static constexpr int SMEM = RING + Q + MERGE + (KG > 1 ? KG * ROWS * 8 : 0) + KG * PA_STAGES * 4 + 128;
+template <int D, int RG, int KG, int S> struct PagedShape {
+    static constexpr int THREADS = 32 * RG * KG, ROWS = 8 * RG, UNIT = 16 * KG;
+    static constexpr int PITCH = D * 2 + 16;                                    // bytes of a row in shared memory: eight rows' chunks in different banks
+    static constexpr int STAGE = 2 * 16 * PITCH;                                // keys and values of 16 keys
+    static constexpr int RING = KG * S * STAGE, MERGE = KG > 1 ? ROWS * D * 4 : 0, STATS = KG > 1 ? KG * ROWS * 8 : 0;
+    static constexpr int SMEM = RING + MERGE + STATS + RG * KG * 256 + KG * S * 4;
 };
 
-template <int D, int RG>
-__global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __grid_constant__ PagedParams p) {
-    using Shape = PagedShape<D, RG>;
-    constexpr int KG = Shape::KG, ROWS = Shape::ROWS, UNIT = Shape::UNIT, STAGE = Shape::STAGE, S = PA_STAGES, CH = D / 8, NT = D / 8, KK = D / 16;
-    constexpr bool QREG = D <= 128;
+template <int D, int RG, int KG, int S>
+__global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __grid_constant__ PagedParams p) {
+    using Shape = PagedShape<D, RG, KG, S>;
+    constexpr int ROWS = Shape::ROWS, UNIT = Shape::UNIT, STAGE = Shape::STAGE, PITCH = Shape::PITCH, CH = D / 8, MT = D / 16, WARPS = RG * KG;
     extern __shared__ __align__(128) uint8_t smem[];
-    uint8_t *q_sm = smem + Shape::RING;
-    float *merge = (float *)(q_sm + Shape::Q);
+    float *merge = (float *)(smem + Shape::RING);
     float2 *stat_sm = (float2 *)((uint8_t *)merge + Shape::MERGE);
-    uint32_t *bad_sm = (uint32_t *)((uint8_t *)stat_sm + (KG > 1 ? KG * ROWS * 8 : 0));
-    __shared__ int64_t scan[PA_THREADS / 32], place[3];
+    longlong2 *row_sm = (longlong2 *)((uint8_t *)stat_sm + Shape::STATS);       // [warp][16]: where the keys and values of the stage being asked for start
+    uint32_t *bad_sm = (uint32_t *)(row_sm + 16 * WARPS);                      // [KG][S]: a stage's keys whose page is missing
+    __shared__ int64_t scan[WARPS], place[3];
     const gq_attention_args &a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, rg = warp % RG, kg = warp / RG, g = lane / 4, t = lane % 4;
     pdl_wait();
@@ -146,9 +155,9 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
     int64_t total, w0, w1;
     Cursor use;
     {
-        const int64_t each = (a.n_seqs + PA_THREADS - 1) / PA_THREADS, s0 = min(tid * each, a.n_seqs), s1 = min(s0 + each, a.n_seqs);
+        const int64_t each = (a.n_seqs + Shape::THREADS - 1) / Shape::THREADS, s0 = min(tid * each, a.n_seqs), s1 = min(s0 + each, a.n_seqs);
         int64_t mine = 0;
-        for (int64_t s = s0; s < s1; ++s) mine += head_units(seq_span(a, s), ROWS, p.group, UNIT) * a.n_kv_heads;
+        for (int64_t s = s0; s < s1; ++s) mine += head_units(seq_span(p, s), ROWS, p.group, UNIT) * a.n_kv_heads;
         int64_t upto = mine;
         for (int o = 1; o < 32; o *= 2) {
             const int64_t v = __shfl_up_sync(~0u, upto, o);
@@ -157,7 +166,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
         if (lane == 31) scan[warp] = upto;
         __syncthreads();
         total = 0;
-        for (int w = 0; w < PA_THREADS / 32; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             if (w < warp) upto += scan[w];
             total += scan[w];
         }
@@ -167,7 +176,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
         int64_t at = upto - mine;
         if (blockIdx.x == 0 || (w0 < w1 && w0 >= at && w0 < upto))
             for (int64_t s = s0; s < s1; ++s) {
-                const int64_t u = head_units(seq_span(a, s), ROWS, p.group, UNIT);
+                const int64_t u = head_units(seq_span(p, s), ROWS, p.group, UNIT);
                 if (blockIdx.x == 0) p.first[s] = at;
                 if (w0 < w1 && w0 >= at && w0 < at + u * a.n_kv_heads) { place[0] = s; place[1] = (w0 - at) / u; place[2] = (w0 - at) % u; }
                 at += u * a.n_kv_heads;
@@ -178,7 +187,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
         use.seq = place[0];
         use.head = (int)place[1];
         int64_t in = place[2];
-        use.v = seq_span(a, use.seq);
+        use.v = seq_span(p, use.seq);
         use.tiles = tiles_of(use.v, ROWS, p.group);
         use.tile = 0;
         load_segment<ROWS, UNIT>(p, use);
@@ -187,7 +196,7 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
     }
     const int64_t count = w1 - w0;
 
-    // ---- loads: a stage of this key group is 16 keys, whose rows lane l & 15 finds ----
+    // ---- loads: a stage of this key group is 16 keys; lane l finds key l & 15, then all lanes copy 16 bytes of each pair of rows ----
     const uint32_t ring = smem_u32(smem) + kg * S * STAGE;
     Cursor get = use;
     int64_t got = 0;
@@ -196,31 +205,44 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
     auto look = [&]() {             // the page of the stage at `get`
         const int key = (get.unit * KG + kg) * 16 + (lane & 15);
         key_ok = got < count && key < get.keys;
-        pos = key / a.page_size;
-        page_ok = key_ok && pos < a.table_width;
-        page = page_ok ? a.page_table[get.seq * a.ld_table + pos] : 0;
-        pos = key - pos * a.page_size;
+        const int at = (int)((uint64_t)(uint32_t)key * p.page_mul >> p.page_shift);
+        page_ok = key_ok && at < a.table_width;
+        page = page_ok ? a.page_table[get.seq * a.ld_table + at] : 0;
+        pos = key - at * a.page_size;
     };
+    longlong2 *rows_at = row_sm + warp * 16;
+    constexpr int PER = 32 / CH, COPIES = 16 * CH / 32;        // rows that 32 lanes copy at once, turns for a stage
+    const int copy_row = lane / CH, copy_c = lane % CH;
     auto ask = [&](int slot) {      // copies the stage that look() has seen, then looks at the next
         if (got < count) {
             const bool ok = page_ok && page >= 0 && page < a.n_pages;
-            const uint32_t bad = __ballot_sync(~0u, key_ok && !ok) & 0xffffu;
-            const int64_t koff = ok ? page * a.k_strides[0] + pos * a.k_strides[1] : 0, voff = ok ? page * a.v_strides[0] + pos * a.v_strides[1] : 0;
-            const uint32_t real = __ballot_sync(~0u, ok) & 0xffffu;
-            const __nv_bfloat16 *k = (const __nv_bfloat16 *)a.k_pages + get.head * a.k_strides[2], *v = (const __nv_bfloat16 *)a.v_pages + get.head * a.v_strides[2];
-            const uint32_t dst = ring + slot * STAGE;
+            const uint32_t bad = __ballot_sync(~0u, key_ok && !ok) & 0xffffu, real = __ballot_sync(~0u, ok) & 0xffffu;
+            __syncwarp();
+            if (lane < 16) rows_at[lane] = ok ? make_longlong2(page * a.k_strides[0] + pos * a.k_strides[1], page * a.v_strides[0] + pos * a.v_strides[1]) : make_longlong2(0, 0);
+            __syncwarp();
+            const __nv_bfloat16 *k = (const __nv_bfloat16 *)a.k_pages + get.head * a.k_strides[2] + copy_c * 8, *v = (const __nv_bfloat16 *)a.v_pages + get.head * a.v_strides[2] + copy_c * 8;
+            const uint32_t dst = ring + slot * STAGE + copy_row * PITCH + copy_c * 16;
+            if (real == 0xffffu) {
 #pragma unroll
-            for (int i = 0; i < 16 * CH / 32 / RG; ++i) {
-                const int piece = (i * RG + rg) * 32 + lane, row = piece / CH, c = piece % CH;
-                const uint32_t to = dst + row * (D * 2) + (((c & ~7) | ((c ^ row) & 7)) << 4);
-                const int64_t ko = __shfl_sync(~0u, koff, row), vo = __shfl_sync(~0u, voff, row);
-                cp_async16(to, k + ko + c * 8, real >> row & 1);
-                cp_async16(to + 16 * D * 2, v + vo + c * 8, real >> row & 1);
+                for (int i = 0; i < (COPIES + RG - 1) / RG; ++i) {
+                    if (COPIES % RG && i * RG + rg >= COPIES) break;
+                    const int row = (RG > 1 ? i * RG + rg : i) * PER;
+                    const longlong2 at = rows_at[row + copy_row];
+                    cp_async16(dst + row * PITCH, k + at.x);
+                    cp_async16(dst + (16 + row) * PITCH, v + at.y);
+                }
+            } else {
+#pragma unroll 1
+                for (int i = 0; i * RG + rg < COPIES; ++i) {
+                    const int row = (i * RG + rg) * PER;
+                    const longlong2 at = rows_at[row + copy_row];
+                    const bool is = real >> (row + copy_row) & 1;
+                    cp_async16(dst + row * PITCH, k + at.x, is);
+                    cp_async16(dst + (16 + row) * PITCH, v + at.y, is);
+                }
+                if (bad && rg == 0 && lane == 0) atomicMax(p.status, GQ_DEV_BAD_SHAPE);
             }
-            if (rg == 0 && lane == 0) {
-                bad_sm[kg * S + slot] = bad;
-                if (bad) atomicMax(p.status, GQ_DEV_BAD_SHAPE);
-            }
+            if (rg == 0 && lane == 0) bad_sm[kg * S + slot] = bad;
             ++got;
             if (++get.unit == get.units && got < count) next_segment<ROWS, UNIT>(p, get);
             look();
@@ -230,105 +252,76 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
     look();
     for (int i = 0; i < S - 1; ++i) ask(i);
 
-    float o[NT][4], top[2], sum[2];
-    uint32_t qf[QREG ? KK : 1][4];
-    int lim[2], lim_first = 0;     // keys that this lane's rows see, and the tile's first row
+    // Transposed products: keys (or dimensions) on M, the eight query rows of the warp on N.  A lane holds, of a score tile, keys g and g + 8 of queries 2 t and 2 t + 1; of the
+    // output, dimensions 16 i + g and 16 i + g + 8 of the same two queries.
+    float o[MT][4], top[2], sum[2];
+    uint32_t qf[MT][2];
+    int lim[2], lim_first = 0;     // keys that this lane's queries see, and the tile's first row
     bool fresh = true;
     int unit0 = 0;                 // this block's first unit of the segment
     int slot = 0;
-    const uint32_t q_addr = smem_u32(q_sm) + rg * 16 * D * 2;
+    // where this lane's row of an ldmatrix starts: keys (rows 0-7, 8-15 of one chunk, then of the next), values (transposed: two chunks of rows 0-7, then of 8-15)
+    const uint32_t k_lane = (((lane >> 3) & 1) * 8 + (lane & 7)) * PITCH + (lane >> 4) * 16, v_lane = (16 + (lane >> 4) * 8 + (lane & 7)) * PITCH + ((lane >> 3) & 1) * 16;
 
     for (int64_t it = 0; it < count; ++it) {
         if (fresh) {
             fresh = false;
             unit0 = use.unit;
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-            const int64_t rows = (int64_t)use.v.n * p.group, row0 = (int64_t)use.tile * ROWS + rg * 16;
-            const __nv_bfloat16 *src[2];
-            bool have[2];
+            const int64_t rows = (int64_t)use.v.n * p.group, row0 = (int64_t)use.tile * ROWS + rg * 8;
+            const int before = use.v.len - use.v.n + 1;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 top[j] = -INFINITY;
                 sum[j] = 0.0f;
-                const int64_t r = row0 + g + 8 * j;
-                have[j] = r < rows;
-                const int i = have[j] ? (int)(r / p.group) : 0, h = have[j] ? (int)(r % p.group) : 0;
-                lim[j] = use.v.len - use.v.n + i + 1;
-                src[j] = (const __nv_bfloat16 *)a.q + (use.v.tok0 + i) * a.q_strides[0] + (use.head * p.group + h) * a.q_strides[1];
+                lim[j] = before + (int)(min(row0 + 2 * t + j, rows - 1) / p.group);
             }
-            lim_first = use.v.len - use.v.n + (int)(((int64_t)use.tile * ROWS) / p.group) + 1;
-            if constexpr (QREG) {
+            lim_first = before + (int)(((int64_t)use.tile * ROWS) / p.group);
+            const int64_t r = row0 + g, i = r / p.group;
+            const uint32_t *src = (const uint32_t *)((const __nv_bfloat16 *)a.q + (use.v.tok0 + i) * a.q_strides[0] + (use.head * p.group + (r - i * p.group)) * a.q_strides[1]) + t;
 #pragma unroll
-                for (int i = 0; i < KK; ++i)
+            for (int x = 0; x < MT; ++x)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) qf[i][j] = have[j & 1] ? *(const uint32_t *)(src[j & 1] + i * 16 + (j >> 1) * 8 + t * 2) : 0u;
-            } else {
-                // the rows of this row group, once for its KG warps: before the barrier of this iteration, behind that of the last merge
-                for (int i = kg * 32 + lane; i < 16 * CH; i += 32 * KG) {
-                    const int row = i / CH, c = i % CH;
-                    const int64_t r = row0 + row;
-                    uint4 val = make_uint4(0, 0, 0, 0);
-                    if (r < rows)
-                        val = *(const uint4 *)((const __nv_bfloat16 *)a.q + (use.v.tok0 + r / p.group) * a.q_strides[0] + (use.head * p.group + r % p.group) * a.q_strides[1] + c * 8);
-                    *(uint4 *)(q_sm + (rg * 16 + row) * (D * 2) + (((c & ~7) | ((c ^ row) & 7)) << 4)) = val;
-                }
-                __syncthreads();
-            }
+                for (int j = 0; j < 2; ++j) qf[x][j] = r < rows ? src[x * 8 + j * 4] : 0u;
         }
         cp_async_wait<S - 2>();
         if constexpr (RG > 1) asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * RG) : "memory");
         else __syncwarp();
-        ask((slot + S - 1) % S);
+        ask(slot == 0 ? S - 1 : slot - 1);
 
         // ---- scores of 16 keys ----
-        const uint32_t ks = ring + slot * STAGE, vs = ks + 16 * D * 2;
-        float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-        {
-            const int row = (lane >> 4) * 8 + (lane & 7), half = (lane >> 3) & 1;
+        const uint32_t stage = ring + slot * STAGE;
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < KK; ++i) {
-                const int c = 2 * i + half;
-                uint32_t kf[4];
-                ldsm4(kf, ks + row * (D * 2) + (((c & ~7) | ((c ^ row) & 7)) << 4));
-                if constexpr (QREG) {
-                    mma_bf16(s[0], qf[i], kf[0], kf[1]);
-                    mma_bf16(s[1], qf[i], kf[2], kf[3]);
-                } else {
-                    const int qr = ((lane >> 3) & 1) * 8 + (lane & 7), qc = 2 * i + (lane >> 4);
-                    uint32_t q4[4];
-                    ldsm4(q4, q_addr + qr * (D * 2) + (((qc & ~7) | ((qc ^ qr) & 7)) << 4));
-                    mma_bf16(s[0], q4, kf[0], kf[1]);
-                    mma_bf16(s[1], q4, kf[2], kf[3]);
-                }
-            }
+        for (int i = 0; i < MT; ++i) {
+            uint32_t kf[4];
+            ldsm4(kf, stage + k_lane + i * 32);
+            mma_bf16(i & 1 ? s2 : s, kf, qf[i][0], qf[i][1]);
         }
         const int key0 = (use.unit * KG + kg) * 16;
         const uint32_t bad = bad_sm[kg * S + slot];
         const bool edge = key0 + 16 > lim_first || bad;        // a row of the tile does not see all of these keys, or a page is missing
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[i][j] *= p.scale2;
+        for (int j = 0; j < 4; ++j) s[j] = (s[j] + s2[j]) * p.scale2;
         if (edge) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = i * 8 + t * 2 + (j & 1);
-                    if (bad >> at & 1) s[i][j] = __int_as_float(0x7fc00000);
-                    if (key0 + at >= lim[j >> 1]) s[i][j] = -INFINITY;
-                }
+            for (int j = 0; j < 4; ++j) {
+                const int at = g + (j >> 1) * 8;
+                if (bad >> at & 1) s[j] = __int_as_float(0x7fc00000);
+                if (key0 + at >= lim[j & 1]) s[j] = -INFINITY;
+            }
         }
         // ---- running maximum and sum ----
         float next[2], ref[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            float m = fmaxf(fmaxf(s[0][2 * j], s[0][2 * j + 1]), fmaxf(s[1][2 * j], s[1][2 * j + 1]));
-            m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
-            m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
+            float m = fmaxf(s[j], s[j + 2]);
+            m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
             next[j] = fmaxf(top[j], m);
             ref[j] = next[j] == -INFINITY ? 0.0f : next[j];
         }
@@ -337,99 +330,94 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
 #pragma unroll
             for (int j = 0; j < 2; ++j) { top[j] = next[j]; sum[j] *= keep[j]; }
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[i][j] *= keep[j >> 1];
+                for (int j = 0; j < 4; ++j) o[i][j] *= keep[j & 1];
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { s[i][j] = ex2(s[i][j] - ref[j >> 1]); sum[j >> 1] += s[i][j]; }
+        for (int j = 0; j < 4; ++j) { s[j] = ex2(s[j] - ref[j & 1]); sum[j & 1] += s[j]; }
         // ---- p v ----
-        uint32_t big[4], small[4], vm0 = ~0u, vm1 = ~0u;
         // Keys that some rows of the tile see and others do not: a masked probability of 0 would still make NaN of an infinite value, so these keys stay out of the MMA and are
         // added row by row.  There are fewer of them in all than new tokens in the tile.
-        const bool split = edge && lim_first < use.keys && key0 + 16 > lim_first;
-        const int from = split ? max(lim_first - key0, 0) : 16, to = split ? min(use.keys - key0, 16) : 16;
+        const bool split = edge && lim_first < use.keys;
+        const int from = split ? max(lim_first - key0, 0) : 16;
         if (split) {
-            const int at = t * 2;
-            vm0 = (at < from ? 0xffffu : 0u) | (at + 1 < from ? 0xffff0000u : 0u);
-            vm1 = (at + 8 < from ? 0xffffu : 0u) | (at + 9 < from ? 0xffff0000u : 0u);
+            const int to = min(use.keys - key0, 16);
             for (int x = from; x < to; ++x) {
-                const int owner = (lane & ~3) | ((x & 7) >> 1), i = x >> 3;
-                const float pa = __shfl_sync(~0u, i ? ((x & 1) ? s[1][1] : s[1][0]) : ((x & 1) ? s[0][1] : s[0][0]), owner);
-                const float pb = __shfl_sync(~0u, i ? ((x & 1) ? s[1][3] : s[1][2]) : ((x & 1) ? s[0][3] : s[0][2]), owner);
+                const int owner = (x & 7) * 4 + t;
+                const float pa = __shfl_sync(~0u, x & 8 ? s[2] : s[0], owner), pb = __shfl_sync(~0u, x & 8 ? s[3] : s[1], owner);
                 const bool see_a = key0 + x < lim[0], see_b = key0 + x < lim[1];
+                const __nv_bfloat16 *v = (const __nv_bfloat16 *)(smem + (stage - smem_u32(smem)) + (16 + x) * PITCH) + g;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const uint32_t w = *(const uint32_t *)(smem + (vs - smem_u32(smem)) + x * (D * 2) + (((n & ~7) | ((n ^ x) & 7)) << 4) + t * 4);
-                    const float v0 = __uint_as_float(w << 16), v1 = __uint_as_float(w & 0xffff0000u);
-                    if (see_a) { o[n][0] += pa * v0; o[n][1] += pa * v1; }
-                    if (see_b) { o[n][2] += pb * v0; o[n][3] += pb * v1; }
-                }
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float val = __bfloat162float(v[i * 16 + j * 8]);
+                        if (see_a) o[i][2 * j] += pa * val;
+                        if (see_b) o[i][2 * j + 1] += pb * val;
+                    }
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (i * 8 + t * 2 + (j & 1) >= from) s[i][j] = 0.0f;
+            for (int j = 0; j < 4; ++j)
+                if (g + (j >> 1) * 8 >= from) s[j] = 0.0f;
         }
+        // the probabilities of eight keys, turned over: queries on g, keys 2 t and 2 t + 1, as the B operand has them
+        uint32_t big[2], small[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bf16_parts(s[j >> 1][2 * (j & 1)], s[j >> 1][2 * (j & 1) + 1], big[j], small[j]);
-        {
-            const int row = ((lane >> 3) & 1) * 8 + (lane & 7), half = lane >> 4;
-#pragma unroll
-            for (int n = 0; n < NT; n += 2) {
-                const int c = n + half;
-                uint32_t vf[4];
-                ldsm4_t(vf, vs + row * (D * 2) + (((c & ~7) | ((c ^ row) & 7)) << 4));
-                if (split) { vf[0] &= vm0; vf[1] &= vm1; vf[2] &= vm0; vf[3] &= vm1; }
-                mma_bf16(o[n], big, vf[0], vf[1]);
-                mma_bf16(o[n + 1], big, vf[2], vf[3]);
-                mma_bf16(o[n], small, vf[0], vf[1]);
-                mma_bf16(o[n + 1], small, vf[2], vf[3]);
-            }
+        for (int j = 0; j < 2; ++j) {
+            bf16_parts(s[2 * j], s[2 * j + 1], big[j], small[j]);
+            big[j] = transpose8(big[j]);
+            small[j] = transpose8(small[j]);
         }
-        slot = (slot + 1) % S;
+        const uint32_t vm0 = (2 * t < from ? 0xffffu : 0u) | (2 * t + 1 < from ? 0xffff0000u : 0u), vm1 = (2 * t + 8 < from ? 0xffffu : 0u) | (2 * t + 9 < from ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            uint32_t vf[4];
+            ldsm4_t(vf, stage + v_lane + i * 32);
+            if (split) { vf[0] &= vm0; vf[1] &= vm0; vf[2] &= vm1; vf[3] &= vm1; }
+            mma_bf16(o[i], vf, big[0], big[1]);
+            mma_bf16(o[i], vf, small[0], small[1]);
+        }
+        if (++slot == S) slot = 0;
         ++use.unit;
         if (use.unit != use.units && it + 1 != count) continue;
 
         // ---- the end of this block's part of a segment: key groups joined, from the last to the first ----
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            sum[j] += __shfl_xor_sync(~0u, sum[j], 1);
-            sum[j] += __shfl_xor_sync(~0u, sum[j], 2);
-        }
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) sum[j] += __shfl_xor_sync(~0u, sum[j], x);
         if constexpr (KG > 1) {
-            if (t == 0)
-                for (int j = 0; j < 2; ++j) stat_sm[kg * ROWS + rg * 16 + g + 8 * j] = make_float2(top[j], sum[j]);
+            if (g == 0)
+                for (int j = 0; j < 2; ++j) stat_sm[kg * ROWS + rg * 8 + 2 * t + j] = make_float2(top[j], sum[j]);
             __syncthreads();
+            float keep[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
+                const float2 *st = stat_sm + rg * 8 + 2 * t + j;
                 float m = -INFINITY, l = 0.0f;
-                for (int x = 0; x < KG; ++x) m = fmaxf(m, stat_sm[x * ROWS + rg * 16 + g + 8 * j].x);
+                for (int x = 0; x < KG; ++x) m = fmaxf(m, st[x * ROWS].x);
                 const float r = m == -INFINITY ? 0.0f : m;
-                for (int x = 0; x < KG; ++x) {
-                    const float2 st = stat_sm[x * ROWS + rg * 16 + g + 8 * j];
-                    l += st.y * ex2(st.x - r);
-                }
-                const float keep = ex2(top[j] - r);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) { o[n][2 * j] *= keep; o[n][2 * j + 1] *= keep; }
+                for (int x = 0; x < KG; ++x) l += st[x * ROWS].y * ex2(st[x * ROWS].x - r);
+                keep[j] = ex2(top[j] - r);
                 top[j] = m;
                 sum[j] = l;
             }
-            float4 *box = (float4 *)merge + rg * 16 * D / 4 + lane;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[i][j] *= keep[j & 1];
+            float4 *box = (float4 *)merge + rg * 2 * D + lane;
             for (int x = KG - 1; x > 0; --x) {
                 if (kg == x)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) box[n * 32] = make_float4(o[n][0], o[n][1], o[n][2], o[n][3]);
+                    for (int i = 0; i < MT; ++i) box[i * 32] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
                 __syncthreads();
                 if (kg == x - 1)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const float4 v = box[n * 32];
-                        o[n][0] += v.x; o[n][1] += v.y; o[n][2] += v.z; o[n][3] += v.w;
+                    for (int i = 0; i < MT; ++i) {
+                        const float4 v = box[i * 32];
+                        o[i][0] += v.x; o[i][1] += v.y; o[i][2] += v.z; o[i][3] += v.w;
                     }
                 __syncthreads();
             }
@@ -439,26 +427,28 @@ __global__ void __launch_bounds__(PA_THREADS) paged_attention_kernel(const __gri
             const int64_t part = 2 * (int64_t)blockIdx.x + (unit0 == 0), rows = (int64_t)use.v.n * p.group;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int64_t r = (int64_t)use.tile * ROWS + rg * 16 + g + 8 * j;
+                const int64_t r = (int64_t)use.tile * ROWS + rg * 8 + 2 * t + j;
                 if (r >= rows) continue;
                 if (whole) {
                     const int64_t tok = use.v.tok0 + r / p.group, h = use.head * p.group + r % p.group;
-                    __nv_bfloat16 *dst = (__nv_bfloat16 *)a.out + tok * a.out_strides[0] + h * a.out_strides[1] + t * 2;
-                    const __nv_bfloat16 *gate = a.gate ? (const __nv_bfloat16 *)a.gate + tok * a.gate_strides[0] + h * a.gate_strides[1] + t * 2 : nullptr;
+                    __nv_bfloat16 *dst = (__nv_bfloat16 *)a.out + tok * a.out_strides[0] + h * a.out_strides[1] + g;
+                    const __nv_bfloat16 *gate = a.gate ? (const __nv_bfloat16 *)a.gate + tok * a.gate_strides[0] + h * a.gate_strides[1] + g : nullptr;
                     const float inv = sum[j] == 0.0f ? 0.0f : 1.0f / sum[j];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int i = 0; i < MT; ++i)
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            float v = o[n][2 * j + x] * inv;
-                            if (gate) v /= 1.0f + ex2(-1.4426950408889634f * __bfloat162float(gate[n * 8 + x]));
-                            dst[n * 8 + x] = __float2bfloat16_rn(v);
+                            float v = o[i][2 * x + j] * inv;
+                            if (gate) v /= 1.0f + ex2(-1.4426950408889634f * __bfloat162float(gate[i * 16 + x * 8]));
+                            dst[i * 16 + x * 8] = __float2bfloat16_rn(v);
                         }
                 } else {
-                    const int64_t at = part * ROWS + rg * 16 + g + 8 * j;
-                    if (t == 0) p.stats[at] = make_float2(top[j], sum[j]);
+                    const int64_t at = part * ROWS + rg * 8 + 2 * t + j;
+                    if (g == 0) p.stats[at] = make_float2(top[j], sum[j]);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) *(float2 *)(p.parts + at * D + n * 8 + t * 2) = make_float2(o[n][2 * j], o[n][2 * j + 1]);
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) p.parts[at * D + i * 16 + x * 8 + g] = o[i][2 * x + j];
                 }
             }
         }
@@ -487,7 +477,7 @@ __global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__
             if (a.q_starts[mid] <= tok) s = mid; else hi = mid;
         }
     } else s = tok / (a.T / a.n_seqs);
-    const SeqSpan v = seq_span(a, s);
+    const SeqSpan v = seq_span(p, s);
     if (tok < v.tok0 || tok >= v.tok0 + v.n) return;          // nobody's row
     const int64_t row = (tok - v.tok0) * p.group + h % p.group;
     const int tile = (int)(row / rows_of_tile);

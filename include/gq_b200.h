@@ -333,7 +333,7 @@ int gq_head_norm_rope(const gq_head_norm_args *args, void *stream);
  * A token that sees no key: zeros.  Tokens of sequence s are q_starts[s] .. q_starts[s + 1] - 1 (null: T / n_seqs each); rows behind the last
  * sequence are left as they were.  Key j stands in row j % page_size of page page_table[s, j / page_size].  A page outside the cache, or a length beyond the table: the
  * rows that see it are NaN and the device status becomes 2.  head_dim 64, 128 or 256; n_heads a multiple of n_kv_heads; every row, head and page starts
- * at a multiple of 16 bytes (gate, and out: of 2).  out shares no memory with an input. */
+ * at a multiple of 16 bytes (gate, and out: of 2).  out shares no memory with an input.  Up to 2^24 tokens, and tables of up to 2^30 keys. */
 typedef struct gq_attention_args {
     const void *q;               /* bf16 [T, n_heads, head_dim] by strides */
     const void *k_pages, *v_pages;
