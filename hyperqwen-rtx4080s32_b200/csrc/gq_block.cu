@@ -141,6 +141,7 @@ template <int D, int RG, int KG, int S> static int attention(const gq_attention_
     uint32_t log2 = 0;
     while ((int64_t)1 << log2 < p->page_size) ++log2;
     PagedParams q{*p, status, (int64_t *)ws, (float2 *)(ws + at_stats), (float *)(ws + at_parts), p->n_heads / p->n_kv_heads, blocks, (int)(p->table_width * p->page_size),
+                  p->page_size % 16 == 0 && p->k_strides[1] < (1 << 27) && p->v_strides[1] < (1 << 27),
                   (uint32_t)(((uint64_t)1 << (31 + log2)) / p->page_size + 1), 31 + log2, p->scale * 1.4426950408889634f};
     if (p->n_pages == 0) {       // every page is outside the cache: nothing is read, but addresses are formed
         q.a.k_pages = q.a.v_pages = p->q;

@@ -24,6 +24,7 @@ struct PagedParams {
     float2 *stats;          // [2 G][rows of a tile]: maximum, sum
     float *parts;           // [2 G][rows of a tile][head_dim]
     int group, blocks, max_keys;        // query heads of a kv head; blocks the GPU holds; keys that the page table has room for
+    int whole;              // pages hold whole stages of 16 keys
     uint32_t page_mul, page_shift;      // key / page_size = key * page_mul >> page_shift, for keys below 2^31
     float scale2;           // scale * log2 e
 };
@@ -133,7 +134,7 @@ template <int D, int RG, int KG, int S> struct PagedShape {
     static constexpr int PITCH = D * 2 + 16;                                    // bytes of a row in shared memory: eight rows' chunks in different banks
     static constexpr int STAGE = 2 * 16 * PITCH;                                // keys and values of 16 keys
     static constexpr int RING = KG * S * STAGE, MERGE = KG > 1 ? ROWS * D * 4 : 0, STATS = KG > 1 ? KG * ROWS * 8 : 0;
-    static constexpr int SMEM = RING + MERGE + STATS + RG * KG * 256 + KG * S * 4;
+    static constexpr int SMEM = RING + MERGE + STATS + RG * KG * 256;
 };
 
 template <int D, int RG, int KG, int S>
@@ -143,8 +144,7 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
     extern __shared__ __align__(128) uint8_t smem[];
     float *merge = (float *)(smem + Shape::RING);
     float2 *stat_sm = (float2 *)((uint8_t *)merge + Shape::MERGE);
-    longlong2 *row_sm = (longlong2 *)((uint8_t *)stat_sm + Shape::STATS);       // [warp][16]: where the keys and values of the stage being asked for start
-    uint32_t *bad_sm = (uint32_t *)(row_sm + 16 * WARPS);                      // [KG][S]: a stage's keys whose page is missing
+    longlong2 *row_sm = (longlong2 *)((uint8_t *)stat_sm + Shape::STATS);       // [warp][16]: bytes to the keys and values of the stage being asked for
     __shared__ int64_t scan[WARPS], place[3];
     const gq_attention_args &a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, rg = warp % RG, kg = warp / RG, g = lane / 4, t = lane % 4;
@@ -194,16 +194,24 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
         while (in >= use.units) { in -= use.units; ++use.tile; load_segment<ROWS, UNIT>(p, use); }
         use.unit = (int)in;
     }
-    const int64_t count = w1 - w0;
+    const int count = (int)(w1 - w0);
 
-    // ---- loads: a stage of this key group is 16 keys; lane l finds key l & 15, then all lanes copy 16 bytes of each pair of rows ----
+    // ---- loads: a stage of this key group is 16 keys ----
     const uint32_t ring = smem_u32(smem) + kg * S * STAGE;
+    constexpr int PER = 32 / CH, COPIES = 16 * CH / 32;        // rows that 32 lanes copy at once, 16 bytes each; turns for a stage
+    const int copy_row = lane / CH, copy_c = lane % CH;
+    const uint32_t copy_to = ring + copy_row * PITCH + copy_c * 16;
     Cursor get = use;
-    int64_t got = 0;
-    int page = 0, pos = 0;          // of key l & 15 of the stage after the one being asked for
+    int got = 0, page = 0, pos = 0;        // of the next stage to ask for: the page and row of its first key, or (pages that end inside a stage) of key lane & 15
     bool page_ok = false, key_ok = false;
-    auto look = [&]() {             // the page of the stage at `get`
-        const int key = (get.unit * KG + kg) * 16 + (lane & 15);
+    uint32_t k_step = (uint32_t)a.k_strides[1] * 2, v_step = (uint32_t)a.v_strides[1] * 2;      // bytes between rows of a page (whole pages: below 2^32)
+    const char *k_head, *v_head;
+    auto heads = [&]() {
+        k_head = (const char *)((const __nv_bfloat16 *)a.k_pages + get.head * a.k_strides[2] + copy_c * 8 + (p.whole ? copy_row * a.k_strides[1] : 0));
+        v_head = (const char *)((const __nv_bfloat16 *)a.v_pages + get.head * a.v_strides[2] + copy_c * 8 + (p.whole ? copy_row * a.v_strides[1] : 0));
+    };
+    auto look = [&]() {
+        const int key = (get.unit * KG + kg) * 16 + (p.whole ? 0 : lane & 15);
         key_ok = got < count && key < get.keys;
         const int at = (int)((uint64_t)(uint32_t)key * p.page_mul >> p.page_shift);
         page_ok = key_ok && at < a.table_width;
@@ -211,44 +219,57 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
         pos = key - at * a.page_size;
     };
     longlong2 *rows_at = row_sm + warp * 16;
-    constexpr int PER = 32 / CH, COPIES = 16 * CH / 32;        // rows that 32 lanes copy at once, turns for a stage
-    const int copy_row = lane / CH, copy_c = lane % CH;
+    uint64_t missing = 0;           // of the stages asked for and not used yet, 16 bits each, the next one lowest: keys whose page is missing
     auto ask = [&](int slot) {      // copies the stage that look() has seen, then looks at the next
+        uint32_t bad = 0;
         if (got < count) {
             const bool ok = page_ok && page >= 0 && page < a.n_pages;
-            const uint32_t bad = __ballot_sync(~0u, key_ok && !ok) & 0xffffu, real = __ballot_sync(~0u, ok) & 0xffffu;
-            __syncwarp();
-            if (lane < 16) rows_at[lane] = ok ? make_longlong2(page * a.k_strides[0] + pos * a.k_strides[1], page * a.v_strides[0] + pos * a.v_strides[1]) : make_longlong2(0, 0);
-            __syncwarp();
-            const __nv_bfloat16 *k = (const __nv_bfloat16 *)a.k_pages + get.head * a.k_strides[2] + copy_c * 8, *v = (const __nv_bfloat16 *)a.v_pages + get.head * a.v_strides[2] + copy_c * 8;
-            const uint32_t dst = ring + slot * STAGE + copy_row * PITCH + copy_c * 16;
-            if (real == 0xffffu) {
+            const uint32_t dst = copy_to + slot * STAGE;
+            if (p.whole) {          // the stage lies in one page
+                const int seen = min(get.keys - (get.unit * KG + kg) * 16, 16), real = ok ? seen : 0;
+                const char *k = k_head + (page * a.k_strides[0] + pos * a.k_strides[1]) * 2, *v = v_head + (page * a.v_strides[0] + pos * a.v_strides[1]) * 2;
+                if (real == 16) {
 #pragma unroll
-                for (int i = 0; i < (COPIES + RG - 1) / RG; ++i) {
-                    if (COPIES % RG && i * RG + rg >= COPIES) break;
-                    const int row = (RG > 1 ? i * RG + rg : i) * PER;
-                    const longlong2 at = rows_at[row + copy_row];
-                    cp_async16(dst + row * PITCH, k + at.x);
-                    cp_async16(dst + (16 + row) * PITCH, v + at.y);
-                }
-            } else {
+                    for (int i = 0; i < (COPIES + RG - 1) / RG; ++i) {
+                        if (COPIES % RG && i * RG + rg >= COPIES) break;
+                        const uint32_t row = (RG > 1 ? i * RG + rg : i) * PER;
+                        cp_async16(dst + row * PITCH, k + (uint64_t)row * k_step);
+                        cp_async16(dst + (16 + row) * PITCH, v + (uint64_t)row * v_step);
+                    }
+                } else {
+                    bad = ok || seen <= 0 ? 0u : (1u << seen) - 1;
 #pragma unroll 1
-                for (int i = 0; i * RG + rg < COPIES; ++i) {
-                    const int row = (i * RG + rg) * PER;
+                    for (int i = rg; i < COPIES; i += RG) {
+                        const uint32_t row = i * PER;
+                        const bool is = (int)row + copy_row < real;
+                        cp_async16(dst + row * PITCH, is ? k + (uint64_t)row * k_step : (const char *)a.k_pages, is);
+                        cp_async16(dst + (16 + row) * PITCH, is ? v + (uint64_t)row * v_step : (const char *)a.v_pages, is);
+                    }
+                }
+            } else {                // lane l finds key l & 15
+                bad = __ballot_sync(~0u, key_ok && !ok) & 0xffffu;
+                const uint32_t real = __ballot_sync(~0u, ok);
+                __syncwarp();
+                if (lane < 16) rows_at[lane] = ok ? make_longlong2(2 * (page * a.k_strides[0] + pos * a.k_strides[1]), 2 * (page * a.v_strides[0] + pos * a.v_strides[1])) : make_longlong2(0, 0);
+                __syncwarp();
+#pragma unroll 2
+                for (int i = rg; i < COPIES; i += RG) {
+                    const int row = i * PER;
                     const longlong2 at = rows_at[row + copy_row];
                     const bool is = real >> (row + copy_row) & 1;
-                    cp_async16(dst + row * PITCH, k + at.x, is);
-                    cp_async16(dst + (16 + row) * PITCH, v + at.y, is);
+                    cp_async16(dst + row * PITCH, k_head + at.x, is);
+                    cp_async16(dst + (16 + row) * PITCH, v_head + at.y, is);
                 }
-                if (bad && rg == 0 && lane == 0) atomicMax(p.status, GQ_DEV_BAD_SHAPE);
             }
-            if (rg == 0 && lane == 0) bad_sm[kg * S + slot] = bad;
+            if (bad && lane == 0) atomicMax(p.status, GQ_DEV_BAD_SHAPE);
             ++got;
-            if (++get.unit == get.units && got < count) next_segment<ROWS, UNIT>(p, get);
+            if (++get.unit == get.units && got < count) { next_segment<ROWS, UNIT>(p, get); heads(); }
             look();
         }
+        missing = missing >> 16 | (uint64_t)bad << (16 * (S - 2));
         cp_async_commit();
     };
+    heads();
     look();
     for (int i = 0; i < S - 1; ++i) ask(i);
 
@@ -257,16 +278,13 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
     float o[MT][4], top[2], sum[2];
     uint32_t qf[MT][2];
     int lim[2], lim_first = 0;     // keys that this lane's queries see, and the tile's first row
-    bool fresh = true;
-    int unit0 = 0;                 // this block's first unit of the segment
     int slot = 0;
     // where this lane's row of an ldmatrix starts: keys (rows 0-7, 8-15 of one chunk, then of the next), values (transposed: two chunks of rows 0-7, then of 8-15)
     const uint32_t k_lane = (((lane >> 3) & 1) * 8 + (lane & 7)) * PITCH + (lane >> 4) * 16, v_lane = (16 + (lane >> 4) * 8 + (lane & 7)) * PITCH + ((lane >> 3) & 1) * 16;
 
-    for (int64_t it = 0; it < count; ++it) {
-        if (fresh) {
-            fresh = false;
-            unit0 = use.unit;
+    for (int it = 0;;) {
+        const int unit0 = use.unit;         // this block's first unit of the segment
+        {
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -287,100 +305,111 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
 #pragma unroll
                 for (int j = 0; j < 2; ++j) qf[x][j] = r < rows ? src[x * 8 + j * 4] : 0u;
         }
-        cp_async_wait<S - 2>();
-        if constexpr (RG > 1) asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * RG) : "memory");
-        else __syncwarp();
-        ask(slot == 0 ? S - 1 : slot - 1);
+        for (const int end = min(use.units, use.unit + count - it); use.unit < end; ++use.unit) {
+            cp_async_wait<S - 2>();
+            if constexpr (RG > 1) asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * RG) : "memory");
+            else __syncwarp();
+            const uint32_t bad = (uint32_t)missing & 0xffffu;
+            ask(slot == 0 ? S - 1 : slot - 1);
 
-        // ---- scores of 16 keys ----
-        const uint32_t stage = ring + slot * STAGE;
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            // ---- scores of 16 keys ----
+            const uint32_t stage = ring + slot * STAGE;
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            uint32_t kf[4];
-            ldsm4(kf, stage + k_lane + i * 32);
-            mma_bf16(i & 1 ? s2 : s, kf, qf[i][0], qf[i][1]);
-        }
-        const int key0 = (use.unit * KG + kg) * 16;
-        const uint32_t bad = bad_sm[kg * S + slot];
-        const bool edge = key0 + 16 > lim_first || bad;        // a row of the tile does not see all of these keys, or a page is missing
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = (s[j] + s2[j]) * p.scale2;
-        if (edge) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int at = g + (j >> 1) * 8;
-                if (bad >> at & 1) s[j] = __int_as_float(0x7fc00000);
-                if (key0 + at >= lim[j & 1]) s[j] = -INFINITY;
+            for (int i = 0; i < MT; ++i) {
+                uint32_t kf[4];
+                ldsm4(kf, stage + k_lane + i * 32);
+                mma_bf16(i & 1 ? s2 : s, kf, qf[i][0], qf[i][1]);
             }
-        }
-        // ---- running maximum and sum ----
-        float next[2], ref[2];
+            const int key0 = (use.unit * KG + kg) * 16;
+            const bool edge = key0 + 16 > lim_first || bad;        // a row of the tile does not see all of these keys, or a page is missing
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            float m = fmaxf(s[j], s[j + 2]);
-            m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
-            m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
-            next[j] = fmaxf(top[j], m);
-            ref[j] = next[j] == -INFINITY ? 0.0f : next[j];
-        }
-        if (__any_sync(~0u, next[0] > top[0] || next[1] > top[1])) {
-            const float keep[2] = {ex2(top[0] - ref[0]), ex2(top[1] - ref[1])};
+            for (int j = 0; j < 4; ++j) s[j] = (s[j] + s2[j]) * p.scale2;
+            if (edge) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) { top[j] = next[j]; sum[j] *= keep[j]; }
+                for (int j = 0; j < 4; ++j) {
+                    const int at = g + (j >> 1) * 8;
+                    if (bad >> at & 1) s[j] = __int_as_float(0x7fc00000);
+                    if (key0 + at >= lim[j & 1]) s[j] = -INFINITY;
+                }
+            }
+            // ---- running maximum and sum ----
+            float next[2], ref[2];
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int j = 0; j < 2; ++j) {
+                float m = fmaxf(s[j], s[j + 2]);
+                m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
+                m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+                m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
+                next[j] = fmaxf(top[j], m);
+                ref[j] = next[j] == -INFINITY ? 0.0f : next[j];
+            }
+            if (__any_sync(~0u, next[0] > top[0] || next[1] > top[1])) {
+                const float keep[2] = {ex2(top[0] - ref[0]), ex2(top[1] - ref[1])};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[i][j] *= keep[j & 1];
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { s[j] = ex2(s[j] - ref[j & 1]); sum[j & 1] += s[j]; }
-        // ---- p v ----
-        // Keys that some rows of the tile see and others do not: a masked probability of 0 would still make NaN of an infinite value, so these keys stay out of the MMA and are
-        // added row by row.  There are fewer of them in all than new tokens in the tile.
-        const bool split = edge && lim_first < use.keys;
-        const int from = split ? max(lim_first - key0, 0) : 16;
-        if (split) {
-            const int to = min(use.keys - key0, 16);
-            for (int x = from; x < to; ++x) {
-                const int owner = (x & 7) * 4 + t;
-                const float pa = __shfl_sync(~0u, x & 8 ? s[2] : s[0], owner), pb = __shfl_sync(~0u, x & 8 ? s[3] : s[1], owner);
-                const bool see_a = key0 + x < lim[0], see_b = key0 + x < lim[1];
-                const __nv_bfloat16 *v = (const __nv_bfloat16 *)(smem + (stage - smem_u32(smem)) + (16 + x) * PITCH) + g;
+                for (int j = 0; j < 2; ++j) { top[j] = next[j]; sum[j] *= keep[j]; }
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float val = __bfloat162float(v[i * 16 + j * 8]);
-                        if (see_a) o[i][2 * j] += pa * val;
-                        if (see_b) o[i][2 * j + 1] += pb * val;
-                    }
+                    for (int j = 0; j < 4; ++j) o[i][j] *= keep[j & 1];
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (g + (j >> 1) * 8 >= from) s[j] = 0.0f;
-        }
-        // the probabilities of eight keys, turned over: queries on g, keys 2 t and 2 t + 1, as the B operand has them
-        uint32_t big[2], small[2];
+            for (int j = 0; j < 4; ++j) { s[j] = ex2(s[j] - ref[j & 1]); sum[j & 1] += s[j]; }
+            // ---- p v ----
+            // Keys that some rows of the tile see and others do not: a masked probability of 0 would still make NaN of an infinite value, so these keys stay out of the MMA and are
+            // added row by row.  There are fewer of them in all than new tokens in the tile.
+            const bool split = edge && lim_first < use.keys;
+            const int from = split ? max(lim_first - key0, 0) : 16;
+            if (split) {
+                const int to = min(use.keys - key0, 16);
+                for (int x = from; x < to; ++x) {
+                    const int owner = (x & 7) * 4 + t;
+                    const float pa = __shfl_sync(~0u, x & 8 ? s[2] : s[0], owner), pb = __shfl_sync(~0u, x & 8 ? s[3] : s[1], owner);
+                    const bool see_a = key0 + x < lim[0], see_b = key0 + x < lim[1];
+                    const __nv_bfloat16 *v = (const __nv_bfloat16 *)(smem + (stage - smem_u32(smem)) + (16 + x) * PITCH) + g;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            bf16_parts(s[2 * j], s[2 * j + 1], big[j], small[j]);
-            big[j] = transpose8(big[j]);
-            small[j] = transpose8(small[j]);
-        }
-        const uint32_t vm0 = (2 * t < from ? 0xffffu : 0u) | (2 * t + 1 < from ? 0xffff0000u : 0u), vm1 = (2 * t + 8 < from ? 0xffffu : 0u) | (2 * t + 9 < from ? 0xffff0000u : 0u);
+                    for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            uint32_t vf[4];
-            ldsm4_t(vf, stage + v_lane + i * 32);
-            if (split) { vf[0] &= vm0; vf[1] &= vm0; vf[2] &= vm1; vf[3] &= vm1; }
-            mma_bf16(o[i], vf, big[0], big[1]);
-            mma_bf16(o[i], vf, small[0], small[1]);
+                        for (int j = 0; j < 2; ++j) {
+                            const float val = __bfloat162float(v[i * 16 + j * 8]);
+                            if (see_a) o[i][2 * j] += pa * val;
+                            if (see_b) o[i][2 * j + 1] += pb * val;
+                        }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (g + (j >> 1) * 8 >= from) s[j] = 0.0f;
+            }
+            // the probabilities of eight keys, turned over: queries on g, keys 2 t and 2 t + 1, as the B operand has them
+            uint32_t big[2], small[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                bf16_parts(s[2 * j], s[2 * j + 1], big[j], small[j]);
+                big[j] = transpose8(big[j]);
+                small[j] = transpose8(small[j]);
+            }
+            if (split) {
+                const uint32_t vm0 = (2 * t < from ? 0xffffu : 0u) | (2 * t + 1 < from ? 0xffff0000u : 0u), vm1 = (2 * t + 8 < from ? 0xffffu : 0u) | (2 * t + 9 < from ? 0xffff0000u : 0u);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    uint32_t vf[4];
+                    ldsm4_t(vf, stage + v_lane + i * 32);
+                    vf[0] &= vm0; vf[1] &= vm0; vf[2] &= vm1; vf[3] &= vm1;
+                    mma_bf16(o[i], vf, big[0], big[1]);
+                    mma_bf16(o[i], vf, small[0], small[1]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    uint32_t vf[4];
+                    ldsm4_t(vf, stage + v_lane + i * 32);
+                    mma_bf16(o[i], vf, big[0], big[1]);
+                    mma_bf16(o[i], vf, small[0], small[1]);
+                }
+            }
+            if (++slot == S) slot = 0;
+            ++it;
         }
-        if (++slot == S) slot = 0;
-        ++use.unit;
-        if (use.unit != use.units && it + 1 != count) continue;
 
         // ---- the end of this block's part of a segment: key groups joined, from the last to the first ----
 #pragma unroll
@@ -452,8 +481,8 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
                 }
             }
         }
-        fresh = true;
-        if (it + 1 != count) next_segment<ROWS, UNIT>(p, use);
+        if (it == count) break;
+        next_segment<ROWS, UNIT>(p, use);
     }
     cp_async_wait<0>();
 }
