@@ -95,7 +95,7 @@ static int check_attention(const gq_attention_args *p) {
     if (p->T < 0 || p->T > INT32_MAX || p->n_seqs < 0 || p->n_seqs > INT32_MAX || p->table_width < 0 || p->n_pages < 0 || p->page_size < 1 || p->n_heads < 1 || p->n_kv_heads < 1 ||
         p->n_heads % p->n_kv_heads || (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)) return GQ_ERR_SHAPE;
     if (!p->q_starts && p->T && (p->n_seqs == 0 || p->T % p->n_seqs)) return GQ_ERR_SHAPE;
-    if (p->n_heads > 65535 || p->T > (1 << 24) || p->table_width > (1 << 30) || p->table_width * p->page_size > (1 << 30)) return GQ_ERR_LIMIT;
+    if (p->n_heads > 65535 || p->T > (1 << 24) || p->T * (p->n_heads / p->n_kv_heads) >= (1 << 30) || p->table_width > (1 << 30) || p->table_width * p->page_size > (1 << 30)) return GQ_ERR_LIMIT;
     return GQ_OK;
 }
 static int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
@@ -133,15 +133,15 @@ template <int D, int RG, int KG, int S> static int attention(const gq_attention_
     using Shape = PagedShape<D, RG, KG, S>;
     int blocks = 0;
     if (const int rc = resident_blocks<paged_attention_kernel<D, RG, KG, S>>(Shape::THREADS, Shape::SMEM, &blocks)) return rc;
-    const int64_t slots = 2 * (int64_t)blocks * Shape::ROWS, at_stats = up256((p->n_seqs + 1) * 8), at_parts = at_stats + up256(slots * 8);
+    const int64_t slots = 2 * (int64_t)blocks * Shape::ROWS, at_parts = up256(slots * 8);
     *bytes = at_parts + slots * D * 4;
     if (!status) return GQ_OK;
     if (!p->workspace || !aligned(p->workspace, 256) || p->workspace_bytes < *bytes) return GQ_ERR_WORKSPACE;
     uint8_t *ws = (uint8_t *)p->workspace;
     uint32_t log2 = 0;
     while ((int64_t)1 << log2 < p->page_size) ++log2;
-    PagedParams q{*p, status, (int64_t *)ws, (float2 *)(ws + at_stats), (float *)(ws + at_parts), p->n_heads / p->n_kv_heads, blocks, (int)(p->table_width * p->page_size),
-                  p->page_size % 16 == 0 && p->k_strides[1] < (1 << 27) && p->v_strides[1] < (1 << 27),
+    PagedParams q{*p, status, (float2 *)ws, (float *)(ws + at_parts), p->n_heads / p->n_kv_heads, blocks, (int)(p->table_width * p->page_size),
+                  p->q_starts ? 0 : (int)(p->T / p->n_seqs), p->page_size % 16 == 0 && p->k_strides[1] < (1 << 27) && p->v_strides[1] < (1 << 27),
                   (uint32_t)(((uint64_t)1 << (31 + log2)) / p->page_size + 1), 31 + log2, p->scale * 1.4426950408889634f};
     if (p->n_pages == 0) {       // every page is outside the cache: nothing is read, but addresses are formed
         q.a.k_pages = q.a.v_pages = p->q;
@@ -149,7 +149,7 @@ template <int D, int RG, int KG, int S> static int attention(const gq_attention_
     }
     GQ_CUDA(launch_pdl(paged_attention_kernel<D, RG, KG, S>, dim3(blocks), Shape::THREADS, Shape::SMEM, stream, q));
     GQ_LAUNCHED();
-    GQ_CUDA(launch_pdl(join_parts_kernel<D>, dim3((unsigned)p->T, p->n_heads), 128, 0, stream, q, Shape::ROWS, Shape::UNIT));
+    GQ_CUDA(launch_pdl(join_parts_kernel<D, Shape::ROWS, Shape::UNIT>, dim3(blocks), JOIN_WARPS * 32, 0, stream, q));
     GQ_LAUNCHED();
     return GQ_OK;
 }
@@ -166,7 +166,7 @@ static int attention_by_shape(const gq_attention_args *p, int64_t *bytes, int *s
         case 256 * 8 + 1: return attention<256, 1, 4, 3>(p, bytes, status, stream);
         case 256 * 8 + 2: return attention<256, 2, 4, 3>(p, bytes, status, stream);
         case 256 * 8 + 3: return attention<256, 3, 4, 2>(p, bytes, status, stream);
-        default: return attention<256, 4, 3, 2>(p, bytes, status, stream);
+        default: return attention<256, 4, 2, 3>(p, bytes, status, stream);
     }
 }
 

@@ -20,10 +20,10 @@ namespace gq {
 struct PagedParams {
     gq_attention_args a;
     int *status;
-    int64_t *first;         // workspace: [n_seqs] first unit of each sequence, then W
-    float2 *stats;          // [2 G][rows of a tile]: maximum, sum
+    float2 *stats;          // workspace: [2 G][rows of a tile]: maximum, sum
     float *parts;           // [2 G][rows of a tile][head_dim]
     int group, blocks, max_keys;        // query heads of a kv head; blocks the GPU holds; keys that the page table has room for
+    int per_seq;            // tokens of a sequence where all have the same
     int whole;              // pages hold whole stages of 16 keys
     uint32_t page_mul, page_shift;      // key / page_size = key * page_mul >> page_shift, for keys below 2^31
     float scale2;           // scale * log2 e
@@ -83,21 +83,26 @@ __device__ __forceinline__ SeqSpan seq_span(const PagedParams &p, int64_t s) {
         const int64_t q0 = min(max((int64_t)a.q_starts[s], (int64_t)0), a.T), q1 = min(max((int64_t)a.q_starts[s + 1], q0), a.T);
         v.tok0 = q0; v.n = (int)(q1 - q0);
     } else {
-        v.n = (int)(a.T / a.n_seqs); v.tok0 = s * v.n;
+        v.n = p.per_seq; v.tok0 = s * v.n;
     }
     v.len = min(max(a.lens[s], 0), p.max_keys + v.n);      // with more keys than the table has, every token sees a missing one
     return v;
 }
-// keys that a tile's last row sees
+// keys that a tile's last row sees (a sequence's rows, its tokens times the group, are fewer than 2^30)
 __device__ __forceinline__ int tile_keys(const SeqSpan &v, int tile, int rows, int group) {
-    const int last = min(v.n - 1, (int)(((int64_t)(tile + 1) * rows - 1) / group));
-    return max(0, v.len - v.n + last + 1);
+    const int last = min(v.n, (int)(((unsigned)(tile + 1) * rows - 1) / (unsigned)group) + 1);       // tokens up to the tile's last
+    return max(0, v.len - v.n + last);
 }
-__device__ __forceinline__ int tiles_of(const SeqSpan &v, int rows, int group) { return (int)(((int64_t)v.n * group + rows - 1) / rows); }
+__device__ __forceinline__ int tiles_of(const SeqSpan &v, int rows, int group) { return (int)(((unsigned)v.n * group + rows - 1) / rows); }
 __device__ __forceinline__ int64_t head_units(const SeqSpan &v, int rows, int group, int unit) {
+    if (v.n * group <= rows) return v.n ? (unsigned)(v.len + unit - 1) / unit : 0;
     int64_t u = 0;
-    for (int t = 0, n = tiles_of(v, rows, group); t < n; ++t) u += (tile_keys(v, t, rows, group) + unit - 1) / unit;
+    for (int t = 0, n = tiles_of(v, rows, group); t < n; ++t) u += (unsigned)(tile_keys(v, t, rows, group) + unit - 1) / unit;
     return u;
+}
+// n / d, in 32 bits where both fit: the 64-bit division is a hundred instructions
+__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
+    return ((uint64_t)n | (uint64_t)d) >> 32 ? (int64_t)((uint64_t)n / (uint64_t)d) : (int64_t)((uint32_t)n / (uint32_t)d);
 }
 
 // Where a block's walk over the line of units stands: the segment (sequence, kv head, tile) and the next unit in it
@@ -129,12 +134,75 @@ template <int ROWS, int UNIT> __device__ __forceinline__ void next_segment(const
     } while (c.units == 0);
 }
 
+// The line of all units as one warp sees it: lane l counts the sequences [l each, (l + 1) each)
+struct Line {
+    int64_t mine, upto, total;      // units of this lane's sequences, of those and all before, of all
+    int64_t s0, s1;
+};
+template <int ROWS, int UNIT> __device__ __forceinline__ Line count_units(const PagedParams &p, int lane) {
+    Line l;
+    const int64_t each = (p.a.n_seqs + 31) / 32;
+    l.s0 = min(lane * each, p.a.n_seqs);
+    l.s1 = min(l.s0 + each, p.a.n_seqs);
+    l.mine = 0;
+    for (int64_t s = l.s0; s < l.s1; ++s) l.mine += head_units(seq_span(p, s), ROWS, p.group, UNIT) * p.a.n_kv_heads;
+    l.upto = l.mine;
+    for (int o = 1; o < 32; o *= 2) {
+        const int64_t v = __shfl_up_sync(~0u, l.upto, o);
+        if (lane >= o) l.upto += v;
+    }
+    l.total = __shfl_sync(~0u, l.upto, 31);
+    return l;
+}
+// How the line is cut: block c's units are [start(c), start(c + 1)), the first `more` blocks have one more than the others
+struct Cut {
+    int64_t each, more, blocks;
+    __device__ __forceinline__ int64_t start(int64_t c) const { return min(c, blocks) * each + min(c, more); }
+    __device__ __forceinline__ int64_t block_of(int64_t x) const {
+        const int64_t large = more * (each + 1);
+        return x < large ? quotient(x, each + 1) : more + quotient(x - large, max(each, (int64_t)1));
+    }
+};
+__device__ __forceinline__ Cut cut_line(const PagedParams &p, int64_t total) {
+    Cut c;
+    c.blocks = p.blocks;
+    c.each = quotient(total, c.blocks);
+    c.more = total - c.each * c.blocks;
+    return c;
+}
+// the segment of unit x of the line (0 <= x < total)
+template <int ROWS, int UNIT> __device__ __forceinline__ void locate(const PagedParams &p, const Line &l, int64_t x, int lane, Cursor &c) {
+    const int owner = __ffs(__ballot_sync(~0u, x < l.upto)) - 1;
+    int64_t seq = 0, in = 0;
+    if (lane == owner) {
+        in = x - (l.upto - l.mine);
+        for (seq = l.s0;; ++seq) {
+            const int64_t u = head_units(seq_span(p, seq), ROWS, p.group, UNIT) * p.a.n_kv_heads;
+            if (in < u) break;
+            in -= u;
+        }
+    }
+    c.seq = __shfl_sync(~0u, seq, owner);
+    in = __shfl_sync(~0u, in, owner);
+    c.v = seq_span(p, c.seq);
+    c.tiles = tiles_of(c.v, ROWS, p.group);
+    const int64_t per_head = head_units(c.v, ROWS, p.group, UNIT);
+    c.head = (int)quotient(in, per_head);
+    in -= c.head * per_head;
+    c.tile = 0;
+    load_segment<ROWS, UNIT>(p, c);
+    while (in >= c.units) { in -= c.units; ++c.tile; load_segment<ROWS, UNIT>(p, c); }
+    c.unit = (int)in;
+}
+
 template <int D, int RG, int KG, int S> struct PagedShape {
     static constexpr int THREADS = 32 * RG * KG, ROWS = 8 * RG, UNIT = 16 * KG;
     static constexpr int PITCH = D * 2 + 16;                                    // bytes of a row in shared memory: eight rows' chunks in different banks
     static constexpr int STAGE = 2 * 16 * PITCH;                                // keys and values of 16 keys
-    static constexpr int RING = KG * S * STAGE, MERGE = KG > 1 ? ROWS * D * 4 : 0, STATS = KG > 1 ? KG * ROWS * 8 : 0;
-    static constexpr int SMEM = RING + MERGE + STATS + RG * KG * 256;
+    static constexpr int TURNS = RG > 2 ? 2 : 1;                                // a key group's output goes through the stage it used last, in as many turns
+    static constexpr int RING = KG * S * STAGE, STATS = KG > 1 ? KG * ROWS * 8 : 0;
+    static_assert(ROWS * D * 4 / TURNS <= STAGE && (D / 16) % (KG * TURNS) == 0, "the key groups share the dimensions of an output out");
+    static constexpr int SMEM = RING + STATS + RG * KG * 256;
 };
 
 template <int D, int RG, int KG, int S>
@@ -142,58 +210,34 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
     using Shape = PagedShape<D, RG, KG, S>;
     constexpr int ROWS = Shape::ROWS, UNIT = Shape::UNIT, STAGE = Shape::STAGE, PITCH = Shape::PITCH, CH = D / 8, MT = D / 16, WARPS = RG * KG;
     extern __shared__ __align__(128) uint8_t smem[];
-    float *merge = (float *)(smem + Shape::RING);
-    float2 *stat_sm = (float2 *)((uint8_t *)merge + Shape::MERGE);
+    float2 *stat_sm = (float2 *)(smem + Shape::RING);
     longlong2 *row_sm = (longlong2 *)((uint8_t *)stat_sm + Shape::STATS);       // [warp][16]: bytes to the keys and values of the stage being asked for
-    __shared__ int64_t scan[WARPS], place[3];
     const gq_attention_args &a = p.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, rg = warp % RG, kg = warp / RG, g = lane / 4, t = lane % 4;
     pdl_wait();
     pdl_trigger();
 
-    // ---- this block's units ----
-    int64_t total, w0, w1;
+    // ---- this block's units (every warp counts for itself) ----
     Cursor use;
+    int64_t w0, w1;
     {
-        const int64_t each = (a.n_seqs + Shape::THREADS - 1) / Shape::THREADS, s0 = min(tid * each, a.n_seqs), s1 = min(s0 + each, a.n_seqs);
-        int64_t mine = 0;
-        for (int64_t s = s0; s < s1; ++s) mine += head_units(seq_span(p, s), ROWS, p.group, UNIT) * a.n_kv_heads;
-        int64_t upto = mine;
-        for (int o = 1; o < 32; o *= 2) {
-            const int64_t v = __shfl_up_sync(~0u, upto, o);
-            if (lane >= o) upto += v;
-        }
-        if (lane == 31) scan[warp] = upto;
-        __syncthreads();
-        total = 0;
-        for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) upto += scan[w];
-            total += scan[w];
-        }
-        const int64_t blocks = min((int64_t)p.blocks, max(total, (int64_t)1));
-        w0 = blockIdx.x < blocks ? blockIdx.x * total / blocks : total;
-        w1 = blockIdx.x < blocks ? (blockIdx.x + 1) * total / blocks : total;
-        int64_t at = upto - mine;
-        if (blockIdx.x == 0 || (w0 < w1 && w0 >= at && w0 < upto))
-            for (int64_t s = s0; s < s1; ++s) {
-                const int64_t u = head_units(seq_span(p, s), ROWS, p.group, UNIT);
-                if (blockIdx.x == 0) p.first[s] = at;
-                if (w0 < w1 && w0 >= at && w0 < at + u * a.n_kv_heads) { place[0] = s; place[1] = (w0 - at) / u; place[2] = (w0 - at) % u; }
-                at += u * a.n_kv_heads;
-            }
-        if (blockIdx.x == 0 && tid == 0) p.first[a.n_seqs] = total;
-        if (w0 == w1) return;
-        __syncthreads();
-        use.seq = place[0];
-        use.head = (int)place[1];
-        int64_t in = place[2];
-        use.v = seq_span(p, use.seq);
-        use.tiles = tiles_of(use.v, ROWS, p.group);
-        use.tile = 0;
-        load_segment<ROWS, UNIT>(p, use);
-        while (in >= use.units) { in -= use.units; ++use.tile; load_segment<ROWS, UNIT>(p, use); }
-        use.unit = (int)in;
+        const Line line = count_units<ROWS, UNIT>(p, lane);
+        const Cut cut = cut_line(p, line.total);
+        w0 = cut.start(blockIdx.x);
+        w1 = cut.start(blockIdx.x + 1);
+        if (w0 < w1) locate<ROWS, UNIT>(p, line, w0, lane, use);
     }
+    // tokens that see no key: their tiles have no units, and belong to the last blocks, which are idle first
+    auto zeros = [&]() {
+        for (int64_t s = gridDim.x - 1 - blockIdx.x; s < a.n_seqs; s += gridDim.x) {
+            const SeqSpan v = seq_span(p, s);
+            for (int tile = 0, n = tiles_of(v, ROWS, p.group); tile < n && tile_keys(v, tile, ROWS, p.group) == 0; ++tile)
+                for (int r = tile * ROWS, end = min(r + ROWS, v.n * p.group); r < end; ++r)
+                    for (int i = tid; i < a.n_kv_heads * D; i += Shape::THREADS)
+                        ((__nv_bfloat16 *)a.out)[(v.tok0 + r / p.group) * a.out_strides[0] + ((i / D) * p.group + r % p.group) * a.out_strides[1] + i % D] = __float2bfloat16_rn(0.0f);
+        }
+    };
+    if (w0 == w1) { zeros(); return; }
     const int count = (int)(w1 - w0);
 
     // ---- loads: a stage of this key group is 16 keys ----
@@ -271,7 +315,9 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
     };
     heads();
     look();
+#pragma unroll 1
     for (int i = 0; i < S - 1; ++i) ask(i);
+    zeros();
 
     // Transposed products: keys (or dimensions) on M, the eight query rows of the warp on N.  A lane holds, of a score tile, keys g and g + 8 of queries 2 t and 2 t + 1; of the
     // output, dimensions 16 i + g and 16 i + g + 8 of the same two queries.
@@ -289,16 +335,16 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
             for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-            const int64_t rows = (int64_t)use.v.n * p.group, row0 = (int64_t)use.tile * ROWS + rg * 8;
+            const int rows = use.v.n * p.group, row0 = use.tile * ROWS + rg * 8;
             const int before = use.v.len - use.v.n + 1;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 top[j] = -INFINITY;
                 sum[j] = 0.0f;
-                lim[j] = before + (int)(min(row0 + 2 * t + j, rows - 1) / p.group);
+                lim[j] = before + (unsigned)min(row0 + 2 * t + j, rows - 1) / (unsigned)p.group;
             }
-            lim_first = before + (int)(((int64_t)use.tile * ROWS) / p.group);
-            const int64_t r = row0 + g, i = r / p.group;
+            lim_first = before + (unsigned)(use.tile * ROWS) / (unsigned)p.group;
+            const int r = row0 + g, i = (unsigned)r / (unsigned)p.group;
             const uint32_t *src = (const uint32_t *)((const __nv_bfloat16 *)a.q + (use.v.tok0 + i) * a.q_strides[0] + (use.head * p.group + (r - i * p.group)) * a.q_strides[1]) + t;
 #pragma unroll
             for (int x = 0; x < MT; ++x)
@@ -416,68 +462,88 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
         for (int j = 0; j < 2; ++j)
 #pragma unroll
             for (int x = 4; x < 32; x *= 2) sum[j] += __shfl_xor_sync(~0u, sum[j], x);
+        constexpr int MINE = MT / KG, TURNS = Shape::TURNS;       // dimension tiles that a key group adds up, the turns of the exchange
+        float sum_o[MINE][4];
         if constexpr (KG > 1) {
             if (g == 0)
                 for (int j = 0; j < 2; ++j) stat_sm[kg * ROWS + rg * 8 + 2 * t + j] = make_float2(top[j], sum[j]);
-            __syncthreads();
-            float keep[2];
+            const int used = (slot == 0 ? S - 1 : slot - 1) * STAGE;
+            if constexpr (RG > 1) asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * RG) : "memory");      // nobody reads that stage any more
+            else __syncwarp();
+            float keep[KG][2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float2 *st = stat_sm + rg * 8 + 2 * t + j;
-                float m = -INFINITY, l = 0.0f;
-                for (int x = 0; x < KG; ++x) m = fmaxf(m, st[x * ROWS].x);
-                const float r = m == -INFINITY ? 0.0f : m;
-                for (int x = 0; x < KG; ++x) l += st[x * ROWS].y * ex2(st[x * ROWS].x - r);
-                keep[j] = ex2(top[j] - r);
-                top[j] = m;
-                sum[j] = l;
-            }
+            for (int h = 0; h < TURNS; ++h) {
+                float4 *box = (float4 *)(smem + kg * S * STAGE + used) + rg * 2 * D / TURNS + lane;
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[i][j] *= keep[j & 1];
-            float4 *box = (float4 *)merge + rg * 2 * D + lane;
-            for (int x = KG - 1; x > 0; --x) {
-                if (kg == x)
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) box[i * 32] = make_float4(o[i][0], o[i][1], o[i][2], o[i][3]);
+                for (int i = 0; i < MT / TURNS; ++i) {
+                    const float(&v)[4] = o[h * (MT / TURNS) + i];
+                    box[i * 32] = make_float4(v[0], v[1], v[2], v[3]);
+                }
                 __syncthreads();
-                if (kg == x - 1)
+                if (h == 0) {
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        const float4 v = box[i * 32];
-                        o[i][0] += v.x; o[i][1] += v.y; o[i][2] += v.z; o[i][3] += v.w;
+                    for (int j = 0; j < 2; ++j) {
+                        const float2 *st = stat_sm + rg * 8 + 2 * t + j;
+                        float m = -INFINITY;
+                        for (int x = 0; x < KG; ++x) m = fmaxf(m, st[x * ROWS].x);
+                        const float r = m == -INFINITY ? 0.0f : m;
+                        top[j] = m;
+                        sum[j] = 0.0f;
+#pragma unroll
+                        for (int x = 0; x < KG; ++x) {
+                            keep[x][j] = ex2(st[x * ROWS].x - r);
+                            sum[j] += st[x * ROWS].y * keep[x][j];
+                        }
                     }
-                __syncthreads();
+                }
+#pragma unroll
+                for (int i = 0; i < MINE / TURNS; ++i) {
+                    float(&v)[4] = sum_o[h * (MINE / TURNS) + i];
+                    v[0] = v[1] = v[2] = v[3] = 0.0f;
+#pragma unroll
+                    for (int x = 0; x < KG; ++x) {
+                        const float4 w = ((const float4 *)(smem + x * S * STAGE + used))[rg * 2 * D / TURNS + (i * KG + kg) * 32 + lane];
+                        v[0] += w.x * keep[x][0]; v[1] += w.y * keep[x][1]; v[2] += w.z * keep[x][0]; v[3] += w.w * keep[x][1];
+                    }
+                }
+                __syncthreads();            // the next turn, or the next stage, comes to the same place
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < MINE; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sum_o[i][j] = o[i][j];
         }
-        if (kg == 0) {
+        auto dim_of = [&](int i) { return ((i / (MINE / TURNS)) * (MT / TURNS) + (i % (MINE / TURNS)) * KG + kg) * 16 + g; };       // of sum_o[i][0], [1]; 8 more: of [2], [3]
+        {
             const bool whole = unit0 == 0 && use.unit == use.units;
-            const int64_t part = 2 * (int64_t)blockIdx.x + (unit0 == 0), rows = (int64_t)use.v.n * p.group;
+            const int64_t part = 2 * (int64_t)blockIdx.x + (unit0 == 0);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int64_t r = (int64_t)use.tile * ROWS + rg * 8 + 2 * t + j;
-                if (r >= rows) continue;
+                const int r = use.tile * ROWS + rg * 8 + 2 * t + j;
+                if (r >= use.v.n * p.group) continue;
                 if (whole) {
-                    const int64_t tok = use.v.tok0 + r / p.group, h = use.head * p.group + r % p.group;
-                    __nv_bfloat16 *dst = (__nv_bfloat16 *)a.out + tok * a.out_strides[0] + h * a.out_strides[1] + g;
-                    const __nv_bfloat16 *gate = a.gate ? (const __nv_bfloat16 *)a.gate + tok * a.gate_strides[0] + h * a.gate_strides[1] + g : nullptr;
+                    const int i0 = (unsigned)r / (unsigned)p.group;
+                    const int64_t tok = use.v.tok0 + i0, h = use.head * p.group + (r - i0 * p.group);
+                    __nv_bfloat16 *dst = (__nv_bfloat16 *)a.out + tok * a.out_strides[0] + h * a.out_strides[1];
+                    const __nv_bfloat16 *gate = a.gate ? (const __nv_bfloat16 *)a.gate + tok * a.gate_strides[0] + h * a.gate_strides[1] : nullptr;
                     const float inv = sum[j] == 0.0f ? 0.0f : 1.0f / sum[j];
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
+                    for (int i = 0; i < MINE; ++i)
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
-                            float v = o[i][2 * x + j] * inv;
-                            if (gate) v /= 1.0f + ex2(-1.4426950408889634f * __bfloat162float(gate[i * 16 + x * 8]));
-                            dst[i * 16 + x * 8] = __float2bfloat16_rn(v);
+                            const int d = dim_of(i) + 8 * x;
+                            float v = sum_o[i][2 * x + j] * inv;
+                            if (gate) v /= 1.0f + ex2(-1.4426950408889634f * __bfloat162float(gate[d]));
+                            dst[d] = __float2bfloat16_rn(v);
                         }
                 } else {
                     const int64_t at = part * ROWS + rg * 8 + 2 * t + j;
-                    if (g == 0) p.stats[at] = make_float2(top[j], sum[j]);
+                    if (g == 0 && kg == 0) p.stats[at] = make_float2(top[j], sum[j]);
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
+                    for (int i = 0; i < MINE; ++i)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) p.parts[at * D + i * 16 + x * 8 + g] = o[i][2 * x + j];
+                        for (int x = 0; x < 2; ++x) p.parts[at * D + dim_of(i) + 8 * x] = sum_o[i][2 * x + j];
                 }
             }
         }
@@ -487,74 +553,75 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
     cp_async_wait<0>();
 }
 
-// The rows whose keys lie in several blocks' ranges, or that see none: one block of 128 threads to a token's query head, its threads in sets of head_dim / 4 that
-// take the parts in turn.
-template <int D>
-__global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__ PagedParams p, int rows_of_tile, int unit) {
-    constexpr int LANES = D / 4, SETS = 128 / LANES;
-    __shared__ float4 acc[SETS][LANES];
-    __shared__ float red[4];
+// The segments that several blocks worked on: block c joins the one that starts in block c's range and ends behind it, a warp to a row and a share of its parts.  All but the
+// parts themselves is found before the wait for the blocks that write them.
+constexpr int JOIN_WARPS = 8;      // 256 threads of 64 registers fit beside the blocks of the kernel in front
+template <int D, int ROWS, int UNIT>
+__global__ void __launch_bounds__(JOIN_WARPS * 32) join_parts_kernel(const __grid_constant__ PagedParams p) {
+    constexpr int SETS = JOIN_WARPS / 8, V = D / 32;          // warps to a row, values to a lane
+    __shared__ float box[JOIN_WARPS][D], sums[JOIN_WARPS];
     const gq_attention_args &a = p.a;
-    const int64_t tok = blockIdx.x;
-    const int h = blockIdx.y, kvh = h / p.group, set = threadIdx.x / LANES, at4 = threadIdx.x % LANES;
-    pdl_wait();
-    int64_t s = 0;
-    if (a.q_starts) {
-        int64_t hi = a.n_seqs;                    // the last sequence that starts at or before the token
-        while (s + 1 < hi) {
-            const int64_t mid = (s + hi) / 2;
-            if (a.q_starts[mid] <= tok) s = mid; else hi = mid;
-        }
-    } else s = tok / (a.T / a.n_seqs);
-    const SeqSpan v = seq_span(p, s);
-    if (tok < v.tok0 || tok >= v.tok0 + v.n) return;          // nobody's row
-    const int64_t row = (tok - v.tok0) * p.group + h % p.group;
-    const int tile = (int)(row / rows_of_tile);
-    int64_t first = p.first[s] + (int64_t)kvh * head_units(v, rows_of_tile, p.group, unit);
-    for (int i = 0; i < tile; ++i) first += (tile_keys(v, i, rows_of_tile, p.group) + unit - 1) / unit;
-    const int64_t units = (tile_keys(v, tile, rows_of_tile, p.group) + unit - 1) / unit, total = p.first[a.n_seqs];
-    const int64_t blocks = min((int64_t)p.blocks, max(total, (int64_t)1));
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float sum = 0.0f;
-    if (units > 0) {
-        const int64_t c0 = ((first + 1) * blocks - 1) / total, c1 = min(((first + units) * blocks - 1) / total, blocks - 1);
-        if (c0 == c1) return;                     // finished by its block
-        const int64_t r = row % rows_of_tile;
-        auto part = [&](int64_t c) { return (2 * c + (c == c0)) * rows_of_tile + r; };
-        float top = -INFINITY;
-        for (int64_t c = c0 + threadIdx.x; c <= c1; c += 128) top = fmaxf(top, p.stats[part(c)].x);
-        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x / 32] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll 4
-        for (int64_t c = c0 + set; c <= c1; c += SETS) {
-            const int64_t q = part(c);
-            const float2 st = p.stats[q];
-            const float4 w = *(const float4 *)(p.parts + q * D + at4 * 4);
-            const float f = ex2(st.x - ref);
-            sum += f * st.y;
-            o.x += f * w.x; o.y += f * w.y; o.z += f * w.z; o.w += f * w.w;
-        }
-        __shared__ float sums[SETS];
-        acc[set][at4] = o;
-        if (at4 == 0) sums[set] = sum;
-        __syncthreads();
-        if (set) return;
-        for (int x = 1; x < SETS; ++x) {
-            const float4 w = acc[x][at4];
-            o.x += w.x; o.y += w.y; o.z += w.z; o.w += w.w;
-            sum += sums[x];
-        }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, set = warp / 8;
+    int64_t end;            // the block of the segment's last unit
+    Cursor c;
+    {
+        const Line line = count_units<ROWS, UNIT>(p, lane);
+        const Cut cut = cut_line(p, line.total);
+        const int64_t w0 = cut.start(blockIdx.x), w1 = cut.start(blockIdx.x + 1);
+        if (w0 == w1) return;
+        locate<ROWS, UNIT>(p, line, w1 - 1, lane, c);
+        const int64_t first = w1 - 1 - c.unit;
+        if (first < w0 || first + c.units == w1) return;
+        end = min(cut.block_of(first + c.units - 1), cut.blocks - 1);
     }
-    if (set) return;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const float val[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
-    __nv_bfloat16 *dst = (__nv_bfloat16 *)a.out + tok * a.out_strides[0] + h * a.out_strides[1] + at4 * 4;
-    const __nv_bfloat16 *gate = a.gate ? (const __nv_bfloat16 *)a.gate + tok * a.gate_strides[0] + h * a.gate_strides[1] + at4 * 4 : nullptr;
+    const int rows = min(ROWS, c.v.n * p.group - c.tile * ROWS);
+    pdl_wait();
+    for (int r = warp % 8; r < ROWS; r += 8) {
+        float o[V], sum = 0.0f, top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) dst[i] = __float2bfloat16_rn(gate ? val[i] / (1.0f + ex2(-1.4426950408889634f * __bfloat162float(gate[i]))) : val[i]);
+        for (int i = 0; i < V; ++i) o[i] = 0.0f;
+        if (r < rows) {
+            auto part = [&](int64_t b) { return (2 * b + (b == (int64_t)blockIdx.x)) * ROWS + r; };
+            // a first look at all maxima, so that the parts can be added in any order of arrival without being scaled again
+            for (int64_t b = blockIdx.x + lane; b <= end; b += 32) top = fmaxf(top, p.stats[part(b)].x);
+            for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+            const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll 8
+            for (int64_t b = blockIdx.x + set; b <= end; b += SETS) {
+                const int64_t at = part(b);
+                const float2 st = p.stats[at];
+                const float f = ex2(st.x - ref);
+                sum += f * st.y;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] += f * p.parts[at * D + i * 32 + lane];
+            }
+        }
+        if (set) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) box[warp][i * 32 + lane] = o[i];
+            if (lane == 0) sums[warp] = sum;
+        }
+        __syncthreads();
+        if (set == 0 && r < rows) {
+            for (int x = 1; x < SETS; ++x) {
+                sum += sums[warp + 8 * x];
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] += box[warp + 8 * x][i * 32 + lane];
+            }
+            const int row = c.tile * ROWS + r, i0 = (unsigned)row / (unsigned)p.group;
+            const int64_t tok = c.v.tok0 + i0, h = c.head * p.group + (row - i0 * p.group);
+            __nv_bfloat16 *dst = (__nv_bfloat16 *)a.out + tok * a.out_strides[0] + h * a.out_strides[1] + lane;
+            const __nv_bfloat16 *gate = a.gate ? (const __nv_bfloat16 *)a.gate + tok * a.gate_strides[0] + h * a.gate_strides[1] + lane : nullptr;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float v = o[i] * inv;
+                if (gate) v /= 1.0f + ex2(-1.4426950408889634f * __bfloat162float(gate[i * 32]));
+                dst[i * 32] = __float2bfloat16_rn(v);
+            }
+        }
+        __syncthreads();
+    }
 }
 
 }  // namespace gq
