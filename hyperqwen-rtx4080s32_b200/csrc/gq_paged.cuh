@@ -553,15 +553,16 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
     cp_async_wait<0>();
 }
 
-// The segments that several blocks worked on: block c joins the one that starts in block c's range and ends behind it, a warp to a row and a share of its parts.  All but the
-// parts themselves is found before the wait for the blocks that write them.
-constexpr int JOIN_WARPS = 8;      // 256 threads of 64 registers fit beside the blocks of the kernel in front
+// The segments that several blocks worked on: block c joins the one that starts in block c's range and ends behind it, each row by as many warps as there are, four parts of
+// a warp in flight.  All but the parts themselves is found before the wait for the blocks that write them.
+constexpr int JOIN_WARPS = 16;
 template <int D, int ROWS, int UNIT>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) join_parts_kernel(const __grid_constant__ PagedParams p) {
-    constexpr int SETS = JOIN_WARPS / 8, V = D / 32;          // warps to a row, values to a lane
-    __shared__ float box[JOIN_WARPS][D], sums[JOIN_WARPS];
+    constexpr int V = D / 32;                                   // values to a lane
+    __shared__ float box[JOIN_WARPS][D];
+    __shared__ float2 box_stats[JOIN_WARPS];
     const gq_attention_args &a = p.a;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, set = warp / 8;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
     int64_t end;            // the block of the segment's last unit
     Cursor c;
     {
@@ -574,40 +575,57 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_parts_kernel(const __gri
         if (first < w0 || first + c.units == w1) return;
         end = min(cut.block_of(first + c.units - 1), cut.blocks - 1);
     }
-    const int rows = min(ROWS, c.v.n * p.group - c.tile * ROWS);
+    const int rows = min(ROWS, c.v.n * p.group - c.tile * ROWS), sets = max(JOIN_WARPS / rows, 1), set = warp / min(rows, JOIN_WARPS);
     pdl_wait();
-    for (int r = warp % 8; r < ROWS; r += 8) {
+    for (int r0 = 0; r0 < rows; r0 += JOIN_WARPS) {
+        const int r = r0 + (rows < JOIN_WARPS ? warp % rows : warp);
+        const bool mine = r < rows && set < sets;
         float o[V], sum = 0.0f, top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < V; ++i) o[i] = 0.0f;
-        if (r < rows) {
-            auto part = [&](int64_t b) { return (2 * b + (b == (int64_t)blockIdx.x)) * ROWS + r; };
-            // a first look at all maxima, so that the parts can be added in any order of arrival without being scaled again
-            for (int64_t b = blockIdx.x + lane; b <= end; b += 32) top = fmaxf(top, p.stats[part(b)].x);
-            for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-            const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll 8
-            for (int64_t b = blockIdx.x + set; b <= end; b += SETS) {
-                const int64_t at = part(b);
-                const float2 st = p.stats[at];
-                const float f = ex2(st.x - ref);
-                sum += f * st.y;
+        if (mine)
+            for (int64_t b = (int64_t)blockIdx.x + set; b <= end; b += 4 * sets) {
+                float2 st[4];
+                float v[4][V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) o[i] += f * p.parts[at * D + i * 32 + lane];
+                for (int x = 0; x < 4; ++x) {
+                    const int64_t of = b + x * sets, at = (2 * of + (of == (int64_t)blockIdx.x)) * ROWS + r;
+                    const bool is = of <= end;
+                    st[x] = is ? __ldcg(p.stats + at) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) v[x][i] = is ? __ldcg(p.parts + at * D + i * 32 + lane) : 0.0f;
+                }
+                const float next = fmaxf(fmaxf(fmaxf(st[0].x, st[1].x), fmaxf(st[2].x, st[3].x)), top), ref = next == -INFINITY ? 0.0f : next, keep = ex2(top - ref);
+                top = next;
+                sum *= keep;
+#pragma unroll
+                for (int i = 0; i < V; ++i) o[i] *= keep;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float f = ex2(st[x].x - ref);
+                    sum += f * st[x].y;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[i] += f * v[x][i];
+                }
             }
-        }
-        if (set) {
+        if (sets > 1) {
+            if (set > 0 && mine) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) box[warp][i * 32 + lane] = o[i];
-            if (lane == 0) sums[warp] = sum;
-        }
-        __syncthreads();
-        if (set == 0 && r < rows) {
-            for (int x = 1; x < SETS; ++x) {
-                sum += sums[warp + 8 * x];
-#pragma unroll
-                for (int i = 0; i < V; ++i) o[i] += box[warp + 8 * x][i * 32 + lane];
+                for (int i = 0; i < V; ++i) box[warp][i * 32 + lane] = o[i];
+                if (lane == 0) box_stats[warp] = make_float2(top, sum);
             }
+            __syncthreads();
+            if (set == 0 && mine)
+                for (int x = 1; x < sets; ++x) {
+                    const float2 st = box_stats[warp + rows * x];
+                    const float next = fmaxf(st.x, top), ref = next == -INFINITY ? 0.0f : next, keep = ex2(top - ref), f = ex2(st.x - ref);
+                    top = next;
+                    sum = sum * keep + st.y * f;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) o[i] = o[i] * keep + box[warp + rows * x][i * 32 + lane] * f;
+                }
+        }
+        if (set == 0 && mine) {
             const int row = c.tile * ROWS + r, i0 = (unsigned)row / (unsigned)p.group;
             const int64_t tok = c.v.tok0 + i0, h = c.head * p.group + (row - i0 * p.group);
             __nv_bfloat16 *dst = (__nv_bfloat16 *)a.out + tok * a.out_strides[0] + h * a.out_strides[1] + lane;
@@ -620,7 +638,6 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_parts_kernel(const __gri
                 dst[i * 32] = __float2bfloat16_rn(v);
             }
         }
-        __syncthreads();
     }
 }
 
