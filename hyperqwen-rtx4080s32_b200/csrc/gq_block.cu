@@ -25,6 +25,16 @@ static int status_word(int **p) {
     return GQ_OK;
 }
 
+// Launches a kernel that begins with griddepcontrol.wait while the kernel in front of it ends.
+template <class... P, class... A> static cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, int smem, void *stream, A... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t)stream; cfg.attrs = &attr; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // ---- low-rank adapters -------------------------------------------------------------------------------
 
 static int check_low_rank(const gq_low_rank_args *p, int64_t *n_total) {
@@ -75,7 +85,7 @@ extern "C" int gq_head_norm_rope(const gq_head_norm_args *p, void *stream) {
     if (p->T == 0) return GQ_OK;
     const int64_t width = ((int64_t)p->n_heads * (p->gated ? 2 : 1) + 2 * (int64_t)p->n_kv_heads) * p->head_dim;
     if (!p->qkv || !p->q_out || !p->positions || (p->rotary_dim && !p->inv_freq) || (p->positions_bytes != 4 && p->positions_bytes != 8) || p->ld_qkv < width) return GQ_ERR_ARG;
-    if (!aligned(p->q_out, 16) || !aligned(p->q_norm, 16) || !aligned(p->k_norm, 16)) return GQ_ERR_ARG;
+    if (!aligned(p->qkv, 16) || p->ld_qkv % 8 || !aligned(p->q_out, 16) || !aligned(p->q_norm, 16) || !aligned(p->k_norm, 16)) return GQ_ERR_ARG;
     if (store) {
         if (!p->k_pages || !p->v_pages || !p->slots || (p->slots_bytes != 4 && p->slots_bytes != 8) || p->k_out || !aligned(p->k_pages, 16) || !aligned(p->v_pages, 16)) return GQ_ERR_ARG;
         for (int i = 0; i < 3; ++i)
@@ -83,7 +93,16 @@ extern "C" int gq_head_norm_rope(const gq_head_norm_args *p, void *stream) {
     } else if (!p->k_out || !aligned(p->k_out, 16)) return GQ_ERR_ARG;
     int *status;
     if (const int rc = status_word(&status)) return rc;
-    head_norm_kernel<<<dim3((unsigned)p->T, p->n_heads + (store ? 2 : 1) * p->n_kv_heads), 64, 0, (cudaStream_t)stream>>>(*p, status);
+    if (p->head_dim % 16 || (!p->interleaved && p->rotary_dim % 16)) {
+        GQ_CUDA(launch_pdl(head_norm_any_kernel, dim3((unsigned)p->T, p->n_heads + (store ? 2 : 1) * p->n_kv_heads), 64, 0, stream, *p, status));
+    } else {
+        int group = 1;                                                       // lanes of a head, a power of two
+        while (group * 16 < p->head_dim) group *= 2;
+        const int batch = p->T >= 2048 ? HEAD_BATCH : 1;                     // few tokens: a block each
+        const unsigned blocks = (unsigned)((p->T + batch - 1) / batch);
+        if (p->interleaved) GQ_CUDA(launch_pdl(head_norm_kernel<true>, dim3(blocks), HEAD_THREADS, 0, stream, *p, batch, group, status));
+        else GQ_CUDA(launch_pdl(head_norm_kernel<false>, dim3(blocks), HEAD_THREADS, 0, stream, *p, batch, group, status));
+    }
     GQ_LAUNCHED();
     return GQ_OK;
 }
@@ -99,16 +118,6 @@ static int check_attention(const gq_attention_args *p) {
     return GQ_OK;
 }
 static int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
-
-// Launches a kernel that begins with griddepcontrol.wait while the kernel in front of it ends.
-template <class... P, class... A> static cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, int smem, void *stream, A... args) {
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t)stream; cfg.attrs = &attr; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
 
 // blocks of a kernel that the current device holds at once; its shared memory is allowed on the way (asked once per device)
 template <auto KERNEL> static int resident_blocks(int threads, int smem, int *blocks) {

@@ -311,7 +311,7 @@ int gq_low_rank_add(const gq_low_rank_args *args, void *stream);
  * The angle is reduced in 64 bits, so positions may be large.  qkv holds n_heads heads of queries (each followed by a gate of the same
  * size if gated: it is left alone), n_kv_heads of keys, n_kv_heads of values.  head_dim is a multiple of 8 up to 512, rotary_dim even (0: no rotation).
  * A negative slot stores nothing; one beyond the cache stores nothing and sets device status 2.  Two tokens of one slot: either may be kept.
- * out and the pages share no memory with qkv; pages and their strides start at multiples of 16 bytes. */
+ * The outputs and the pages share no memory with qkv; rows of qkv, rows and heads of pages, outputs and weights start at multiples of 16 bytes. */
 typedef struct gq_head_norm_args {
     const void *qkv;             /* bf16 [T, n_heads * head_dim * (gated ? 2 : 1) + 2 * n_kv_heads * head_dim], row stride ld_qkv */
     const void *positions;       /* int32 or int64 [T] */
