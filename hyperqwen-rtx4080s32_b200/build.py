@@ -19,7 +19,7 @@ OBJ_DIR = os.path.join(CSRC, "_generated")
 EXT_SOURCE = os.path.join(CSRC, "gq_torch.cpp")
 EXT_STAMP = os.path.join(CSRC, "_generated", "gq_torch.stamp")     # what the extension was compiled against
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))) + [os.path.join("..", "..", "include", "gq_b200.h")]
-BLOCK_HEADERS = ["gq_adapters.cuh", "gq_heads.cuh", "gq_paged.cuh"]      # read by gq_block.cu alone
+BLOCK_HEADERS = ["gq_adapters.cuh", "gq_bf16.cuh", "gq_heads.cuh", "gq_paged.cuh"]      # read by gq_block.cu alone
 UNIT_HEADERS = {"gq_b200.cu": [h for h in HEADERS if h not in BLOCK_HEADERS],
                 "gq_block.cu": BLOCK_HEADERS + ["gq_common.cuh", "gq_host.h", "gq_layout.h", HEADERS[-1]]}
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "--expt-relaxed-constexpr", "-diag-suppress", "177",

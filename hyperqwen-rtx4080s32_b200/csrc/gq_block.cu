@@ -38,7 +38,7 @@ template <class... P, class... A> static cudaError_t launch_pdl(void (*kernel)(P
 // ---- low-rank adapters -------------------------------------------------------------------------------
 
 static int check_low_rank(const gq_low_rank_args *p, int64_t *n_total) {
-    if (!p || p->M < 0 || p->M > INT32_MAX || p->K <= 0 || p->K % GQ_QK || p->rank <= 0 || p->rank % 8 || p->n_adapters <= 0) return p ? GQ_ERR_SHAPE : GQ_ERR_ARG;
+    if (!p || p->M < 0 || p->M > (1 << 22) || p->K <= 0 || p->K % GQ_QK || p->K > (1 << 24) || p->rank <= 0 || p->rank % 8 || p->n_adapters <= 0) return p ? GQ_ERR_SHAPE : GQ_ERR_ARG;
     if (p->rank > GQ_MAX_RANK || p->n_shards < 1 || p->n_shards > GQ_MAX_DEVICE_SHARDS) return GQ_ERR_LIMIT;
     *n_total = 0;
     for (int s = 0; s < p->n_shards; ++s) {
@@ -47,10 +47,18 @@ static int check_low_rank(const gq_low_rank_args *p, int64_t *n_total) {
     }
     return *n_total > INT32_MAX ? GQ_ERR_SHAPE : GQ_OK;
 }
+static int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
+static int ranks_of(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
+// adapters that a tile of rows may hold, and the parts that K is cut into: enough blocks for the GPU, a part of 8 steps of 32 at least
+static int low_rank_groups(const gq_low_rank_args *p) { return (int)std::min<int64_t>(std::min<int64_t>(p->M, LR_ROWS), p->n_adapters); }
+static int low_rank_parts(const gq_low_rank_args *p) {
+    const int64_t tiles = (p->M + LR_ROWS - 1) / LR_ROWS, blocks = tiles * (tiles == 1 ? low_rank_groups(p) : 1);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, p->K / 256), 296 / std::max<int64_t>(blocks, 1)));
+}
 extern "C" int64_t gq_low_rank_workspace_bytes(const gq_low_rank_args *p) {
     int64_t n = 0;
     if (const int rc = check_low_rank(p, &n)) return rc;
-    return p->M * p->n_shards * p->rank * 4;
+    return n == 0 ? 0 : p->M * p->n_shards * ranks_of(p->rank) * low_rank_parts(p) * 4;
 }
 extern "C" int gq_low_rank_add(const gq_low_rank_args *p, void *stream) {
     int64_t n = 0;
@@ -58,17 +66,33 @@ extern "C" int gq_low_rank_add(const gq_low_rank_args *p, void *stream) {
     if (p->M == 0 || n == 0) return GQ_OK;
     if (!p->base || !p->x || !p->a || !p->b || !p->scales || !p->ids || !p->out || (p->ids_bytes != 4 && p->ids_bytes != 8)) return GQ_ERR_ARG;
     if (!aligned(p->x, 16) || !aligned(p->a, 16) || !aligned(p->b, 16) || p->ldx % 8 || p->ldx < p->K || p->ld_base < n || p->ld_out < n) return GQ_ERR_ARG;
-    if (p->workspace_bytes < gq_low_rank_workspace_bytes(p) || !p->workspace) return GQ_ERR_WORKSPACE;
+    if (p->workspace_bytes < gq_low_rank_workspace_bytes(p) || !p->workspace || !aligned(p->workspace, 256)) return GQ_ERR_WORKSPACE;
     int *status;
     if (const int rc = status_word(&status)) return rc;
+    const int ranks = ranks_of(p->rank), parts = low_rank_parts(p), groups = low_rank_groups(p);
+    const int64_t tiles = (p->M + LR_ROWS - 1) / LR_ROWS;
+    bool vec = aligned(p->base, 16) && aligned(p->out, 16) && p->ld_base % 8 == 0 && p->ld_out % 8 == 0;
     LowRankParams q{(const __nv_bfloat16 *)p->base, (const __nv_bfloat16 *)p->x, (const __nv_bfloat16 *)p->a, (const __nv_bfloat16 *)p->b, p->scales, p->ids,
-                    (__nv_bfloat16 *)p->out, (float *)p->workspace, p->K, p->ld_base, p->ldx, p->ld_out, n, {0},
-                    (int)p->M, p->n_shards, p->n_adapters, p->rank, p->ids_bytes == 8};
-    for (int s = 0; s < p->n_shards; ++s) q.edges[s + 1] = q.edges[s] + p->n_outs[s];
-    const int64_t values = p->M * p->n_shards * p->rank;
-    low_rank_inner_kernel<<<(unsigned)((values + 7) / 8), 256, 0, (cudaStream_t)stream>>>(q);
+                    (__nv_bfloat16 *)p->out, (float *)p->workspace, status, p->ld_base, p->ldx, p->ld_out, n, {0},
+                    (int)p->M, (int)p->K, p->n_shards, p->n_adapters, p->rank, ranks, parts, p->ids_bytes == 8, 0, 0};
+    for (int s = 0; s < p->n_shards; ++s) {
+        q.edges[s + 1] = q.edges[s] + p->n_outs[s];
+        vec = vec && q.edges[s] % 8 == 0;
+    }
+    q.vec = vec;
+    q.cols = tiles * (n / 256) < 1024 ? 256 : 1024;
+    int64_t blocks = 0;
+    for (int s = 0; s < p->n_shards; ++s) blocks += (p->n_outs[s] + q.cols - 1) / q.cols;
+    if (tiles > 65535) return GQ_ERR_LIMIT;
+    GQ_CUDA(launch_pdl(low_rank_inner_kernel, dim3(parts, (unsigned)tiles, tiles == 1 ? groups : 1), LR_THREADS, 0, stream, q));
     GQ_LAUNCHED();
-    low_rank_outer_kernel<<<dim3((unsigned)p->M, (unsigned)((n + 255) / 256)), 256, 0, (cudaStream_t)stream>>>(q, status);
+    const dim3 grid((unsigned)blocks, (unsigned)tiles, tiles == 1 ? (unsigned)std::max<int64_t>(1, std::min<int64_t>(groups, 888 / blocks)) : 1);
+    switch (ranks) {
+        case 16: GQ_CUDA(launch_pdl(low_rank_outer_kernel<1>, grid, LR_THREADS, 0, stream, q)); break;
+        case 32: GQ_CUDA(launch_pdl(low_rank_outer_kernel<2>, grid, LR_THREADS, 0, stream, q)); break;
+        case 64: GQ_CUDA(launch_pdl(low_rank_outer_kernel<4>, grid, LR_THREADS, 0, stream, q)); break;
+        default: GQ_CUDA(launch_pdl(low_rank_outer_kernel<8>, grid, LR_THREADS, 0, stream, q));
+    }
     GQ_LAUNCHED();
     return GQ_OK;
 }
@@ -117,8 +141,6 @@ static int check_attention(const gq_attention_args *p) {
     if (p->n_heads > 65535 || p->T > (1 << 24) || p->T * (p->n_heads / p->n_kv_heads) >= (1 << 30) || p->table_width > (1 << 30) || p->table_width * p->page_size > (1 << 30)) return GQ_ERR_LIMIT;
     return GQ_OK;
 }
-static int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
-
 // blocks of a kernel that the current device holds at once; its shared memory is allowed on the way (asked once per device)
 template <auto KERNEL> static int resident_blocks(int threads, int smem, int *blocks) {
     static std::atomic<int> known[64];

@@ -13,7 +13,7 @@
 // accumulators are the A operand of p v.  p enters as two bf16 parts (p and what its rounding left): one part would add an error as large as the output's own rounding, and the tensor pipe has room.
 // tcgen05 has nothing to give here: 16 rows of its 128 would be used, and the loads are the bound.
 #pragma once
-#include "gq_common.cuh"
+#include "gq_bf16.cuh"
 
 namespace gq {
 
@@ -42,21 +42,10 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    uint32_t u;
-    memcpy(&u, &v, 4);
-    return u;
 }
 // two probabilities as bf16 and what that rounding left, as bf16
 __device__ __forceinline__ void bf16_parts(float lo, float hi, uint32_t &big, uint32_t &small) {
