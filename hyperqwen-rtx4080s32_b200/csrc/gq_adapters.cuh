@@ -28,17 +28,18 @@ struct LowRankParams {
 __device__ __forceinline__ int64_t id_at(const void *ids, int wide, int64_t i) { return wide ? ((const int64_t *)ids)[i] : ((const int32_t *)ids)[i]; }
 
 // The rows of a tile by adapter: list[start[s]] .. list[start[s + 1] - 1] are those of the s-th adapter that occurs (-1: none, -2: an id outside the bank)
-struct RowGroups {
-    int id_of_row[LR_ROWS], first[LR_ROWS], list[LR_ROWS], start[LR_ROWS + 1], id[LR_ROWS], groups;
+struct alignas(16) RowGroups {
+    int id_of_row[LR_ROWS], size[LR_ROWS];         // size: of the group that a row is the first of, else 0
+    int list[LR_ROWS], start[LR_ROWS + 1], id[LR_ROWS], groups;
 };
 __device__ __forceinline__ void group_rows(const LowRankParams &p, int row0, RowGroups &g) {
     const int tid = threadIdx.x, n = min(LR_ROWS, p.M - row0);
-    int mine = 0;
+    int mine = INT32_MIN;                // rows behind the last form a group of their own, the last one
     if (tid < n) {
         const int64_t id = id_at(p.ids, p.wide_ids, row0 + tid);
         mine = id == -1 ? -1 : id < 0 || id >= p.n_adapters ? -2 : (int)id;
-        g.id_of_row[tid] = mine;
     }
+    if (tid < LR_ROWS) g.id_of_row[tid] = mine;
     __syncthreads();
     const bool same = __syncthreads_and(tid >= n || mine == g.id_of_row[0]);
     if (same) {                          // the usual case of a long chunk
@@ -47,31 +48,42 @@ __device__ __forceinline__ void group_rows(const LowRankParams &p, int row0, Row
         __syncthreads();
         return;
     }
-    int f = 0;
-    if (tid < n) {
-        while (g.id_of_row[f] != mine) ++f;
-        g.first[tid] = f;
+    uint64_t equal = 0;                  // the rows of this row's adapter
+    if (tid < LR_ROWS) {
+#pragma unroll
+        for (int j = 0; j < LR_ROWS; j += 4) {
+            const int4 v = *(const int4 *)(g.id_of_row + j);
+            equal |= (uint64_t)((v.x == mine) | (v.y == mine) << 1 | (v.z == mine) << 2 | (v.w == mine) << 3) << j;
+        }
+        g.size[tid] = __ffsll(equal) - 1 == tid ? __popcll(equal) : 0;
     }
     __syncthreads();
-    if (tid < n) {
-        int place = 0, group = 0;
-        for (int j = 0; j < n; ++j) {
-            const int fj = g.first[j];
-            place += fj < f || (fj == f && j < tid);
-            group += fj == j && j < f;
+    if (tid < LR_ROWS) {
+        const int f = __ffsll(equal) - 1;
+        int before = 0, group = 0;       // rows and groups whose first row stands in front of this group's
+#pragma unroll
+        for (int j = 0; j < LR_ROWS; j += 4) {
+            const int4 v = *(const int4 *)(g.size + j);
+            before += (j < f ? v.x : 0) + (j + 1 < f ? v.y : 0) + (j + 2 < f ? v.z : 0) + (j + 3 < f ? v.w : 0);
+            group += (j < f && v.x) + (j + 1 < f && v.y) + (j + 2 < f && v.z) + (j + 3 < f && v.w);
         }
-        g.list[place] = tid;
-        if (f == tid) { g.start[group] = place; g.id[group] = mine; }
-        if (place == n - 1) { g.start[group + 1] = n; g.groups = group + 1; }
+        if (tid < n) {
+            const int place = before + __popcll(equal & (((uint64_t)1 << tid) - 1));
+            g.list[place] = tid;
+            if (f == tid) { g.start[group] = place; g.id[group] = mine; }
+            if (place == n - 1) { g.start[group + 1] = n; g.groups = group + 1; }
+        }
     }
     __syncthreads();
 }
 
-// The sums over part blockIdx.x of K of a tile's inner products.  Ranks on M, rows on N.  A warp takes 16 rows and up to 64 ranks; warps that are not needed for rows share the steps
-// of 32 k, and their sums are added in order through shared memory.
+// The sums over part blockIdx.x of K of a tile's inner products.  Ranks on M, rows on N.  A warp takes 16 rows and 16 MT ranks at a time; warps that are not needed for rows share the steps
+// of 32 k, and their sums are added in order through shared memory.  Lanes without a row or a rank read another's: what they compute is not looked at, and no load waits behind a branch.
+template <int MT>
 __global__ void __launch_bounds__(LR_THREADS) low_rank_inner_kernel(const __grid_constant__ LowRankParams p) {
     __shared__ RowGroups groups;
-    __shared__ float red[LR_WARPS][16][68];
+    constexpr int PITCH = MT * 16 + 4;
+    __shared__ float red[LR_WARPS][16][PITCH];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane % 4;
     const int row0 = blockIdx.y * LR_ROWS, steps = p.K / 32, per_shard = (p.rank + 15) / 16, tiles = p.n_shards * per_shard;
     const int step0 = (int)((int64_t)blockIdx.x * steps / p.parts), step1 = (int)((int64_t)(blockIdx.x + 1) * steps / p.parts);
@@ -86,31 +98,29 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_inner_kernel(const __grid
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int r = rw * 16 + j * 8 + g;
-            x[j] = r < count ? p.x + (int64_t)(row0 + groups.list[at + r]) * p.ldx + t * 8 : nullptr;
+            x[j] = p.x + (int64_t)(row0 + groups.list[at + min(r, count - 1)]) * p.ldx + t * 8;
         }
-        for (int tile0 = 0; tile0 < tiles; tile0 += 4) {
-            const __nv_bfloat16 *a[4][2];
+        for (int tile0 = 0; tile0 < tiles; tile0 += MT) {
+            const __nv_bfloat16 *a[MT][2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int tile = tile0 + i, shard = tile / per_shard, r = (tile - shard * per_shard) * 16 + j * 8 + g;
-                    a[i][j] = tile < tiles && r < p.rank ? p.a + ((int64_t)id * p.n_shards * p.rank + shard * p.rank + r) * p.K + t * 8 : nullptr;
+                    const int tile = min(tile0 + i, tiles - 1), shard = tile / per_shard, r = min((tile - shard * per_shard) * 16 + j * 8 + g, p.rank - 1);
+                    a[i][j] = p.a + ((int64_t)id * p.n_shards * p.rank + shard * p.rank + r) * p.K + t * 8;
                 }
-            float acc[4][2][4] = {};
-            const int here = min(tiles - tile0, 4);
+            float acc[MT][2][4] = {};
 #pragma unroll 2
             for (int step = step0 + kw; step < step1; step += k_warps) {
-                uint4 xv[2], av[4][2];
+                uint4 xv[2], av[MT][2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) xv[j] = x[j] ? *(const uint4 *)(x[j] + step * 32) : make_uint4(0, 0, 0, 0);
+                for (int j = 0; j < 2; ++j) xv[j] = *(const uint4 *)(x[j] + step * 32);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) av[i][j] = a[i][j] ? *(const uint4 *)(a[i][j] + step * 32) : make_uint4(0, 0, 0, 0);
+                    for (int j = 0; j < 2; ++j) av[i][j] = *(const uint4 *)(a[i][j] + step * 32);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (i >= here) break;
+                for (int i = 0; i < MT; ++i) {
                     const uint32_t lo[4] = {av[i][0].x, av[i][1].x, av[i][0].y, av[i][1].y}, hi[4] = {av[i][0].z, av[i][1].z, av[i][0].w, av[i][1].w};
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
@@ -120,15 +130,15 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_inner_kernel(const __grid
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) red[warp][j * 8 + t * 2 + (e & 1)][i * 16 + g + (e >> 1) * 8] = acc[i][j][e];
             __syncthreads();
-            for (int i = tid; i < row_warps * 16 * 64; i += LR_THREADS) {
-                const int c = i % 64, r = i / 64, tile = tile0 + c / 16;
-                if (r >= count || tile >= tiles) continue;
+            for (int i = tid; i < count * MT * 16; i += LR_THREADS) {
+                const int r = i / (MT * 16), c = i - r * (MT * 16), tile = tile0 + c / 16;
+                if (tile >= tiles) continue;
                 float sum = 0.0f;
                 for (int k = 0; k < k_warps; ++k) sum += red[k * row_warps + r / 16][r % 16][c];
                 const int shard = tile / per_shard, rank = (tile - shard * per_shard) * 16 + c % 16;
@@ -157,6 +167,7 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_outer_kernel(const __grid
     }
     const int64_t col0 = p.edges[shard] + block * p.cols;
     const int ncols = (int)min((int64_t)p.cols, p.edges[shard + 1] - col0);
+    const bool vec = p.vec && ncols >= 8;
     pdl_wait();
     pdl_trigger();
     group_rows(p, row0, groups);
@@ -188,35 +199,40 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_outer_kernel(const __grid
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int n = n0 + 8 * (g / 2) + 2 * i + (g & 1);
-                const __nv_bfloat16 *src = n < ncols ? p.b + ((int64_t)id * p.n_total + col0 + n) * p.rank : nullptr;
+                const __nv_bfloat16 *src = p.b + ((int64_t)id * p.n_total + col0 + min(n, ncols - 1)) * p.rank;
                 if constexpr (KS == 1) {
-                    const uint2 v = src && t * 4 < p.rank ? *(const uint2 *)(src + t * 4) : make_uint2(0, 0);
-                    bf[i][0][0] = v.x; bf[i][0][1] = v.y;
+                    const bool in = t * 4 < p.rank;            // ranks that only fill the tile are zero here and in the inner values
+                    const uint2 v = *(const uint2 *)(src + (in ? t * 4 : 0));
+                    bf[i][0][0] = in ? v.x : 0u; bf[i][0][1] = in ? v.y : 0u;
                 } else {
 #pragma unroll
                     for (int k = 0; k < KS; k += 2) {
-                        const uint4 v = src && k * 16 + t * 8 < p.rank ? *(const uint4 *)(src + k * 16 + t * 8) : make_uint4(0, 0, 0, 0);
-                        bf[i][k][0] = v.x; bf[i][k][1] = v.y; bf[i][k + 1][0] = v.z; bf[i][k + 1][1] = v.w;
+                        const bool in = k * 16 + t * 8 < p.rank;
+                        const uint4 v = *(const uint4 *)(src + (in ? k * 16 + t * 8 : 0));
+                        bf[i][k][0] = in ? v.x : 0u; bf[i][k][1] = in ? v.y : 0u; bf[i][k + 1][0] = in ? v.z : 0u; bf[i][k + 1][1] = in ? v.w : 0u;
                     }
                 }
             }
             for (int m0 = 0; m0 < count; m0 += 16) {
                 const int n = n0 + t * 8;
-                const bool have[2] = {m0 + g < count && n < ncols, m0 + g + 8 < count && n < ncols}, whole = p.vec && n + 8 <= ncols;
+                const bool have[2] = {m0 + g < count && n < ncols, m0 + g + 8 < count && n < ncols}, whole = n + 8 <= ncols;
                 int64_t m[2];
                 uint4 old[2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    m[j] = have[j] ? row0 + groups.list[at + m0 + g + 8 * j] : 0;
-                    const __nv_bfloat16 *src = p.base + m[j] * p.ld_base + col0 + n;
-                    if (have[j] && whole) old[j] = *(const uint4 *)src;
-                    else if (have[j]) {
+                for (int j = 0; j < 2; ++j) m[j] = row0 + groups.list[at + min(m0 + g + 8 * j, count - 1)];
+                if (vec) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) old[j] = *(const uint4 *)(p.base + m[j] * p.ld_base + col0 + (whole ? n : 0));       // of an eighth that ends early: below
+                }
+                if (!vec || !whole)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const __nv_bfloat16 *src = p.base + m[j] * p.ld_base + col0;
                         uint16_t e[8];
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) e[x] = n + x < ncols ? __bfloat16_as_ushort(src[x]) : 0;
+                        for (int x = 0; x < 8; ++x) e[x] = __bfloat16_as_ushort(src[min(n + x, ncols - 1)]);
                         memcpy(&old[j], e, 16);
                     }
-                }
                 float acc[4][4] = {};
 #pragma unroll
                 for (int k = 0; k < KS; k += KS == 1 ? 1 : 2) {
@@ -250,7 +266,7 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_outer_kernel(const __grid
 #pragma unroll
                     for (int i = 0; i < 4; ++i) y[i] = bf16_pair(__uint_as_float(w[i] << 16) + acc[i][2 * j], __uint_as_float(w[i] & 0xffff0000u) + acc[i][2 * j + 1]);
                     __nv_bfloat16 *dst = p.out + m[j] * p.ld_out + col0 + n;
-                    if (whole) *(uint4 *)dst = make_uint4(y[0], y[1], y[2], y[3]);
+                    if (vec && whole) *(uint4 *)dst = make_uint4(y[0], y[1], y[2], y[3]);
                     else {
 #pragma unroll
                         for (int x = 0; x < 8; ++x)

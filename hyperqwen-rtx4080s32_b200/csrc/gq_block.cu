@@ -84,7 +84,14 @@ extern "C" int gq_low_rank_add(const gq_low_rank_args *p, void *stream) {
     int64_t blocks = 0;
     for (int s = 0; s < p->n_shards; ++s) blocks += (p->n_outs[s] + q.cols - 1) / q.cols;
     if (tiles > 65535) return GQ_ERR_LIMIT;
-    GQ_CUDA(launch_pdl(low_rank_inner_kernel, dim3(parts, (unsigned)tiles, tiles == 1 ? groups : 1), LR_THREADS, 0, stream, q));
+    const dim3 inner(parts, (unsigned)tiles, tiles == 1 ? groups : 1);
+    const int rank_tiles = p->n_shards * ((p->rank + 15) / 16);              // a warp's turn: as many as divide them, up to four
+    switch (rank_tiles <= 4 ? rank_tiles : rank_tiles % 4 && rank_tiles % 3 == 0 ? 3 : 4) {
+        case 1: GQ_CUDA(launch_pdl(low_rank_inner_kernel<1>, inner, LR_THREADS, 0, stream, q)); break;
+        case 2: GQ_CUDA(launch_pdl(low_rank_inner_kernel<2>, inner, LR_THREADS, 0, stream, q)); break;
+        case 3: GQ_CUDA(launch_pdl(low_rank_inner_kernel<3>, inner, LR_THREADS, 0, stream, q)); break;
+        default: GQ_CUDA(launch_pdl(low_rank_inner_kernel<4>, inner, LR_THREADS, 0, stream, q));
+    }
     GQ_LAUNCHED();
     const dim3 grid((unsigned)blocks, (unsigned)tiles, tiles == 1 ? (unsigned)std::max<int64_t>(1, std::min<int64_t>(groups, 888 / blocks)) : 1);
     switch (ranks) {
