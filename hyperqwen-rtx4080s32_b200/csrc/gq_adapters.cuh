@@ -1,7 +1,7 @@
 // Low-rank adapters beside a shared projection: out = base + scale * B (A x) for each row's own adapter.
 //
 // Rows are taken in tiles of 64; a block sorts its tile's rows by adapter, and every adapter that occurs multiplies its own rows only, so no row's sums ever hold another adapter's numbers and
-// rows of one adapter need not stand together.  Two launches: the inner products A x, their sums over parts of K left in the workspace, and the outer products B (A x) with the addition.
+// rows of one adapter need not stand together.  Two launches: the inner products A x, K split over the blocks of a cluster, left in the workspace, and the outer products B (A x) with the addition.
 // Both read bf16 operands from global memory straight into the fragments of mma.sync m16n8k16: any order of k serves as long as both operands have the same, so a lane takes 8
 // neighbours (16 bytes) where the instruction names scattered ones.  Bound by bytes: in decode those of the adapters (latency below a few MB), in prefill those of base and out;
 // the ranks are too small for tcgen05's 128 rows to be filled.
@@ -12,17 +12,23 @@ namespace gq {
 
 constexpr int LR_ROWS = 64, LR_THREADS = 256, LR_WARPS = LR_THREADS / 32;
 
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 struct LowRankParams {
     const __nv_bfloat16 *base, *x, *a, *b;
     const float *scales;
     const void *ids;
     __nv_bfloat16 *out;
-    float *inner;                // workspace: [parts][M][n_shards * ranks], scaled
+    __nv_bfloat16 *big, *small;  // workspace: the scaled inner values [M, n_shards * ranks] as bf16, and what that rounding left
     int *status;
     int64_t ld_base, ldx, ld_out, n_total;
     int64_t edges[9];            // first column of each shard, and the end
     int M, K, n_shards, n_adapters, rank, ranks, parts, wide_ids;       // ranks: the rank as the outer products see it, 16, 32, 64 or 128
-    int cols, vec;               // columns of an outer block; base and out can be read and written 16 bytes at a time
+    int vec;                     // base and out can be read and written 16 bytes at a time
 };
 
 __device__ __forceinline__ int64_t id_at(const void *ids, int wide, int64_t i) { return wide ? ((const int64_t *)ids)[i] : ((const int32_t *)ids)[i]; }
@@ -86,7 +92,7 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_inner_kernel(const __grid
     __shared__ float red[LR_WARPS][16][PITCH];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane % 4;
     const int row0 = blockIdx.y * LR_ROWS, steps = p.K / 32, per_shard = (p.rank + 15) / 16, tiles = p.n_shards * per_shard;
-    const int step0 = (int)((int64_t)blockIdx.x * steps / p.parts), step1 = (int)((int64_t)(blockIdx.x + 1) * steps / p.parts);
+    const int step0 = (int)((int64_t)blockIdx.x * (steps / 2) / p.parts) * 2, step1 = (int)((int64_t)(blockIdx.x + 1) * (steps / 2) / p.parts) * 2;      // pairs
     pdl_wait();
     pdl_trigger();
     group_rows(p, row0, groups);
@@ -110,24 +116,31 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_inner_kernel(const __grid
                     a[i][j] = p.a + ((int64_t)id * p.n_shards * p.rank + shard * p.rank + r) * p.K + t * 8;
                 }
             float acc[MT][2][4] = {};
-#pragma unroll 2
-            for (int step = step0 + kw; step < step1; step += k_warps) {
-                uint4 xv[2], av[MT][2];
+            // two steps at a time, the 128 bytes of a row that lie side by side
+#pragma unroll(MT <= 2 ? 2 : 1)
+            for (int step = step0 + 2 * kw; step < step1; step += 2 * k_warps) {
+                uint4 xv[2][2], av[2][MT][2];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) xv[j] = *(const uint4 *)(x[j] + step * 32);
+                for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+                    for (int j = 0; j < 2; ++j) xv[h][j] = *(const uint4 *)(x[j] + (step + h) * 32);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) av[i][j] = *(const uint4 *)(a[i][j] + step * 32);
+                    for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const uint32_t lo[4] = {av[i][0].x, av[i][1].x, av[i][0].y, av[i][1].y}, hi[4] = {av[i][0].z, av[i][1].z, av[i][0].w, av[i][1].w};
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        mma_bf16(acc[i][j], lo, xv[j].x, xv[j].y);
-                        mma_bf16(acc[i][j], hi, xv[j].z, xv[j].w);
-                    }
+                        for (int j = 0; j < 2; ++j) av[h][i][j] = *(const uint4 *)(a[i][j] + (step + h) * 32);
                 }
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const uint4 a0 = av[h][i][0], a1 = av[h][i][1];
+                        const uint32_t lo[4] = {a0.x, a1.x, a0.y, a1.y}, hi[4] = {a0.z, a1.z, a0.w, a1.w};
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            mma_bf16(acc[i][j], lo, xv[h][j].x, xv[h][j].y);
+                            mma_bf16(acc[i][j], hi, xv[h][j].z, xv[h][j].w);
+                        }
+                    }
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i)
@@ -136,146 +149,299 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_inner_kernel(const __grid
 #pragma unroll
                     for (int e = 0; e < 4; ++e) red[warp][j * 8 + t * 2 + (e & 1)][i * 16 + g + (e >> 1) * 8] = acc[i][j][e];
             __syncthreads();
+            // over the warps of this block, then over the blocks of the cluster, both in order
             for (int i = tid; i < count * MT * 16; i += LR_THREADS) {
+                const int r = i / (MT * 16), c = i - r * (MT * 16);
+                float sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < LR_WARPS; ++k)
+                    if (k < k_warps) sum += red[k * row_warps + r / 16][r % 16][c];
+                red[r / 16][r % 16][c] = sum;              // read by this thread alone so far
+            }
+            if (p.parts > 1) cluster_sync_all();
+            else __syncthreads();
+            for (int i = tid + blockIdx.x * LR_THREADS; i < count * MT * 16; i += LR_THREADS * p.parts) {
                 const int r = i / (MT * 16), c = i - r * (MT * 16), tile = tile0 + c / 16;
                 if (tile >= tiles) continue;
                 float sum = 0.0f;
-                for (int k = 0; k < k_warps; ++k) sum += red[k * row_warps + r / 16][r % 16][c];
+                if (p.parts > 1) {
+                    const uint32_t at = smem_u32(&red[r / 16][r % 16][c]);
+                    for (int k0 = 0; k0 < p.parts; k0 += 8) {
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v[k] = k0 + k < p.parts ? ld_cluster_f32(map_to_rank(at, k0 + k)) : 0.0f;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) sum += v[k];
+                    }
+                } else sum = red[r / 16][r % 16][c];
                 const int shard = tile / per_shard, rank = (tile - shard * per_shard) * 16 + c % 16;
-                p.inner[((int64_t)blockIdx.x * p.M + row0 + groups.list[at + r]) * (p.n_shards * p.ranks) + shard * p.ranks + rank] = sum * p.scales[id * p.n_shards + shard];
+                sum *= p.scales[id * p.n_shards + shard];
+                const int64_t to = (int64_t)(row0 + groups.list[at + r]) * (p.n_shards * p.ranks) + shard * p.ranks + rank;
+                const __nv_bfloat16 big = __float2bfloat16_rn(sum);
+                p.big[to] = big;
+                p.small[to] = __float2bfloat16_rn(sum - __bfloat162float(big));
             }
-            __syncthreads();
+            if (p.parts > 1) cluster_sync_all();            // nobody reads this block's sums any more
+            else __syncthreads();
         }
     }
 }
 
-// base + B (A x) in `cols` columns of one shard.  Rows on M, columns on N; the inner values enter as two bf16 parts (the value and what its rounding left: one part would add an error as
-// large as the output's rounding).  A warp takes 32 columns, whose order over its four MMAs gives a lane eight neighbours: base and out move 16 bytes at a time.
-template <int KS>
-__global__ void __launch_bounds__(LR_THREADS) low_rank_outer_kernel(const __grid_constant__ LowRankParams p) {
-    constexpr int R = KS * 16, PITCH = R + 8;
-    __shared__ RowGroups groups;
-    __shared__ __align__(16) __nv_bfloat16 big[LR_ROWS][PITCH], small[LR_ROWS][PITCH];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane % 4, row0 = blockIdx.y * LR_ROWS;
+// base + B (A x), the outer products.  Rows on M, columns on N; the inner values enter as two bf16 parts (the value and what its rounding left: one part would add an error as large as the
+// output's rounding).  A warp takes 32 columns, whose order over its four MMAs gives a lane eight neighbours, so that base and out move 16 bytes at a time; the base is what the accumulators
+// start from.  A tile of 16 rows that has several adapters is multiplied once with each and keeps that one's rows.
+
+// a warp's 32 columns of adapter `id` as B operands: of shard columns n0 .. of which `here` are real
+template <int KS> __device__ __forceinline__ void load_columns(const LowRankParams &p, int id, int64_t col, int here, int lane, uint32_t (&bf)[4][KS][2]) {
+    const int g = lane / 4, t = lane % 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat16 *src = p.b + ((int64_t)id * p.n_total + col + min(8 * (g / 2) + 2 * i + (g & 1), here - 1)) * p.rank;
+        if constexpr (KS == 1) {
+            const bool in = t * 4 < p.rank;            // ranks that only fill the tile are zero here and in the inner values
+            const uint2 v = *(const uint2 *)(src + (in ? t * 4 : 0));
+            bf[i][0][0] = in ? v.x : 0u; bf[i][0][1] = in ? v.y : 0u;
+        } else {
+#pragma unroll
+            for (int k = 0; k < KS; k += 2) {
+                const bool in = k * 16 + t * 8 < p.rank;
+                const uint4 v = *(const uint4 *)(src + (in ? k * 16 + t * 8 : 0));
+                bf[i][k][0] = in ? v.x : 0u; bf[i][k][1] = in ? v.y : 0u; bf[i][k + 1][0] = in ? v.z : 0u; bf[i][k + 1][1] = in ? v.w : 0u;
+            }
+        }
+    }
+}
+// rows g and g + 8 of the inner values (big and small: where they start) times the columns, onto acc
+template <int KS, class B, class S> __device__ __forceinline__ void add_products(const LowRankParams &p, B big, S small, const uint32_t (&bf)[4][KS][2], int t, float (&acc)[4][4]) {
+#pragma unroll
+    for (int k = 0; k < KS; k += KS == 1 ? 1 : 2) {
+        uint32_t hi[2][4], lo[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if constexpr (KS == 1) {
+                const bool in = t * 4 < p.rank;
+                const uint2 v = *(const uint2 *)(big(j) + t * 4), x = *(const uint2 *)(small(j) + t * 4);
+                hi[0][j] = in ? v.x : 0u; hi[0][j + 2] = in ? v.y : 0u;
+                lo[0][j] = in ? x.x : 0u; lo[0][j + 2] = in ? x.y : 0u;
+            } else {
+                const bool in = k * 16 + t * 8 < p.rank;
+                const uint4 v = *(const uint4 *)(big(j) + k * 16 + t * 8), x = *(const uint4 *)(small(j) + k * 16 + t * 8);
+                hi[0][j] = in ? v.x : 0u; hi[0][j + 2] = in ? v.y : 0u; hi[1][j] = in ? v.z : 0u; hi[1][j + 2] = in ? v.w : 0u;
+                lo[0][j] = in ? x.x : 0u; lo[0][j + 2] = in ? x.y : 0u; lo[1][j] = in ? x.z : 0u; lo[1][j + 2] = in ? x.w : 0u;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < (KS == 1 ? 1 : 2); ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                mma_bf16(acc[i], hi[q], bf[i][k + q][0], bf[i][k + q][1]);
+                mma_bf16(acc[i], lo[q], bf[i][k + q][0], bf[i][k + q][1]);
+            }
+    }
+}
+__device__ __forceinline__ int adapter_of(const LowRankParams &p, int row) {
+    const int64_t id = id_at(p.ids, p.wide_ids, row);
+    return id == -1 ? -1 : id < 0 || id >= p.n_adapters ? -2 : (int)id;
+}
+// eight bf16 values of two rows -> accumulators (columns 8 t + 2 i and the next: of row g in 0, 1, of row g + 8 in 2, 3), and back
+__device__ __forceinline__ void unpack_rows(const uint4 (&w)[2], float (&res)[4][4]) {
+    const uint32_t u[2][4] = {{w[0].x, w[0].y, w[0].z, w[0].w}, {w[1].x, w[1].y, w[1].z, w[1].w}};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) { res[i][2 * j] = __uint_as_float(u[j][i] << 16); res[i][2 * j + 1] = __uint_as_float(u[j][i] & 0xffff0000u); }
+}
+__device__ __forceinline__ uint4 pack_row(const float (&res)[4][4], int j) {
+    return make_uint4(bf16_pair(res[0][2 * j], res[0][2 * j + 1]), bf16_pair(res[1][2 * j], res[1][2 * j + 1]), bf16_pair(res[2][2 * j], res[2][2 * j + 1]),
+                      bf16_pair(res[3][2 * j], res[3][2 * j + 1]));
+}
+// one tile of rows: `mine` is the adapter of row lane & 15, `have` the one whose columns bf holds
+template <int KS, class B, class S> __device__ __forceinline__ void outer_tile(const LowRankParams &p, int mine, int &have, uint32_t (&bf)[4][KS][2], int64_t col, int here, int lane, B big, S small,
+                                                                               float (&res)[4][4], int (&of_row)[2]) {
+    const int g = lane / 4, t = lane % 4;
+    of_row[0] = __shfl_sync(~0u, mine, g);
+    of_row[1] = __shfl_sync(~0u, mine, g + 8);
+    uint32_t todo = __ballot_sync(~0u, mine >= 0) & 0xffffu;
+    while (todo) {
+        const int of = __shfl_sync(~0u, mine, __ffs(todo) - 1);
+        const uint32_t its = __ballot_sync(~0u, mine == of) & 0xffffu;
+        todo &= ~its;
+        if (of != have) {
+            have = of;
+            load_columns<KS>(p, of, col, here, lane, bf);
+        }
+        if (its == 0xffffu) {
+            add_products<KS>(p, big, small, bf, t, res);
+            return;
+        }
+        float acc[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = res[i][j];
+        add_products<KS>(p, big, small, bf, t, acc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) res[i][j] = of_row[j >> 1] == of ? acc[i][j] : res[i][j];
+    }
+    if (__any_sync(~0u, mine == -2)) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (of_row[j >> 1] == -2)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) res[i][j] = __int_as_float(0x7fc00000);
+        if (blockIdx.x == 0 && threadIdx.x == 0) atomicMax(p.status, GQ_DEV_BAD_SHAPE);
+    }
+}
+// which shard's columns block `block` of `cols` has: first of them, and how many
+__device__ __forceinline__ int shard_of(const LowRankParams &p, int64_t block, int cols, int64_t &col0, int &ncols) {
     int shard = 0;
-    int64_t block = blockIdx.x;
-    while (true) {                       // which shard's columns
-        const int64_t n = (p.edges[shard + 1] - p.edges[shard] + p.cols - 1) / p.cols;
+    while (true) {
+        const int64_t n = (p.edges[shard + 1] - p.edges[shard] + cols - 1) / cols;
         if (block < n) break;
         block -= n;
         ++shard;
     }
-    const int64_t col0 = p.edges[shard] + block * p.cols;
-    const int ncols = (int)min((int64_t)p.cols, p.edges[shard + 1] - col0);
-    const bool vec = p.vec && ncols >= 8;
+    col0 = p.edges[shard] + block * cols;
+    ncols = (int)min((int64_t)cols, p.edges[shard + 1] - col0);
+    return shard;
+}
+
+// Decode: a warp by itself has 32 columns of 4 rows (the MMA's others idle): every row may have an adapter of its own, and four of them are not a long way behind one another.
+constexpr int LR_OUTER_WARPS = 4, LR_FEW = 4;
+template <int KS>
+__global__ void __launch_bounds__(LR_OUTER_WARPS * 32) low_rank_few_kernel(const __grid_constant__ LowRankParams p) {
+    const int lane = threadIdx.x & 31, g = lane / 4, t = lane % 4, row0 = blockIdx.y * LR_FEW, last = min(row0 + LR_FEW, p.M) - 1;
+    int64_t col0;
+    int ncols;
+    const int shard = shard_of(p, blockIdx.x, LR_OUTER_WARPS * 32, col0, ncols);
+    col0 += threadIdx.x / 32 * 32;
+    ncols = min(ncols - (int)(threadIdx.x / 32) * 32, 32);
+    const int n = t * 8;
+    const bool full = p.vec && n + 8 <= ncols;                     // this lane's columns: 16 aligned bytes
     pdl_wait();
     pdl_trigger();
-    group_rows(p, row0, groups);
-    for (int s = blockIdx.z; s < groups.groups; s += gridDim.z) {
-        const int id = groups.id[s], at = groups.start[s], count = groups.start[s + 1] - at;
-        if (id < 0) {
-            if (id == -2 && blockIdx.x == 0 && tid == 0) atomicMax(p.status, GQ_DEV_BAD_SHAPE);
-            if (id == -2 || p.out != p.base)
-                for (int i = tid; i < count * ncols; i += LR_THREADS) {
-                    const int64_t m = row0 + groups.list[at + i / ncols], n = col0 + i % ncols;
-                    p.out[m * p.ld_out + n] = id == -2 ? __ushort_as_bfloat16(0x7fc0) : p.base[m * p.ld_base + n];
-                }
-            continue;
-        }
-        for (int i = tid; i < (count + 15) / 16 * 16 * R; i += LR_THREADS) {
-            const int r = i / R, k = i % R;
-            float v = 0.0f;
-            if (r < count && k < p.rank) {
-                const float *src = p.inner + (int64_t)(row0 + groups.list[at + r]) * (p.n_shards * p.ranks) + shard * p.ranks + k;
-                for (int part = 0; part < p.parts; ++part) v += src[(int64_t)part * p.M * (p.n_shards * p.ranks)];
+    if (ncols <= 0) return;
+    const int mine = adapter_of(p, min(row0 + (lane & 15), last));
+    uint4 w[2];
+    w[1] = make_uint4(0, 0, 0, 0);
+    const __nv_bfloat16 *src = p.base + min(row0 + g, last) * p.ld_base + col0 + n;
+    if (full) w[0] = *(const uint4 *)src;
+    else {
+        uint16_t e[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) e[x] = n + x < ncols ? __bfloat16_as_ushort(src[x]) : 0;
+        memcpy(&w[0], e, 16);
+    }
+    float res[4][4];
+    unpack_rows(w, res);
+    uint32_t bf[4][KS][2];
+    int have = -1, of_row[2];
+    const int64_t at = (int64_t)min(row0 + g, last) * (p.n_shards * p.ranks) + shard * p.ranks;
+    outer_tile<KS>(p, mine, have, bf, col0, ncols, lane, [&](int) { return p.big + at; }, [&](int) { return p.small + at; }, res, of_row);
+    if (row0 + g > last || (of_row[0] == -1 && p.out == p.base)) return;         // in place, rows without an adapter stay as they are
+    const uint4 y = pack_row(res, 0);
+    __nv_bfloat16 *dst = p.out + (row0 + g) * p.ld_out + col0 + n;
+    if (full) *(uint4 *)dst = y;
+    else {
+        uint16_t e[8];
+        memcpy(e, &y, 16);
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            if (n + x < ncols) dst[x] = __ushort_as_bfloat16(e[x]);
+    }
+}
+
+// Chunks: a block keeps its 256 columns and walks down the rows, 32 at a time, so an adapter's part of B is read once.  Base and inner values come through shared memory, a tile ahead, and the
+// sums leave from there in whole lines: what is in flight does not depend on registers, and a thread's addresses only step.
+template <int KS> struct ChunkShape {
+    static constexpr int COLS = 256, ROWS = 32, PITCH = COLS * 2 + 64, BLOCKS = KS <= 2 ? 4 : 2;        // rows g and g + 1 in different banks; blocks to an SM
+    static constexpr int RP = KS * 16 + 8, STAGE = ROWS * PITCH + 2 * ROWS * RP * 2, SMEM = 2 * STAGE;
+};
+template <int KS>
+__global__ void __launch_bounds__(LR_THREADS, ChunkShape<KS>::BLOCKS) low_rank_chunk_kernel(const __grid_constant__ LowRankParams p, int tiles) {
+    using Shape = ChunkShape<KS>;
+    constexpr int COLS = Shape::COLS, ROWS = Shape::ROWS, PITCH = Shape::PITCH, RP = Shape::RP, E = COLS / 8, STEP = LR_THREADS / E, R8 = KS * 2;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane % 4;
+    int64_t col0;
+    int ncols;
+    const int shard = shard_of(p, blockIdx.x, COLS, col0, ncols);
+    const int row0 = blockIdx.y * tiles * ROWS, row1 = min(row0 + tiles * ROWS, p.M), eighths = p.vec ? ncols / 8 : 0, rest = ncols - eighths * 8;
+    const int er = tid / E, ec = tid % E;                          // this thread's row and eighth of a tile's copies
+    pdl_wait();
+    pdl_trigger();
+    if (row0 >= row1) return;
+    auto ask = [&](int row, int stage) {
+        if (row < row1) {
+            uint8_t *to = smem + stage * Shape::STAGE;
+            const int rows = min(ROWS, row1 - row);
+            if (ec < eighths) {
+                const __nv_bfloat16 *src = p.base + (row + er) * p.ld_base + col0 + ec * 8;
+                const uint32_t dst = smem_u32(to) + er * PITCH + ec * 16;
+#pragma unroll
+                for (int i = 0; i < ROWS / STEP; ++i, src += STEP * p.ld_base)
+                    if (er + i * STEP < rows) cp_async16(dst + i * STEP * PITCH, src);
             }
-            const __nv_bfloat16 b = __float2bfloat16_rn(v);
-            big[r][k] = b;
-            small[r][k] = __float2bfloat16_rn(v - __bfloat162float(b));
+            for (int i = tid; i < rows * rest; i += LR_THREADS) {  // columns that do not fill 16 aligned bytes
+                const int r = i / rest, c = eighths * 8 + i % rest;
+                *(__nv_bfloat16 *)(to + r * PITCH + c * 2) = p.base[(row + r) * p.ld_base + col0 + c];
+            }
+            for (int i = tid; i < rows * R8 * 2; i += LR_THREADS) {        // the workspace's rows are `ranks` long
+                const int small = i >= rows * R8, x = i - small * rows * R8, r = x / R8, c = x % R8;
+                const __nv_bfloat16 *src = (small ? p.small : p.big) + (int64_t)(row + r) * (p.n_shards * p.ranks) + shard * p.ranks + c * 8;
+                cp_async16(smem_u32(to + ROWS * PITCH + (small * ROWS + r) * RP * 2 + c * 16), src);
+            }
         }
+        cp_async_commit();
+    };
+    uint32_t bf[4][KS][2];
+    int have = -1;
+    const int n0 = warp * 32;
+    ask(row0, 0);
+    for (int row = row0, stage = 0; row < row1; row += ROWS, stage ^= 1) {
+        ask(row + ROWS, stage ^ 1);
+        int mine[ROWS / 16];
+#pragma unroll
+        for (int i = 0; i < ROWS / 16; ++i) mine[i] = adapter_of(p, min(row + i * 16 + (lane & 15), row1 - 1));
+        cp_async_wait<1>();
         __syncthreads();
-        for (int n0 = warp * 32; n0 < ncols; n0 += LR_WARPS * 32) {
-            uint32_t bf[4][KS][2];
+        uint8_t *base = smem + stage * Shape::STAGE;
+        const __nv_bfloat16 *big = (const __nv_bfloat16 *)(base + ROWS * PITCH), *small = big + ROWS * RP;
+        if (n0 < ncols)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int n = n0 + 8 * (g / 2) + 2 * i + (g & 1);
-                const __nv_bfloat16 *src = p.b + ((int64_t)id * p.n_total + col0 + min(n, ncols - 1)) * p.rank;
-                if constexpr (KS == 1) {
-                    const bool in = t * 4 < p.rank;            // ranks that only fill the tile are zero here and in the inner values
-                    const uint2 v = *(const uint2 *)(src + (in ? t * 4 : 0));
-                    bf[i][0][0] = in ? v.x : 0u; bf[i][0][1] = in ? v.y : 0u;
-                } else {
-#pragma unroll
-                    for (int k = 0; k < KS; k += 2) {
-                        const bool in = k * 16 + t * 8 < p.rank;
-                        const uint4 v = *(const uint4 *)(src + (in ? k * 16 + t * 8 : 0));
-                        bf[i][k][0] = in ? v.x : 0u; bf[i][k][1] = in ? v.y : 0u; bf[i][k + 1][0] = in ? v.z : 0u; bf[i][k + 1][1] = in ? v.w : 0u;
-                    }
-                }
-            }
-            for (int m0 = 0; m0 < count; m0 += 16) {
-                const int n = n0 + t * 8;
-                const bool have[2] = {m0 + g < count && n < ncols, m0 + g + 8 < count && n < ncols}, whole = n + 8 <= ncols;
-                int64_t m[2];
-                uint4 old[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) m[j] = row0 + groups.list[at + min(m0 + g + 8 * j, count - 1)];
-                if (vec) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) old[j] = *(const uint4 *)(p.base + m[j] * p.ld_base + col0 + (whole ? n : 0));       // of an eighth that ends early: below
-                }
-                if (!vec || !whole)
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const __nv_bfloat16 *src = p.base + m[j] * p.ld_base + col0;
-                        uint16_t e[8];
-#pragma unroll
-                        for (int x = 0; x < 8; ++x) e[x] = __bfloat16_as_ushort(src[min(n + x, ncols - 1)]);
-                        memcpy(&old[j], e, 16);
-                    }
-                float acc[4][4] = {};
-#pragma unroll
-                for (int k = 0; k < KS; k += KS == 1 ? 1 : 2) {
-                    uint32_t hi[2][4], lo[2][4];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const int r = m0 + g + 8 * j;
-                        if constexpr (KS == 1) {
-                            const uint2 v = *(const uint2 *)&big[r][t * 4], w = *(const uint2 *)&small[r][t * 4];
-                            hi[0][j] = v.x; hi[0][j + 2] = v.y;
-                            lo[0][j] = w.x; lo[0][j + 2] = w.y;
-                        } else {
-                            const uint4 v = *(const uint4 *)&big[r][k * 16 + t * 8], w = *(const uint4 *)&small[r][k * 16 + t * 8];
-                            hi[0][j] = v.x; hi[0][j + 2] = v.y; hi[1][j] = v.z; hi[1][j + 2] = v.w;
-                            lo[0][j] = w.x; lo[0][j + 2] = w.y; lo[1][j] = w.z; lo[1][j + 2] = w.w;
-                        }
-                    }
-#pragma unroll
-                    for (int q = 0; q < (KS == 1 ? 1 : 2); ++q)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            mma_bf16(acc[i], hi[q], bf[i][k + q][0], bf[i][k + q][1]);
-                            mma_bf16(acc[i], lo[q], bf[i][k + q][0], bf[i][k + q][1]);
-                        }
-                }
+            for (int i = 0; i < ROWS / 16; ++i) {
+                if (row + i * 16 >= row1) continue;
+                uint4 *at[2], w[2];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    if (!have[j]) continue;
-                    const uint32_t w[4] = {old[j].x, old[j].y, old[j].z, old[j].w};
-                    uint32_t y[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = bf16_pair(__uint_as_float(w[i] << 16) + acc[i][2 * j], __uint_as_float(w[i] & 0xffff0000u) + acc[i][2 * j + 1]);
-                    __nv_bfloat16 *dst = p.out + m[j] * p.ld_out + col0 + n;
-                    if (vec && whole) *(uint4 *)dst = make_uint4(y[0], y[1], y[2], y[3]);
-                    else {
-#pragma unroll
-                        for (int x = 0; x < 8; ++x)
-                            if (n + x < ncols) dst[x] = __ushort_as_bfloat16((uint16_t)(y[x / 2] >> (16 * (x & 1))));
-                    }
+                    at[j] = (uint4 *)(base + (i * 16 + g + 8 * j) * PITCH + (n0 + t * 8) * 2);
+                    w[j] = *at[j];
                 }
+                float res[4][4];
+                int of_row[2];
+                unpack_rows(w, res);
+                auto of = [&](const __nv_bfloat16 *v) { return [=](int j) { return v + (i * 16 + g + 8 * j) * RP; }; };
+                outer_tile<KS>(p, mine[i], have, bf, col0 + n0, min(ncols - n0, 32), lane, of(big), of(small), res, of_row);
+                *at[0] = pack_row(res, 0);
+                *at[1] = pack_row(res, 1);
             }
-        }
         __syncthreads();
+        const int rows = min(ROWS, row1 - row);
+        const bool keep = p.out == p.base;                         // in place, rows without an adapter stay as they are
+        if (ec < eighths) {
+            __nv_bfloat16 *dst = p.out + (row + er) * p.ld_out + col0 + ec * 8;
+            const uint8_t *src = base + er * PITCH + ec * 16;
+#pragma unroll
+            for (int i = 0; i < ROWS / STEP; ++i, dst += STEP * p.ld_out)
+                if (er + i * STEP < rows && !(keep && adapter_of(p, row + er + i * STEP) == -1)) *(uint4 *)dst = *(const uint4 *)(src + i * STEP * PITCH);
+        }
+        for (int i = tid; i < rows * rest; i += LR_THREADS) {
+            const int r = i / rest, c = eighths * 8 + i % rest;
+            if (!(keep && adapter_of(p, row + r) == -1)) p.out[(row + r) * p.ld_out + col0 + c] = *(const __nv_bfloat16 *)(base + r * PITCH + c * 2);
+        }
+        __syncthreads();                                           // the next request writes here
     }
 }
 

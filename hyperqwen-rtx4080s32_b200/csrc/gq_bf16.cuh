@@ -1,4 +1,4 @@
-// bf16 products of the operators beside the quantized layers.
+// bf16 products and asynchronous copies of the operators beside the quantized layers.
 #pragma once
 #include "gq_common.cuh"
 
@@ -16,5 +16,14 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
     memcpy(&u, &v, 4);
     return u;
 }
+
+// 16 bytes from global to shared memory, asynchronously
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+// the same, or 16 zeros
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 }  // namespace gq

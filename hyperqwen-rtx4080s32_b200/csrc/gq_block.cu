@@ -35,10 +35,24 @@ template <class... P, class... A> static cudaError_t launch_pdl(void (*kernel)(P
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// blocks of a kernel that the current device holds at once; its shared memory is allowed on the way (asked once per device)
+template <auto KERNEL> static int resident_blocks(int threads, int smem, int *blocks) {
+    static std::atomic<int> known[64];
+    int dev = 0, sms = 0, per_sm = 0;
+    GQ_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && (*blocks = known[dev].load(std::memory_order_acquire))) return GQ_OK;
+    GQ_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    GQ_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    GQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, KERNEL, threads, smem));
+    *blocks = sms * (per_sm < 1 ? 1 : per_sm);
+    if (dev < 64) known[dev].store(*blocks, std::memory_order_release);
+    return GQ_OK;
+}
+
 // ---- low-rank adapters -------------------------------------------------------------------------------
 
 static int check_low_rank(const gq_low_rank_args *p, int64_t *n_total) {
-    if (!p || p->M < 0 || p->M > (1 << 22) || p->K <= 0 || p->K % GQ_QK || p->K > (1 << 24) || p->rank <= 0 || p->rank % 8 || p->n_adapters <= 0) return p ? GQ_ERR_SHAPE : GQ_ERR_ARG;
+    if (!p || p->M < 0 || p->M > 65535 * (int64_t)LR_ROWS || p->K <= 0 || p->K % GQ_QK || p->K > (1 << 24) || p->rank <= 0 || p->rank % 8 || p->n_adapters <= 0) return p ? GQ_ERR_SHAPE : GQ_ERR_ARG;
     if (p->rank > GQ_MAX_RANK || p->n_shards < 1 || p->n_shards > GQ_MAX_DEVICE_SHARDS) return GQ_ERR_LIMIT;
     *n_total = 0;
     for (int s = 0; s < p->n_shards; ++s) {
@@ -49,7 +63,7 @@ static int check_low_rank(const gq_low_rank_args *p, int64_t *n_total) {
 }
 static int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 static int ranks_of(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
-// adapters that a tile of rows may hold, and the parts that K is cut into: enough blocks for the GPU, a part of 8 steps of 32 at least
+// adapters that a tile of rows may hold, and the parts that K is cut into: blocks for the whole GPU, 256 of K to a part at least, a cluster of sixteen at most
 static int low_rank_groups(const gq_low_rank_args *p) { return (int)std::min<int64_t>(std::min<int64_t>(p->M, LR_ROWS), p->n_adapters); }
 static int low_rank_parts(const gq_low_rank_args *p) {
     const int64_t tiles = (p->M + LR_ROWS - 1) / LR_ROWS, blocks = tiles * (tiles == 1 ? low_rank_groups(p) : 1);
@@ -58,7 +72,43 @@ static int low_rank_parts(const gq_low_rank_args *p) {
 extern "C" int64_t gq_low_rank_workspace_bytes(const gq_low_rank_args *p) {
     int64_t n = 0;
     if (const int rc = check_low_rank(p, &n)) return rc;
-    return n == 0 ? 0 : p->M * p->n_shards * ranks_of(p->rank) * low_rank_parts(p) * 4;
+    return n == 0 ? 0 : 2 * up256(p->M * p->n_shards * ranks_of(p->rank) * 2);
+}
+template <int MT> static cudaError_t low_rank_inner(const LowRankParams &q, dim3 grid, void *stream) {
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = q.parts; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3(LR_THREADS); cfg.stream = (cudaStream_t)stream; cfg.attrs = attr; cfg.numAttrs = 2;
+    if (q.parts > 8) {            // more than the portable cluster: allowed once per device
+        static std::atomic<uint64_t> allowed{0};
+        int dev = 0;
+        if (const cudaError_t e = cudaGetDevice(&dev)) return e;
+        if (dev >= 64 || !(allowed.load() >> dev & 1)) {
+            if (const cudaError_t e = cudaFuncSetAttribute(low_rank_inner_kernel<MT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
+            if (dev < 64) allowed.fetch_or((uint64_t)1 << dev);
+        }
+    }
+    return cudaLaunchKernelEx(&cfg, low_rank_inner_kernel<MT>, q);
+}
+template <int KS> static int low_rank_outer(const LowRankParams &q, void *stream) {
+    using Shape = ChunkShape<KS>;
+    const bool few = q.M <= 128;
+    const int cols = few ? LR_OUTER_WARPS * 32 : Shape::COLS;
+    int64_t blocks = 0;
+    for (int s = 0; s < q.n_shards; ++s) blocks += (q.edges[s + 1] - q.edges[s] + cols - 1) / cols;
+    if (few) {
+        GQ_CUDA(launch_pdl(low_rank_few_kernel<KS>, dim3((unsigned)blocks, (q.M + LR_FEW - 1) / LR_FEW), LR_OUTER_WARPS * 32, 0, stream, q));
+    } else {                      // as many walks down the rows as the GPU holds blocks, at least one for every block of columns
+        int resident = 0;
+        if (const int rc = resident_blocks<low_rank_chunk_kernel<KS>>(LR_THREADS, Shape::SMEM, &resident)) return rc;
+        const int tiles = (q.M + Shape::ROWS - 1) / Shape::ROWS, walks = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, resident / blocks)), per = (tiles + walks - 1) / walks;
+        GQ_CUDA(launch_pdl(low_rank_chunk_kernel<KS>, dim3((unsigned)blocks, (tiles + per - 1) / per), LR_THREADS, Shape::SMEM, stream, q, per));
+    }
+    GQ_LAUNCHED();
+    return GQ_OK;
 }
 extern "C" int gq_low_rank_add(const gq_low_rank_args *p, void *stream) {
     int64_t n = 0;
@@ -66,42 +116,35 @@ extern "C" int gq_low_rank_add(const gq_low_rank_args *p, void *stream) {
     if (p->M == 0 || n == 0) return GQ_OK;
     if (!p->base || !p->x || !p->a || !p->b || !p->scales || !p->ids || !p->out || (p->ids_bytes != 4 && p->ids_bytes != 8)) return GQ_ERR_ARG;
     if (!aligned(p->x, 16) || !aligned(p->a, 16) || !aligned(p->b, 16) || p->ldx % 8 || p->ldx < p->K || p->ld_base < n || p->ld_out < n) return GQ_ERR_ARG;
-    if (p->workspace_bytes < gq_low_rank_workspace_bytes(p) || !p->workspace || !aligned(p->workspace, 256)) return GQ_ERR_WORKSPACE;
+    const int64_t bytes = gq_low_rank_workspace_bytes(p);
+    if (p->workspace_bytes < bytes || !p->workspace || !aligned(p->workspace, 256)) return GQ_ERR_WORKSPACE;
     int *status;
     if (const int rc = status_word(&status)) return rc;
-    const int ranks = ranks_of(p->rank), parts = low_rank_parts(p), groups = low_rank_groups(p);
     const int64_t tiles = (p->M + LR_ROWS - 1) / LR_ROWS;
     bool vec = aligned(p->base, 16) && aligned(p->out, 16) && p->ld_base % 8 == 0 && p->ld_out % 8 == 0;
     LowRankParams q{(const __nv_bfloat16 *)p->base, (const __nv_bfloat16 *)p->x, (const __nv_bfloat16 *)p->a, (const __nv_bfloat16 *)p->b, p->scales, p->ids,
-                    (__nv_bfloat16 *)p->out, (float *)p->workspace, status, p->ld_base, p->ldx, p->ld_out, n, {0},
-                    (int)p->M, (int)p->K, p->n_shards, p->n_adapters, p->rank, ranks, parts, p->ids_bytes == 8, 0, 0};
+                    (__nv_bfloat16 *)p->out, (__nv_bfloat16 *)p->workspace, (__nv_bfloat16 *)((uint8_t *)p->workspace + bytes / 2), status, p->ld_base, p->ldx, p->ld_out, n, {0},
+                    (int)p->M, (int)p->K, p->n_shards, p->n_adapters, p->rank, ranks_of(p->rank), low_rank_parts(p), p->ids_bytes == 8, 0};
     for (int s = 0; s < p->n_shards; ++s) {
         q.edges[s + 1] = q.edges[s] + p->n_outs[s];
         vec = vec && q.edges[s] % 8 == 0;
     }
     q.vec = vec;
-    q.cols = tiles * (n / 256) < 1024 ? 256 : 1024;
-    int64_t blocks = 0;
-    for (int s = 0; s < p->n_shards; ++s) blocks += (p->n_outs[s] + q.cols - 1) / q.cols;
-    if (tiles > 65535) return GQ_ERR_LIMIT;
-    const dim3 inner(parts, (unsigned)tiles, tiles == 1 ? groups : 1);
+    const dim3 inner(q.parts, (unsigned)tiles, tiles == 1 ? low_rank_groups(p) : 1);
     const int rank_tiles = p->n_shards * ((p->rank + 15) / 16);              // a warp's turn: as many as divide them, up to four
     switch (rank_tiles <= 4 ? rank_tiles : rank_tiles % 4 && rank_tiles % 3 == 0 ? 3 : 4) {
-        case 1: GQ_CUDA(launch_pdl(low_rank_inner_kernel<1>, inner, LR_THREADS, 0, stream, q)); break;
-        case 2: GQ_CUDA(launch_pdl(low_rank_inner_kernel<2>, inner, LR_THREADS, 0, stream, q)); break;
-        case 3: GQ_CUDA(launch_pdl(low_rank_inner_kernel<3>, inner, LR_THREADS, 0, stream, q)); break;
-        default: GQ_CUDA(launch_pdl(low_rank_inner_kernel<4>, inner, LR_THREADS, 0, stream, q));
+        case 1: GQ_CUDA(low_rank_inner<1>(q, inner, stream)); break;
+        case 2: GQ_CUDA(low_rank_inner<2>(q, inner, stream)); break;
+        case 3: GQ_CUDA(low_rank_inner<3>(q, inner, stream)); break;
+        default: GQ_CUDA(low_rank_inner<4>(q, inner, stream));
     }
     GQ_LAUNCHED();
-    const dim3 grid((unsigned)blocks, (unsigned)tiles, tiles == 1 ? (unsigned)std::max<int64_t>(1, std::min<int64_t>(groups, 888 / blocks)) : 1);
-    switch (ranks) {
-        case 16: GQ_CUDA(launch_pdl(low_rank_outer_kernel<1>, grid, LR_THREADS, 0, stream, q)); break;
-        case 32: GQ_CUDA(launch_pdl(low_rank_outer_kernel<2>, grid, LR_THREADS, 0, stream, q)); break;
-        case 64: GQ_CUDA(launch_pdl(low_rank_outer_kernel<4>, grid, LR_THREADS, 0, stream, q)); break;
-        default: GQ_CUDA(launch_pdl(low_rank_outer_kernel<8>, grid, LR_THREADS, 0, stream, q));
+    switch (q.ranks) {
+        case 16: return low_rank_outer<1>(q, stream);
+        case 32: return low_rank_outer<2>(q, stream);
+        case 64: return low_rank_outer<4>(q, stream);
+        default: return low_rank_outer<8>(q, stream);
     }
-    GQ_LAUNCHED();
-    return GQ_OK;
 }
 
 // ---- norms and rotation of heads ---------------------------------------------------------------------
@@ -148,20 +191,6 @@ static int check_attention(const gq_attention_args *p) {
     if (p->n_heads > 65535 || p->T > (1 << 24) || p->T * (p->n_heads / p->n_kv_heads) >= (1 << 30) || p->table_width > (1 << 30) || p->table_width * p->page_size > (1 << 30)) return GQ_ERR_LIMIT;
     return GQ_OK;
 }
-// blocks of a kernel that the current device holds at once; its shared memory is allowed on the way (asked once per device)
-template <auto KERNEL> static int resident_blocks(int threads, int smem, int *blocks) {
-    static std::atomic<int> known[64];
-    int dev = 0, sms = 0, per_sm = 0;
-    GQ_CUDA(cudaGetDevice(&dev));
-    if (dev < 64 && (*blocks = known[dev].load(std::memory_order_acquire))) return GQ_OK;
-    GQ_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    GQ_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    GQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, KERNEL, threads, smem));
-    *blocks = sms * (per_sm < 1 ? 1 : per_sm);
-    if (dev < 64) known[dev].store(*blocks, std::memory_order_release);
-    return GQ_OK;
-}
-
 // rows of a tile: those of a sequence's tokens under one kv head, as far as the batch's average tells
 static int row_groups(const gq_attention_args *p) {
     const int64_t tokens = p->n_seqs ? (p->T + p->n_seqs - 1) / p->n_seqs : 1, rows = tokens * (p->n_heads / p->n_kv_heads);
