@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(LR_OUTER_WARPS * 32) low_rank_few_kernel(const
 // Chunks: a block keeps its 256 columns and walks down the rows, 32 at a time, so an adapter's part of B is read once.  Base and inner values come through shared memory, a tile ahead, and the
 // sums leave from there in whole lines: what is in flight does not depend on registers, and a thread's addresses only step.
 template <int KS> struct ChunkShape {
-    static constexpr int COLS = 256, ROWS = 32, PITCH = COLS * 2 + 64, BLOCKS = KS <= 2 ? 4 : 2;        // rows g and g + 1 in different banks; blocks to an SM
+    static constexpr int COLS = 256, ROWS = 32, PITCH = COLS * 2 + 64, BLOCKS = KS == 1 ? 4 : KS == 2 ? 3 : 2;        // rows g and g + 1 in different banks; blocks to an SM
     static constexpr int RP = KS * 16 + 8, STAGE = ROWS * PITCH + 2 * ROWS * RP * 2, SMEM = 2 * STAGE;
 };
 template <int KS>
