@@ -300,6 +300,79 @@ class GGUFLinearMethod:
         return out.reshape(*lead, out.shape[-1])
 
 
+    def add_adapters(self, layer: torch.nn.Module, n_adapters: int, rank: int) -> LowRankAdapters:
+        """Puts a bank of low-rank adapters beside a loaded layer (layer.gguf_adapters) for apply_with_adapters; the quantized weights stay
+        as they are.  An addition to the reference's method."""
+        layer.gguf_adapters = LowRankAdapters(layer, n_adapters, rank)
+        return layer.gguf_adapters
+
+    def apply_with_adapters(self, layer: torch.nn.Module, x: torch.Tensor, ids: torch.Tensor, pre=None, bias: torch.Tensor | None = None) -> torch.Tensor:
+        """apply_with_pre plus, for every row, the low-rank adapter ids names (int32 or int64, one per row; -1: none).  Layer and adapters multiply the same
+        activation, so a `pre` runs in front of both here.  Not inside ops.fused_allreduce: the sum over the ranks would miss the adapters."""
+        bank = getattr(layer, "gguf_adapters", None)
+        if bank is None:
+            raise RuntimeError("the layer has no bank of adapters: add_adapters was not called")
+        if ops.in_fused_allreduce():
+            raise ops.GqError("adapters are added before the sum over the ranks: call the layer outside fused_allreduce and all-reduce its output")
+        if pre is not None:
+            x = pre.unfused(x)
+        return bank.add_(self.apply(layer, x, bias), x, ids)
+
+
+# ---- low-rank adapters beside a layer ------------------------------------------------------------------
+
+class LowRankAdapters:
+    """A bank of low-rank adapters beside one layer, `n_adapters` of up to `rank` (rounded up to a multiple of 8, the rest zeros): the operands of
+    ops.low_rank_add.  A slot holds one adapter of every shard of the layer; an empty one adds nothing."""
+
+    def __init__(self, layer: torch.nn.Module, n_adapters: int, rank: int):
+        groups, tiles = getattr(layer, "gguf_groups", None), getattr(layer, "gguf_tiles", None)
+        if not groups or not tiles:
+            raise RuntimeError("GGUF layer has no packed tiles: process_weights_after_loading was not run")
+        self.order = ["__all__"] if "__all__" in tiles else _gguf_ordered_shard_ids(list(layer.weight.shard_id))
+        whole = getattr(layer.weight, "shard_offset_map", None) if self.order == ["__all__"] else None
+        if whole:            # shards of one type, held as one tensor: adapters still come shard by shard
+            self.order = sorted(whole, key=lambda sid: whole[sid][0])
+            self.n_outs = [whole[sid][1] - whole[sid][0] for sid in self.order]
+        else:
+            self.n_outs = [int(layer.gguf_tiles_rows[sid]) for sid in self.order]
+        self.rank = -(-int(rank) // 8) * 8
+        if n_adapters < 1 or rank < 1 or self.rank > ops.MAX_RANK:
+            raise ops.GqError(f"a bank holds one adapter or more of rank 1 to {ops.MAX_RANK}")
+        packed, _, _, _, nb, _ = next(iter(groups.values()))
+        self.k, dev, n = nb * F.QK, packed.device, sum(self.n_outs)
+        self.a = torch.zeros((n_adapters, len(self.order) * self.rank, self.k), dtype=torch.bfloat16, device=dev)
+        self.b = torch.zeros((n_adapters, n, self.rank), dtype=torch.bfloat16, device=dev)
+        self.scales = torch.zeros((n_adapters, len(self.order)), dtype=torch.float32, device=dev)
+
+    def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0, shard_id=None) -> None:
+        """The adapter of one shard (the only one, if shard_id is None): a [r, K], b [n_out, r] of any float type, its products times `scale`."""
+        if shard_id is None and len(self.order) == 1:
+            shard_id = self.order[0]
+        if shard_id not in self.order or not 0 <= slot < self.a.shape[0]:
+            raise ops.GqError(f"no shard {shard_id!r} among {self.order}, or no slot {slot} among {self.a.shape[0]}")
+        j = self.order.index(shard_id)
+        r, first = a.shape[0], sum(self.n_outs[:j])
+        if a.dim() != 2 or b.dim() != 2 or a.shape[1] != self.k or b.shape[1] != r or b.shape[0] != self.n_outs[j] or not 1 <= r <= self.rank:
+            raise ops.GqError(f"an adapter of this shard is [r, {self.k}] and [{self.n_outs[j]}, r] with r up to {self.rank}, got {tuple(a.shape)} and {tuple(b.shape)}")
+        mine, rows = self.a[slot, j * self.rank:(j + 1) * self.rank], self.b[slot, first:first + self.n_outs[j]]
+        mine[:r], mine[r:] = a.to(self.a), 0
+        rows[:, :r], rows[:, r:] = b.to(self.b), 0
+        self.scales[slot, j] = float(scale)
+
+    def clear(self, slot: int) -> None:
+        """Empties a slot."""
+        self.scales[slot] = 0
+        self.a[slot] = 0
+        self.b[slot] = 0
+
+    def add_(self, y: torch.Tensor, x: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
+        """y [..., N] += the adapters `ids` (one for every row of x [..., K]; -1: none) of x, in place."""
+        y2 = y.view(-1, y.shape[-1])
+        ops.low_rank_add(y2, x.reshape(-1, x.shape[-1]), self.a, self.b, self.scales, ids.reshape(-1), self.n_outs, out=y2)
+        return y
+
+
 # ---- standalone loading helpers (what vLLM's weight loaders do for a GGUF checkpoint) -----------------
 
 class GGUFLinear(torch.nn.Module):
@@ -321,5 +394,8 @@ class GGUFLinear(torch.nn.Module):
         self.quant_method.process_weights_after_loading(self)
         return self
 
-    def forward(self, x: torch.Tensor, pre=None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, pre=None, adapters: torch.Tensor | None = None) -> torch.Tensor:
+        """pre: the op in front of the layer (apply_with_pre); adapters: the rows' adapters in the layer's bank (apply_with_adapters)."""
+        if adapters is not None:
+            return self.quant_method.apply_with_adapters(self, x, adapters, pre, self.bias)
         return self.quant_method.apply_with_pre(self, x, pre, self.bias)

@@ -7,7 +7,7 @@ it serves), narrowed to this path: read the file's tensor table, give every tens
 hand the quantized 2-D weights to GGUFLinearMethod's weight loaders — q / k / v and gate / up as the shards of the
 merged layers vLLM builds (shard ids "q", "k", "v" and 0, 1) —, which repack them tile-major on the device.  Norms,
 convolution and state-space tensors, the vision tower and the projector are not linear-method weights: they are
-reported with their names and left to the engine.
+reported with their names and left to the engine (the head norms of an attention block go into LoadedModel.attention).
 
 The file is read with the `gguf` package (the reference pins gguf==0.17.1, gguf-plugin/requirements.txt:1); tensor data
 stay memory-mapped until they are copied to the device, one tensor at a time.
@@ -94,7 +94,11 @@ def read_gguf(path: str) -> Iterator[GGUFTensor]:
     """The file's tensors in file order (data memory-mapped by the gguf package)."""
     from gguf import GGUFReader
 
-    for t in GGUFReader(path).tensors:
+    yield from _tensors(GGUFReader(path))
+
+
+def _tensors(reader) -> Iterator[GGUFTensor]:
+    for t in reader.tensors:
         shape = tuple(int(d) for d in reversed(t.shape))          # GGUF lists the innermost dimension first
         yield GGUFTensor(str(t.name), int(t.tensor_type), shape, t.data)
 
@@ -106,6 +110,34 @@ class LoadedModel:
     other: dict[str, GGUFTensor] = field(default_factory=dict)     # HF name -> norms etc., for the engine
     unmapped: list[str] = field(default_factory=list)              # names this adapter does not know
     unsupported: dict[str, str] = field(default_factory=dict)      # linear weights in a GGML type the kernels do not decode
+    meta: dict[str, object] = field(default_factory=dict)          # the file's numbers and texts, keys without the architecture: "rope.freq_base"
+
+    def add_adapters(self, n_adapters: int, rank: int) -> None:
+        """A bank of low-rank adapters beside every linear layer of the decoder blocks (load_adapter fills them)."""
+        for name, lin in self.linears.items():
+            if name.startswith("layers."):
+                lin.quant_method.add_adapters(lin, n_adapters, rank)
+
+    def attention(self, layer: int, *, head_dim: int | None = None, **rotary):
+        """The attention half of a block (attention.GGUFAttention) from its qkv_proj, o_proj and head norms.  What the file says about heads, rotation and eps is
+        taken from it; `head_dim` and the arguments of ops.rotary_frequencies (rotary_dim, base, scaling, factor, original_context) go before."""
+        from . import ops
+        from .attention import GGUFAttention
+
+        def norm(which):
+            t = self.other.get(f"model.language_model.layers.{layer}.self_attn.{which}_norm.weight")
+            return None if t is None else torch.from_numpy(np.array(t.data, copy=True)).to(device=device, dtype=torch.bfloat16)
+
+        qkv, o, meta = self.linears[f"layers.{layer}.self_attn.qkv_proj"], self.linears[f"layers.{layer}.self_attn.o_proj"], self.meta
+        device = next(iter(qkv.gguf_groups.values()))[0].device
+        q_norm, k_norm = norm("q"), norm("k")
+        head_dim = head_dim or (q_norm.numel() if q_norm is not None else None) or meta.get("attention.key_length")
+        if not head_dim:
+            raise ValueError("neither the file nor the call says how wide a head is")
+        known = {"rotary_dim": meta.get("rope.dimension_count", head_dim), "base": meta.get("rope.freq_base", 10000.0), "scaling": meta.get("rope.scaling.type"),
+                 "factor": meta.get("rope.scaling.factor", 1.0), "original_context": meta.get("rope.scaling.original_context_length")}
+        inv_freq, amplitude = ops.rotary_frequencies(**{**known, **rotary}, device=device)
+        return GGUFAttention(qkv, o, int(head_dim), inv_freq, amplitude=amplitude, q_norm=q_norm, k_norm=k_norm, eps=float(meta.get("attention.layer_norm_rms_epsilon", 1e-6)))
 
 
 def load_gguf(path: str, device="cuda", strict: bool = True) -> LoadedModel:
@@ -113,10 +145,13 @@ def load_gguf(path: str, device="cuda", strict: bool = True) -> LoadedModel:
     and gate / up fused as vLLM fuses them; every weight goes through GGUFLinearMethod's weight loaders and is repacked
     tile-major on `device`.  With strict, a linear weight in a type the kernels do not decode raises; otherwise it is listed
     in `unsupported` and its module is left out."""
-    out = LoadedModel()
+    from gguf import GGUFReader
+
+    reader = GGUFReader(path)
+    out = LoadedModel(meta=_metadata(reader))
     pending: dict[str, list[tuple[object, GGUFTensor]]] = {}
     order = {"q": 0, "k": 1, "v": 2, 0: 0, 1: 1, None: 0}
-    for t in read_gguf(path):
+    for t in _tensors(reader):
         mapped = map_tensor_name(t.name)
         if mapped is None:
             out.unmapped.append(t.name)
@@ -149,6 +184,57 @@ def load_gguf(path: str, device="cuda", strict: bool = True) -> LoadedModel:
             lin.load_shard(raw.to(device), t.ggml_type, sid)
         out.linears[key] = lin.finalize()
     return out
+
+
+def _metadata(reader) -> dict[str, object]:
+    """The file's single numbers and texts; "qwen35.rope.freq_base" is listed as "rope.freq_base" too."""
+    out: dict[str, object] = {}
+    for name, f in reader.fields.items():
+        if len(f.types) == 1 and len(f.data) == 1:
+            v = f.contents()
+            if isinstance(v, (int, float, str, bool)):
+                out[name] = v
+    arch = str(out.get("general.architecture", ""))
+    return {**out, **{k[len(arch) + 1:]: v for k, v in out.items() if arch and k.startswith(arch + ".")}}
+
+
+def load_adapter(path: str, model: LoadedModel, slot: int, scale: float = 1.0) -> list[str]:
+    """Reads a GGUF adapter file (general.type "adapter", adapter.type "lora": a pair X.lora_a [r, K], X.lora_b [n_out, r] for every adapted weight X, and
+    adapter.lora.alpha) into `slot` of the banks that model.add_adapters made, which is emptied first; its products count alpha / r * scale.
+    Returns the layers that have it.  A weight that is no linear layer of the model raises ValueError, before anything is changed."""
+    from gguf import GGUFReader
+
+    reader = GGUFReader(path)
+    meta = _metadata(reader)
+    if meta.get("adapter.type") != "lora":
+        raise ValueError(f"{path} is not a low-rank adapter")
+    parts: dict[str, dict[str, torch.Tensor]] = {}
+    for t in _tensors(reader):
+        name, _, which = t.name.rpartition(".lora_")
+        if which not in ("a", "b") or t.ggml_type not in (0, 1, 30):
+            raise ValueError(f"{t.name}: not one of a pair of matrices in F32, F16 or BF16")
+        data = np.array(t.data, copy=True)
+        value = torch.from_numpy(data) if t.ggml_type != 30 else torch.from_numpy(data).view(torch.bfloat16)
+        parts.setdefault(name, {})[which] = value.reshape(t.shape)
+    found = []
+    for name, pair in parts.items():
+        mapped = map_tensor_name(name)
+        key = None if mapped is None or mapped.layer is None or mapped.module is None else f"layers.{mapped.layer}.{mapped.merged or mapped.module}"
+        lin = model.linears.get(key) if key else None
+        if lin is None or len(pair) != 2:
+            raise ValueError(f"{name}: no layer of the model, or half of an adapter")
+        bank = getattr(lin, "gguf_adapters", None)
+        if bank is None or pair["a"].shape[0] > bank.rank:
+            raise ValueError(f"{name}: model.add_adapters(rank >= {pair['a'].shape[0]}) comes first")
+        found.append((key, bank, pair, mapped.shard_id))
+    for lin in model.linears.values():
+        if getattr(lin, "gguf_adapters", None) is not None:
+            lin.gguf_adapters.clear(slot)
+    alpha = float(meta.get("adapter.lora.alpha", 0.0))
+    for _, bank, pair, shard_id in found:
+        r = pair["a"].shape[0]
+        bank.load(slot, pair["a"], pair["b"], scale * (alpha / r if alpha else 1.0), shard_id)
+    return sorted({key for key, *_ in found})
 
 
 def embedding_lookup(raw: torch.Tensor, wtype: int, ids: torch.Tensor, dtype=torch.bfloat16) -> torch.Tensor:

@@ -340,6 +340,10 @@ def fused_allreduce(ctx):
         _FUSED_AR = prev
 
 
+def in_fused_allreduce() -> bool:
+    return _FUSED_AR is not None
+
+
 class PreSiluMul:
     """The layer's input is silu(t[:, :K]) * t[:, K:] of the [M, 2K] tensor handed in (vLLM's silu_and_mul in front of
     down_proj), computed inside the activation preparation."""
@@ -578,7 +582,11 @@ def low_rank_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     [adapters, shards], ids int32 or int64 [M], n_outs the shards' columns (N in all).  The rank is a multiple of 8 up to 128 (pad with zeros), K of 256.
     ids[m] = -1: the row has no adapter and is base's.  Any other id outside the bank makes its row NaN and device_status 2.  `out` may be base
     (in place); it is new memory if left out.  Sums in 32 bits, one rounding; a row's sums hold nothing of other rows' adapters."""
-    return native().low_rank_add(base, x, a, b, scales, ids, [int(n) for n in n_outs], out)
+    n_outs = [int(n) for n in n_outs]
+    if torch.compiler.is_compiling():
+        sums = torch.ops.gq_b200.low_rank_add(base, x, a, b, scales, ids, n_outs)
+        return sums if out is None else out.copy_(sums)
+    return native().low_rank_add(base, x, a, b, scales, ids, n_outs, out)
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0, original_context: int | None = None,
@@ -614,6 +622,8 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Ten
     The first 2 * len(inv_freq) dimensions of a head turn, as pairs half of them apart or, `interleaved`, side by side; inv_freq (float64) and amplitude as
     rotary_frequencies makes them; angles are reduced in 64 bits.  positions int32 or int64 [T].  `gated`: every query head is followed
     by an output gate of head_dim values, which stays where it is (paged_attention takes it)."""
+    if torch.compiler.is_compiling():
+        return torch.ops.gq_b200.qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated)
     return native().qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated, None, None, None)
 
 
@@ -625,6 +635,9 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
 
     k_pages, v_pages bf16 [pages, rows, n_kv_heads, head_dim] by strides; token t goes to slot slots[t] (int32 or int64) = page * rows + row.  A negative
     slot stores nothing (padding); one beyond the cache stores nothing and makes device_status 2.  Of two tokens with one slot either may be kept."""
+    if torch.compiler.is_compiling():
+        return torch.ops.gq_b200.qk_norm_rope_store(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated,
+                                                    k_pages, v_pages, slots)
     return native().qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated,
                                  k_pages, v_pages, slots)
 
@@ -641,6 +654,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     scale: head_dim ** -0.5 if left out.  gate (q's shape, any strides over tokens and heads): the result is multiplied by sigmoid(gate).
     A page outside the cache or a length beyond the table: NaN in the rows that see it, and device_status 2.  Probabilities, sums and the join of the
     cache's parts in 32 bits, one rounding; the order of the sums does not depend on timing."""
+    if torch.compiler.is_compiling():
+        o = torch.ops.gq_b200.paged_attention(q, k_pages, v_pages, page_table, lens, q_starts, scale, gate, out)
+        return o if out is None else out.copy_(o)
     return native().paged_attention(q, k_pages, v_pages, page_table, lens, q_starts, scale, gate, out)
 
 
@@ -656,3 +672,20 @@ _OP_LIB.define("fused_mul_mat_gguf_tiles_grouped(Tensor x, Tensor packed, Tensor
 _OP_LIB.impl("fused_mul_mat_gguf_tiles_grouped", mul_mat_tiles_grouped, "CUDA")
 torch.library.register_fake("gq_b200::fused_mul_mat_gguf_tiles_grouped")(_fake)
 fused_mul_mat_gguf_tiles_grouped = torch.ops.gq_b200.fused_mul_mat_gguf_tiles_grouped
+
+
+# The operators beside the layers, as a traced program calls them.  The last argument of paged_attention is what rows behind the last sequence keep.
+_OP_LIB.define("low_rank_add(Tensor base, Tensor x, Tensor a, Tensor b, Tensor scales, Tensor ids, int[] n_outs) -> Tensor")
+_OP_LIB.define("qk_norm_rope(Tensor qkv, Tensor positions, Tensor inv_freq, int n_heads, int n_kv_heads, int head_dim, Tensor? q_norm, Tensor? k_norm, "
+               "float eps, float amplitude, bool interleaved, bool gated) -> (Tensor, Tensor)")
+_OP_LIB.define("qk_norm_rope_store(Tensor qkv, Tensor positions, Tensor inv_freq, int n_heads, int n_kv_heads, int head_dim, Tensor? q_norm, Tensor? k_norm, "
+               "float eps, float amplitude, bool interleaved, bool gated, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor slots) -> Tensor")
+_OP_LIB.define("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor lens, Tensor? q_starts, float? scale, Tensor? gate, Tensor? kept) -> Tensor")
+_OP_LIB.impl("low_rank_add", lambda *args: native().low_rank_add(*args, None), "CUDA")
+_OP_LIB.impl("qk_norm_rope", lambda *args: native().qk_norm_rope(*args, None, None, None), "CUDA")
+_OP_LIB.impl("qk_norm_rope_store", lambda *args: native().qk_norm_rope(*args), "CUDA")
+_OP_LIB.impl("paged_attention", lambda *args: native().paged_attention(*args[:-1], None if args[-1] is None else args[-1].clone(memory_format=torch.contiguous_format)), "CUDA")
+torch.library.register_fake("gq_b200::low_rank_add")(lambda base, *_: base.new_empty(base.shape))
+torch.library.register_fake("gq_b200::qk_norm_rope")(lambda qkv, positions, inv_freq, hq, hk, d, *_: (qkv.new_empty((qkv.shape[0], hq, d)), qkv.new_empty((qkv.shape[0], hk, d))))
+torch.library.register_fake("gq_b200::qk_norm_rope_store")(lambda qkv, positions, inv_freq, hq, hk, d, *_: qkv.new_empty((qkv.shape[0], hq, d)))
+torch.library.register_fake("gq_b200::paged_attention")(lambda q, *_: q.new_empty(q.shape))

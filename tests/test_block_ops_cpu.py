@@ -101,3 +101,50 @@ def test_frequencies():
     for bad in (dict(rotary_dim=7), dict(rotary_dim=8, base=0), dict(rotary_dim=8, factor=-1), dict(rotary_dim=8, scaling="other"), dict(rotary_dim=8, scaling="yarn", factor=2)):
         with pytest.raises(E):
             ops.rotary_frequencies(device="cpu", **bad)
+
+
+def test_slots_of_a_cache():
+    from hyperqwen_rtx4080s32_b200.attention import PagedKVCache
+
+    cache = PagedKVCache(7, 4, 2, 8, device="cpu")
+    assert cache.k.shape == cache.v.shape == (7, 4, 2, 8) and cache.k.stride() == (64, 8, 32, 1)
+    table = torch.tensor([[5, 1], [6, 0]], dtype=torch.int32)
+    got = cache.slots(table, torch.tensor([0, 0, 1, 1, 0]), torch.tensor([0, 6, 3, 4, -1]))
+    assert got.tolist() == [20, 6, 27, 0, -1]
+    for bad in ((0, 4), (4, 0)):
+        with pytest.raises(E):
+            PagedKVCache(*bad, 2, 8, device="cpu")
+
+
+def test_heads_that_do_not_fit_the_projections():
+    from hyperqwen_rtx4080s32_b200.attention import GGUFAttention
+    from hyperqwen_rtx4080s32_b200.linear import GGUFLinear, LowRankAdapters
+
+    inv = torch.zeros(4, dtype=torch.float64)
+    o = GGUFLinear(512, [768])
+    att = GGUFAttention(GGUFLinear(768, [1024, 128, 128]), o, 64, inv)
+    assert att.gated and (att.n_heads, att.n_kv_heads) == (8, 2)
+    assert not GGUFAttention(GGUFLinear(768, [512, 128, 128]), o, 64, inv).gated
+    for rows in ([512, 128], [512, 128, 64], [768, 128, 128], [512, 96, 96]):
+        with pytest.raises(E):
+            GGUFAttention(GGUFLinear(768, rows), o, 64, inv)
+    with pytest.raises(RuntimeError, match="no packed tiles"):
+        LowRankAdapters(o, 2, 8)
+
+
+def test_the_operators_trace_with_fake_tensors():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    def fn(base, x, a, b, scales, ids, pos, inv, k_pages, v_pages, slots, table, lens):
+        y = ops.low_rank_add(base, x, a, b, scales, ids, [64, 16, 16])
+        q, _ = ops.qk_norm_rope(y, pos, inv, 4, 1, 16)
+        q = ops.qk_norm_rope_store(y, pos, inv, 4, 1, 16, k_pages, v_pages, slots) + q
+        return ops.paged_attention(q.repeat(1, 1, 4), k_pages.repeat(1, 1, 1, 4), v_pages.repeat(1, 1, 1, 4), table, lens)
+
+    with FakeTensorMode():
+        e = lambda *s, t=torch.bfloat16: torch.empty(s, dtype=t, device="meta")  # noqa: E731
+        i64, i32 = torch.int64, torch.int32
+        gm, _ = torch._dynamo.export(fn)(e(6, 96), e(6, 256), e(2, 24, 256), e(2, 96, 8), e(2, 3, t=torch.float32), e(6, t=i64), e(6, t=i64), e(8, t=torch.float64), e(3, 4, 1, 16),
+                                         e(3, 4, 1, 16), e(6, t=i64), e(2, 2, t=i32), e(2, t=i32))
+    names = str([n.target for n in gm.graph.nodes if n.op == "call_function"])
+    assert all(n in names for n in ("low_rank_add", "qk_norm_rope", "qk_norm_rope_store", "paged_attention"))
