@@ -196,10 +196,10 @@ static int row_groups(const gq_attention_args *p) {
     const int64_t tokens = p->n_seqs ? (p->T + p->n_seqs - 1) / p->n_seqs : 1, rows = tokens * (p->n_heads / p->n_kv_heads);
     return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;
 }
-template <int D, int RG, int KG, int S> static int attention(const gq_attention_args *p, int64_t *bytes, int *status, void *stream) {
-    using Shape = PagedShape<D, RG, KG, S>;
+template <int D, int NQ, int KG, int DG, int S> static int attention(const gq_attention_args *p, int64_t *bytes, int *status, void *stream) {
+    using Shape = PagedShape<D, NQ, KG, DG, S>;
     int blocks = 0;
-    if (const int rc = resident_blocks<paged_attention_kernel<D, RG, KG, S>>(Shape::THREADS, Shape::SMEM, &blocks)) return rc;
+    if (const int rc = resident_blocks<paged_attention_kernel<D, NQ, KG, DG, S>>(Shape::THREADS, Shape::SMEM, &blocks)) return rc;
     const int64_t slots = 2 * (int64_t)blocks * Shape::ROWS, at_parts = up256(slots * 8);
     *bytes = at_parts + slots * D * 4;
     if (!status) return GQ_OK;
@@ -214,7 +214,7 @@ template <int D, int RG, int KG, int S> static int attention(const gq_attention_
         q.a.k_pages = q.a.v_pages = p->q;
         for (int i = 0; i < 3; ++i) q.a.k_strides[i] = q.a.v_strides[i] = 0;
     }
-    GQ_CUDA(launch_pdl(paged_attention_kernel<D, RG, KG, S>, dim3(blocks), Shape::THREADS, Shape::SMEM, stream, q));
+    GQ_CUDA(launch_pdl(paged_attention_kernel<D, NQ, KG, DG, S>, dim3(blocks), Shape::THREADS, Shape::SMEM, stream, q));
     GQ_LAUNCHED();
     GQ_CUDA(launch_pdl(join_parts_kernel<D, Shape::ROWS, Shape::UNIT>, dim3(blocks), JOIN_WARPS * 32, 0, stream, q));
     GQ_LAUNCHED();
@@ -222,18 +222,18 @@ template <int D, int RG, int KG, int S> static int attention(const gq_attention_
 }
 static int attention_by_shape(const gq_attention_args *p, int64_t *bytes, int *status, void *stream) {
     switch (p->head_dim * 8 + row_groups(p)) {
-        case 64 * 8 + 1: return attention<64, 1, 4, 3>(p, bytes, status, stream);
-        case 64 * 8 + 2: return attention<64, 2, 4, 3>(p, bytes, status, stream);
-        case 64 * 8 + 3: return attention<64, 3, 2, 3>(p, bytes, status, stream);
-        case 64 * 8 + 4: return attention<64, 4, 2, 3>(p, bytes, status, stream);
-        case 128 * 8 + 1: return attention<128, 1, 4, 3>(p, bytes, status, stream);
-        case 128 * 8 + 2: return attention<128, 2, 4, 3>(p, bytes, status, stream);
-        case 128 * 8 + 3: return attention<128, 3, 2, 3>(p, bytes, status, stream);
-        case 128 * 8 + 4: return attention<128, 4, 2, 3>(p, bytes, status, stream);
-        case 256 * 8 + 1: return attention<256, 1, 4, 3>(p, bytes, status, stream);
-        case 256 * 8 + 2: return attention<256, 2, 4, 3>(p, bytes, status, stream);
-        case 256 * 8 + 3: return attention<256, 3, 4, 2>(p, bytes, status, stream);
-        default: return attention<256, 4, 2, 3>(p, bytes, status, stream);
+        case 64 * 8 + 1: return attention<64, 1, 4, 1, 3>(p, bytes, status, stream);
+        case 64 * 8 + 2: return attention<64, 2, 4, 1, 3>(p, bytes, status, stream);
+        case 64 * 8 + 3: return attention<64, 3, 2, 1, 3>(p, bytes, status, stream);
+        case 64 * 8 + 4: return attention<64, 4, 2, 1, 3>(p, bytes, status, stream);
+        case 128 * 8 + 1: return attention<128, 1, 4, 1, 3>(p, bytes, status, stream);
+        case 128 * 8 + 2: return attention<128, 2, 4, 1, 3>(p, bytes, status, stream);
+        case 128 * 8 + 3: return attention<128, 3, 4, 1, 3>(p, bytes, status, stream);
+        case 128 * 8 + 4: return attention<128, 4, 2, 2, 3>(p, bytes, status, stream);
+        case 256 * 8 + 1: return attention<256, 1, 4, 2, 3>(p, bytes, status, stream);
+        case 256 * 8 + 2: return attention<256, 2, 4, 2, 3>(p, bytes, status, stream);
+        case 256 * 8 + 3: return attention<256, 3, 4, 2, 3>(p, bytes, status, stream);
+        default: return attention<256, 4, 4, 2, 3>(p, bytes, status, stream);
     }
 }
 

@@ -1,6 +1,6 @@
 // Attention of a sequence's newest tokens over its keys and values in the pages of a cache.
 //
-//   o = sum_j p_j v_j / sum_j p_j,  p_j = exp2(c q . k_j - m),  c = scale log2 e,  m the running maximum: one pass over keys and values.
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = exp2(c q . k_j - m),  c = scale log2 e,  m near the running maximum: one pass over keys and values.
 //
 // Bound by the bytes of the cache: a key-value head's key and value are 4 head_dim bytes, and the rows that share them (the query heads of the group, times the new tokens)
 // are few.  So the work is cut evenly by keys, not by sequences: the units of all (sequence, kv head, tile of rows) in a line, a unit being KG * 16 keys, and block c of G takes
@@ -177,27 +177,30 @@ template <int ROWS, int UNIT> __device__ __forceinline__ void locate(const Paged
     c.unit = (int)in;
 }
 
-template <int D, int RG, int KG, int S> struct PagedShape {
-    static constexpr int THREADS = 32 * RG * KG, ROWS = 8 * RG, UNIT = 16 * KG;
+template <int D, int NQ, int KG, int DG, int S> struct PagedShape {
+    static constexpr int THREADS = 32 * KG * DG, ROWS = 8 * NQ, UNIT = 16 * KG;
     static constexpr int PITCH = D * 2 + 16;                                    // bytes of a row in shared memory: eight rows' chunks in different banks
     static constexpr int STAGE = 2 * 16 * PITCH;                                // keys and values of 16 keys
-    static constexpr int TURNS = RG > 2 ? 2 : 1;                                // a key group's output goes through the stage it used last, in as many turns
-    static constexpr int RING = KG * S * STAGE, STATS = KG > 1 ? KG * ROWS * 8 : 0;
-    static_assert(ROWS * D * 4 / TURNS <= STAGE && (D / 16) % (KG * TURNS) == 0, "the key groups share the dimensions of an output out");
-    static constexpr int SMEM = RING + STATS + RG * KG * 256;
+    static constexpr int TURNS = NQ > 2 ? 2 : 1;                                // a key group's output goes through the stage it used last, in as many turns
+    static constexpr int RING = KG * S * STAGE, STATS = KG * ROWS * 8, TABLES = KG * DG * 256, HALVES = DG > 1 ? KG * DG * NQ * 512 : 0;
+    static constexpr int SMEM = RING + STATS + TABLES + HALVES;
+    static_assert(ROWS * D * 4 / TURNS <= STAGE && (D / 16 / DG) % (KG * TURNS) == 0, "the key groups share the dimensions of an output out");
+    static_assert(KG > 1 && 2 * KG <= 15, "named barriers: one for a key group's stages, one for its halves of scores");
 };
 
-template <int D, int RG, int KG, int S>
-__global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __grid_constant__ PagedParams p) {
-    using Shape = PagedShape<D, RG, KG, S>;
-    constexpr int ROWS = Shape::ROWS, UNIT = Shape::UNIT, STAGE = Shape::STAGE, PITCH = Shape::PITCH, CH = D / 8, MT = D / 16, WARPS = RG * KG;
+template <int D, int NQ, int KG, int DG, int S>
+__global__ void __launch_bounds__(32 * KG * DG) paged_attention_kernel(const __grid_constant__ PagedParams p) {
+    using Shape = PagedShape<D, NQ, KG, DG, S>;
+    constexpr int ROWS = Shape::ROWS, UNIT = Shape::UNIT, STAGE = Shape::STAGE, PITCH = Shape::PITCH, CH = D / 8, MT = D / 16 / DG, WARPS = KG * DG;
     extern __shared__ __align__(128) uint8_t smem[];
     float2 *stat_sm = (float2 *)(smem + Shape::RING);
     longlong2 *row_sm = (longlong2 *)((uint8_t *)stat_sm + Shape::STATS);       // [warp][16]: bytes to the keys and values of the stage being asked for
     const gq_attention_args &a = p.a;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, rg = warp % RG, kg = warp / RG, g = lane / 4, t = lane % 4;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, kg = warp / DG, dg = warp % DG, g = lane / 4, t = lane % 4;
     pdl_wait();
     pdl_trigger();
+
+    float4 *half_sm = (float4 *)(row_sm + 16 * WARPS) + kg * DG * NQ * 32;             // [DG][NQ][lane]: scores over a dimension group's part of head_dim
 
     // ---- this block's units (every warp counts for itself) ----
     Cursor use;
@@ -256,16 +259,15 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
                 const char *k = k_head + (page * a.k_strides[0] + pos * a.k_strides[1]) * 2, *v = v_head + (page * a.v_strides[0] + pos * a.v_strides[1]) * 2;
                 if (real == 16) {
 #pragma unroll
-                    for (int i = 0; i < (COPIES + RG - 1) / RG; ++i) {
-                        if (COPIES % RG && i * RG + rg >= COPIES) break;
-                        const uint32_t row = (RG > 1 ? i * RG + rg : i) * PER;
+                    for (int i = 0; i < COPIES / DG; ++i) {
+                        const uint32_t row = (DG > 1 ? i * DG + dg : i) * PER;
                         cp_async16(dst + row * PITCH, k + (uint64_t)row * k_step);
                         cp_async16(dst + (16 + row) * PITCH, v + (uint64_t)row * v_step);
                     }
                 } else {
                     bad = ok || seen <= 0 ? 0u : (1u << seen) - 1;
 #pragma unroll 1
-                    for (int i = rg; i < COPIES; i += RG) {
+                    for (int i = dg; i < COPIES; i += DG) {
                         const uint32_t row = i * PER;
                         const bool is = (int)row + copy_row < real;
                         cp_async16(dst + row * PITCH, is ? k + (uint64_t)row * k_step : (const char *)a.k_pages, is);
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
                 if (lane < 16) rows_at[lane] = ok ? make_longlong2(2 * (page * a.k_strides[0] + pos * a.k_strides[1]), 2 * (page * a.v_strides[0] + pos * a.v_strides[1])) : make_longlong2(0, 0);
                 __syncwarp();
 #pragma unroll 2
-                for (int i = rg; i < COPIES; i += RG) {
+                for (int i = dg; i < COPIES; i += DG) {
                     const int row = i * PER;
                     const longlong2 at = rows_at[row + copy_row];
                     const bool is = real >> (row + copy_row) & 1;
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
                     cp_async16(dst + (16 + row) * PITCH, v_head + at.y, is);
                 }
             }
-            if (bad && lane == 0) atomicMax(p.status, GQ_DEV_BAD_SHAPE);
+            if (bad && dg == 0 && lane == 0) atomicMax(p.status, GQ_DEV_BAD_SHAPE);
             ++got;
             if (++get.unit == get.units && got < count) { next_segment<ROWS, UNIT>(p, get); heads(); }
             look();
@@ -301,88 +303,118 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
     for (int i = 0; i < S - 1; ++i) ask(i);
     zeros();
 
-    // Transposed products: keys (or dimensions) on M, the eight query rows of the warp on N.  A lane holds, of a score tile, keys g and g + 8 of queries 2 t and 2 t + 1; of the
+    // Transposed products: keys (or dimensions) on M, eight query rows on N, NQ times.  A lane holds, of a score tile, keys g and g + 8 of queries 2 t and 2 t + 1; of the
     // output, dimensions 16 i + g and 16 i + g + 8 of the same two queries.
-    float o[MT][4], top[2], sum[2];
-    uint32_t qf[MT][2];
-    int lim[2], lim_first = 0;     // keys that this lane's queries see, and the tile's first row
+    float o[NQ][MT][4], top[NQ][2], sum[NQ][2];
+    uint32_t qf[NQ][MT][2];
+    int lim[NQ][2], lim_first = 0;     // keys that this lane's queries see, and the tile's first row
     int slot = 0;
     // where this lane's row of an ldmatrix starts: keys (rows 0-7, 8-15 of one chunk, then of the next), values (transposed: two chunks of rows 0-7, then of 8-15)
-    const uint32_t k_lane = (((lane >> 3) & 1) * 8 + (lane & 7)) * PITCH + (lane >> 4) * 16, v_lane = (16 + (lane >> 4) * 8 + (lane & 7)) * PITCH + ((lane >> 3) & 1) * 16;
+    const uint32_t k_lane = (((lane >> 3) & 1) * 8 + (lane & 7)) * PITCH + (lane >> 4) * 16 + dg * MT * 32, v_lane = (16 + (lane >> 4) * 8 + (lane & 7)) * PITCH + ((lane >> 3) & 1) * 16 + dg * MT * 32;
 
     for (int it = 0;;) {
         const int unit0 = use.unit;         // this block's first unit of the segment
-        {
+        const int rows = use.v.n * p.group, before = use.v.len - use.v.n + 1;
+        lim_first = before + (unsigned)(use.tile * ROWS) / (unsigned)p.group;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
-            const int rows = use.v.n * p.group, row0 = use.tile * ROWS + rg * 8;
-            const int before = use.v.len - use.v.n + 1;
+                for (int j = 0; j < 4; ++j) o[q][i][j] = 0.0f;
+            const int row0 = use.tile * ROWS + q * 8;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                top[j] = -INFINITY;
-                sum[j] = 0.0f;
-                lim[j] = before + (unsigned)min(row0 + 2 * t + j, rows - 1) / (unsigned)p.group;
+                top[q][j] = -INFINITY;
+                sum[q][j] = 0.0f;
+                lim[q][j] = before + (unsigned)min(row0 + 2 * t + j, rows - 1) / (unsigned)p.group;
             }
-            lim_first = before + (unsigned)(use.tile * ROWS) / (unsigned)p.group;
             const int r = row0 + g, i = (unsigned)r / (unsigned)p.group;
-            const uint32_t *src = (const uint32_t *)((const __nv_bfloat16 *)a.q + (use.v.tok0 + i) * a.q_strides[0] + (use.head * p.group + (r - i * p.group)) * a.q_strides[1]) + t;
+            const uint32_t *src = (const uint32_t *)((const __nv_bfloat16 *)a.q + (use.v.tok0 + i) * a.q_strides[0] + (use.head * p.group + (r - i * p.group)) * a.q_strides[1] + dg * MT * 16) + t;
 #pragma unroll
             for (int x = 0; x < MT; ++x)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) qf[x][j] = r < rows ? src[x * 8 + j * 4] : 0u;
+                for (int j = 0; j < 2; ++j) qf[q][x][j] = r < rows ? src[x * 8 + j * 4] : 0u;
         }
         for (const int end = min(use.units, use.unit + count - it); use.unit < end; ++use.unit) {
             cp_async_wait<S - 2>();
-            if constexpr (RG > 1) asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * RG) : "memory");
+            if constexpr (DG > 1) asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * DG) : "memory");
             else __syncwarp();
             const uint32_t bad = (uint32_t)missing & 0xffffu;
             ask(slot == 0 ? S - 1 : slot - 1);
 
             // ---- scores of 16 keys ----
             const uint32_t stage = ring + slot * STAGE;
-            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s2[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            float s[NQ][4] = {}, s2[NQ][4] = {};
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 uint32_t kf[4];
                 ldsm4(kf, stage + k_lane + i * 32);
-                mma_bf16(i & 1 ? s2 : s, kf, qf[i][0], qf[i][1]);
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) mma_bf16(i & 1 ? s2[q] : s[q], kf, qf[q][i][0], qf[q][i][1]);
+            }
+            if constexpr (DG > 1) {         // both halves add in the same order, and go on with the same scores
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) half_sm[(dg * NQ + q) * 32 + lane] = make_float4(s[q][0] + s2[q][0], s[q][1] + s2[q][1], s[q][2] + s2[q][2], s[q][3] + s2[q][3]);
+                asm volatile("bar.sync %0, %1;" ::"r"(1 + KG + kg), "n"(32 * DG) : "memory");
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    const float4 a0 = half_sm[q * 32 + lane], a1 = half_sm[(NQ + q) * 32 + lane];
+                    s[q][0] = a0.x; s[q][1] = a0.y; s[q][2] = a0.z; s[q][3] = a0.w;
+                    s2[q][0] = a1.x; s2[q][1] = a1.y; s2[q][2] = a1.z; s2[q][3] = a1.w;
+                }
             }
             const int key0 = (use.unit * KG + kg) * 16;
             const bool edge = key0 + 16 > lim_first || bad;        // a row of the tile does not see all of these keys, or a page is missing
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] = (s[j] + s2[j]) * p.scale2;
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[q][j] = (s[q][j] + s2[q][j]) * p.scale2;
             if (edge) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = g + (j >> 1) * 8;
-                    if (bad >> at & 1) s[j] = __int_as_float(0x7fc00000);
-                    if (key0 + at >= lim[j & 1]) s[j] = -INFINITY;
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int at = g + (j >> 1) * 8;
+                        if (bad >> at & 1) s[q][j] = __int_as_float(0x7fc00000);
+                        if (key0 + at >= lim[q][j & 1]) s[q][j] = -INFINITY;
+                    }
+            }
+            // ---- probabilities, against a reference that follows the maximum from afar: a score may stand up to 2^8 over it, where nothing is near a limit or less exact, so that
+            // after a segment's first keys no maximum is taken and nothing is scaled again ----
+            bool higher = false;
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) higher |= s[q][j] > top[q][j & 1] + 8.0f;
+            if (__any_sync(~0u, higher)) {
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    float keep[2];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        float m = fmaxf(s[q][j], s[q][j + 2]);
+                        m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
+                        m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+                        m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
+                        m = fmaxf(m, top[q][j]);
+                        keep[j] = ex2(top[q][j] - (m == -INFINITY ? 0.0f : m));
+                        top[q][j] = m;
+                        sum[q][j] *= keep[j];
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[q][i][j] *= keep[j & 1];
                 }
             }
-            // ---- running maximum and sum ----
-            float next[2], ref[2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float m = fmaxf(s[j], s[j + 2]);
-                m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
-                m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
-                m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
-                next[j] = fmaxf(top[j], m);
-                ref[j] = next[j] == -INFINITY ? 0.0f : next[j];
-            }
-            if (__any_sync(~0u, next[0] > top[0] || next[1] > top[1])) {
-                const float keep[2] = {ex2(top[0] - ref[0]), ex2(top[1] - ref[1])};
+            for (int q = 0; q < NQ; ++q)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) { top[j] = next[j]; sum[j] *= keep[j]; }
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[i][j] *= keep[j & 1];
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { s[j] = ex2(s[j] - ref[j & 1]); sum[j & 1] += s[j]; }
+                for (int j = 0; j < 4; ++j) {
+                    s[q][j] = ex2(s[q][j] - (top[q][j & 1] == -INFINITY ? 0.0f : top[q][j & 1]));
+                    sum[q][j & 1] += s[q][j];
+                }
             // ---- p v ----
             // Keys that some rows of the tile see and others do not: a masked probability of 0 would still make NaN of an infinite value, so these keys stay out of the MMA and are
             // added row by row.  There are fewer of them in all than new tokens in the tile.
@@ -392,143 +424,148 @@ __global__ void __launch_bounds__(32 * RG * KG) paged_attention_kernel(const __g
                 const int to = min(use.keys - key0, 16);
                 for (int x = from; x < to; ++x) {
                     const int owner = (x & 7) * 4 + t;
-                    const float pa = __shfl_sync(~0u, x & 8 ? s[2] : s[0], owner), pb = __shfl_sync(~0u, x & 8 ? s[3] : s[1], owner);
-                    const bool see_a = key0 + x < lim[0], see_b = key0 + x < lim[1];
-                    const __nv_bfloat16 *v = (const __nv_bfloat16 *)(smem + (stage - smem_u32(smem)) + (16 + x) * PITCH) + g;
+                    const __nv_bfloat16 *v = (const __nv_bfloat16 *)(smem + (stage - smem_u32(smem)) + (16 + x) * PITCH) + dg * MT * 16 + g;
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
+                    for (int q = 0; q < NQ; ++q) {
+                        const float pa = __shfl_sync(~0u, x & 8 ? s[q][2] : s[q][0], owner), pb = __shfl_sync(~0u, x & 8 ? s[q][3] : s[q][1], owner);
+                        const bool see_a = key0 + x < lim[q][0], see_b = key0 + x < lim[q][1];
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const float val = __bfloat162float(v[i * 16 + j * 8]);
-                            if (see_a) o[i][2 * j] += pa * val;
-                            if (see_b) o[i][2 * j + 1] += pb * val;
-                        }
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const float val = __bfloat162float(v[i * 16 + j * 8]);
+                                if (see_a) o[q][i][2 * j] += pa * val;
+                                if (see_b) o[q][i][2 * j + 1] += pb * val;
+                            }
+                    }
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (g + (j >> 1) * 8 >= from) s[j] = 0.0f;
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (g + (j >> 1) * 8 >= from) s[q][j] = 0.0f;
             }
             // the probabilities of eight keys, turned over: queries on g, keys 2 t and 2 t + 1, as the B operand has them
-            uint32_t big[2], small[2];
+            uint32_t big[NQ][2], small[NQ][2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                bf16_parts(s[2 * j], s[2 * j + 1], big[j], small[j]);
-                big[j] = transpose8(big[j]);
-                small[j] = transpose8(small[j]);
-            }
-            if (split) {
-                const uint32_t vm0 = (2 * t < from ? 0xffffu : 0u) | (2 * t + 1 < from ? 0xffff0000u : 0u), vm1 = (2 * t + 8 < from ? 0xffffu : 0u) | (2 * t + 9 < from ? 0xffff0000u : 0u);
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    bf16_parts(s[q][2 * j], s[q][2 * j + 1], big[q][j], small[q][j]);
+                    big[q][j] = transpose8(big[q][j]);
+                    small[q][j] = transpose8(small[q][j]);
+                }
+            const uint32_t vm0 = (2 * t < from ? 0xffffu : 0u) | (2 * t + 1 < from ? 0xffff0000u : 0u), vm1 = (2 * t + 8 < from ? 0xffffu : 0u) | (2 * t + 9 < from ? 0xffff0000u : 0u);
+            auto values = [&](bool masked) {
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
                     uint32_t vf[4];
                     ldsm4_t(vf, stage + v_lane + i * 32);
-                    vf[0] &= vm0; vf[1] &= vm0; vf[2] &= vm1; vf[3] &= vm1;
-                    mma_bf16(o[i], vf, big[0], big[1]);
-                    mma_bf16(o[i], vf, small[0], small[1]);
-                }
-            } else {
+                    if (masked) { vf[0] &= vm0; vf[1] &= vm0; vf[2] &= vm1; vf[3] &= vm1; }
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    uint32_t vf[4];
-                    ldsm4_t(vf, stage + v_lane + i * 32);
-                    mma_bf16(o[i], vf, big[0], big[1]);
-                    mma_bf16(o[i], vf, small[0], small[1]);
+                    for (int q = 0; q < NQ; ++q) {
+                        mma_bf16(o[q][i], vf, big[q][0], big[q][1]);
+                        mma_bf16(o[q][i], vf, small[q][0], small[q][1]);
+                    }
                 }
-            }
+            };
+            if (split) values(true);
+            else values(false);
             if (++slot == S) slot = 0;
             ++it;
         }
 
-        // ---- the end of this block's part of a segment: key groups joined, from the last to the first ----
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int x = 4; x < 32; x *= 2) sum[j] += __shfl_xor_sync(~0u, sum[j], x);
+        // ---- the end of this block's part of a segment: key groups joined, from the first to the last ----
         constexpr int MINE = MT / KG, TURNS = Shape::TURNS;       // dimension tiles that a key group adds up, the turns of the exchange
-        float sum_o[MINE][4];
-        if constexpr (KG > 1) {
-            if (g == 0)
-                for (int j = 0; j < 2; ++j) stat_sm[kg * ROWS + rg * 8 + 2 * t + j] = make_float2(top[j], sum[j]);
-            const int used = (slot == 0 ? S - 1 : slot - 1) * STAGE;
-            if constexpr (RG > 1) asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * RG) : "memory");      // nobody reads that stage any more
-            else __syncwarp();
-            float keep[KG][2];
+        float sum_o[NQ][MINE][4], keep[NQ][KG][2];
 #pragma unroll
-            for (int h = 0; h < TURNS; ++h) {
-                float4 *box = (float4 *)(smem + kg * S * STAGE + used) + rg * 2 * D / TURNS + lane;
+        for (int q = 0; q < NQ; ++q)
 #pragma unroll
-                for (int i = 0; i < MT / TURNS; ++i) {
-                    const float(&v)[4] = o[h * (MT / TURNS) + i];
-                    box[i * 32] = make_float4(v[0], v[1], v[2], v[3]);
+            for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                for (int x = 4; x < 32; x *= 2) sum[q][j] += __shfl_xor_sync(~0u, sum[q][j], x);
+                if (g == 0 && dg == 0) stat_sm[kg * ROWS + q * 8 + 2 * t + j] = make_float2(top[q][j], sum[q][j]);
+            }
+        const int used = (slot == 0 ? S - 1 : slot - 1) * STAGE;
+        if constexpr (DG > 1) asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * DG) : "memory");      // nobody reads that stage any more
+        else __syncwarp();
+#pragma unroll
+        for (int h = 0; h < TURNS; ++h) {
+            constexpr int PART = MT / TURNS;
+            float4 *box = (float4 *)(smem + kg * S * STAGE + used) + dg * NQ * PART * 32 + lane;
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                for (int i = 0; i < PART; ++i) {
+                    const float(&v)[4] = o[q][h * PART + i];
+                    box[(q * PART + i) * 32] = make_float4(v[0], v[1], v[2], v[3]);
                 }
-                __syncthreads();
-                if (h == 0) {
+            __syncthreads();
+            if (h == 0) {
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        const float2 *st = stat_sm + rg * 8 + 2 * t + j;
+                        const float2 *st = stat_sm + q * 8 + 2 * t + j;
                         float m = -INFINITY;
                         for (int x = 0; x < KG; ++x) m = fmaxf(m, st[x * ROWS].x);
                         const float r = m == -INFINITY ? 0.0f : m;
-                        top[j] = m;
-                        sum[j] = 0.0f;
+                        top[q][j] = m;
+                        sum[q][j] = 0.0f;
 #pragma unroll
                         for (int x = 0; x < KG; ++x) {
-                            keep[x][j] = ex2(st[x * ROWS].x - r);
-                            sum[j] += st[x * ROWS].y * keep[x][j];
+                            keep[q][x][j] = ex2(st[x * ROWS].x - r);
+                            sum[q][j] += st[x * ROWS].y * keep[q][x][j];
                         }
                     }
-                }
+            }
+#pragma unroll
+            for (int q = 0; q < NQ; ++q)
 #pragma unroll
                 for (int i = 0; i < MINE / TURNS; ++i) {
-                    float(&v)[4] = sum_o[h * (MINE / TURNS) + i];
+                    float(&v)[4] = sum_o[q][h * (MINE / TURNS) + i];
                     v[0] = v[1] = v[2] = v[3] = 0.0f;
 #pragma unroll
                     for (int x = 0; x < KG; ++x) {
-                        const float4 w = ((const float4 *)(smem + x * S * STAGE + used))[rg * 2 * D / TURNS + (i * KG + kg) * 32 + lane];
-                        v[0] += w.x * keep[x][0]; v[1] += w.y * keep[x][1]; v[2] += w.z * keep[x][0]; v[3] += w.w * keep[x][1];
+                        const float4 w = ((const float4 *)(smem + x * S * STAGE + used))[dg * NQ * PART * 32 + (q * PART + i * KG + kg) * 32 + lane];
+                        v[0] += w.x * keep[q][x][0]; v[1] += w.y * keep[q][x][1]; v[2] += w.z * keep[q][x][0]; v[3] += w.w * keep[q][x][1];
                     }
                 }
-                __syncthreads();            // the next turn, or the next stage, comes to the same place
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < MINE; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sum_o[i][j] = o[i][j];
+            __syncthreads();            // the next turn, or the next stage, comes to the same place
         }
-        auto dim_of = [&](int i) { return ((i / (MINE / TURNS)) * (MT / TURNS) + (i % (MINE / TURNS)) * KG + kg) * 16 + g; };       // of sum_o[i][0], [1]; 8 more: of [2], [3]
-        {
-            const bool whole = unit0 == 0 && use.unit == use.units;
-            const int64_t part = 2 * (int64_t)blockIdx.x + (unit0 == 0);
+        auto dim_of = [&](int i) { return ((i / (MINE / TURNS)) * (MT / TURNS) + (i % (MINE / TURNS)) * KG + kg + dg * MT) * 16 + g; };       // of sum_o[.][i][0], [1]; 8 more: of [2], [3]
+        const bool whole = unit0 == 0 && use.unit == use.units;
+        const int64_t part = 2 * (int64_t)blockIdx.x + (unit0 == 0);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int r = use.tile * ROWS + rg * 8 + 2 * t + j;
-                if (r >= use.v.n * p.group) continue;
+                const int in_tile = q * 8 + 2 * t + j, r = use.tile * ROWS + in_tile;
+                if (r >= rows) continue;
                 if (whole) {
                     const int i0 = (unsigned)r / (unsigned)p.group;
                     const int64_t tok = use.v.tok0 + i0, h = use.head * p.group + (r - i0 * p.group);
                     __nv_bfloat16 *dst = (__nv_bfloat16 *)a.out + tok * a.out_strides[0] + h * a.out_strides[1];
                     const __nv_bfloat16 *gate = a.gate ? (const __nv_bfloat16 *)a.gate + tok * a.gate_strides[0] + h * a.gate_strides[1] : nullptr;
-                    const float inv = sum[j] == 0.0f ? 0.0f : 1.0f / sum[j];
+                    const float inv = sum[q][j] == 0.0f ? 0.0f : 1.0f / sum[q][j];
 #pragma unroll
                     for (int i = 0; i < MINE; ++i)
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             const int d = dim_of(i) + 8 * x;
-                            float v = sum_o[i][2 * x + j] * inv;
+                            float v = sum_o[q][i][2 * x + j] * inv;
                             if (gate) v /= 1.0f + ex2(-1.4426950408889634f * __bfloat162float(gate[d]));
                             dst[d] = __float2bfloat16_rn(v);
                         }
                 } else {
-                    const int64_t at = part * ROWS + rg * 8 + 2 * t + j;
-                    if (g == 0 && kg == 0) p.stats[at] = make_float2(top[j], sum[j]);
+                    const int64_t at = part * ROWS + in_tile;
+                    if (g == 0 && kg == 0 && dg == 0) p.stats[at] = make_float2(top[q][j], sum[q][j]);
 #pragma unroll
                     for (int i = 0; i < MINE; ++i)
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) p.parts[at * D + dim_of(i) + 8 * x] = sum_o[i][2 * x + j];
+                        for (int x = 0; x < 2; ++x) p.parts[at * D + dim_of(i) + 8 * x] = sum_o[q][i][2 * x + j];
                 }
             }
-        }
         if (it == count) break;
         next_segment<ROWS, UNIT>(p, use);
     }
