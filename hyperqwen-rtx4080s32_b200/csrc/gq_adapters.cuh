@@ -28,6 +28,7 @@ struct LowRankParams {
     int64_t ld_base, ldx, ld_out, n_total;
     int64_t edges[9];            // first column of each shard, and the end
     int M, K, n_shards, n_adapters, rank, ranks, parts, wide_ids;       // ranks: the rank as the outer products see it, 16, 32, 64 or 128
+    int group_blocks;            // blocks along z that share a tile's adapters; the others take further ranks
     int vec;                     // base and out can be read and written 16 bytes at a time
 };
 
@@ -96,7 +97,8 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_inner_kernel(const __grid
     pdl_wait();
     pdl_trigger();
     group_rows(p, row0, groups);
-    for (int s = blockIdx.z; s < groups.groups; s += gridDim.z) {
+    const int tile0 = blockIdx.z / p.group_blocks * MT;            // this block's ranks, in sixteens over all shards
+    for (int s = blockIdx.z % p.group_blocks; s < groups.groups; s += p.group_blocks) {
         const int id = groups.id[s], at = groups.start[s], count = groups.start[s + 1] - at;
         if (id < 0) continue;
         const int row_warps = count <= 16 ? 1 : count <= 32 ? 2 : 4, k_warps = LR_WARPS / row_warps, rw = warp % row_warps, kw = warp / row_warps;
@@ -106,84 +108,82 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_inner_kernel(const __grid
             const int r = rw * 16 + j * 8 + g;
             x[j] = p.x + (int64_t)(row0 + groups.list[at + min(r, count - 1)]) * p.ldx + t * 8;
         }
-        for (int tile0 = 0; tile0 < tiles; tile0 += MT) {
-            const __nv_bfloat16 *a[MT][2];
+        const __nv_bfloat16 *a[MT][2];
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int tile = min(tile0 + i, tiles - 1), shard = tile / per_shard, r = min((tile - shard * per_shard) * 16 + j * 8 + g, p.rank - 1);
-                    a[i][j] = p.a + ((int64_t)id * p.n_shards * p.rank + shard * p.rank + r) * p.K + t * 8;
-                }
-            float acc[MT][2][4] = {};
-            // two steps at a time, the 128 bytes of a row that lie side by side
+            for (int j = 0; j < 2; ++j) {
+                const int tile = min(tile0 + i, tiles - 1), shard = tile / per_shard, r = min((tile - shard * per_shard) * 16 + j * 8 + g, p.rank - 1);
+                a[i][j] = p.a + ((int64_t)id * p.n_shards * p.rank + shard * p.rank + r) * p.K + t * 8;
+            }
+        float acc[MT][2][4] = {};
+        // two steps at a time, the 128 bytes of a row that lie side by side
 #pragma unroll(MT <= 2 ? 2 : 1)
-            for (int step = step0 + 2 * kw; step < step1; step += 2 * k_warps) {
-                uint4 xv[2][2], av[2][MT][2];
+        for (int step = step0 + 2 * kw; step < step1; step += 2 * k_warps) {
+            uint4 xv[2][2], av[2][MT][2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) xv[h][j] = *(const uint4 *)(x[j] + (step + h) * 32);
+                for (int j = 0; j < 2; ++j) xv[h][j] = *(const uint4 *)(x[j] + (step + h) * 32);
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) av[h][i][j] = *(const uint4 *)(a[i][j] + (step + h) * 32);
+                    for (int j = 0; j < 2; ++j) av[h][i][j] = *(const uint4 *)(a[i][j] + (step + h) * 32);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const uint4 a0 = av[h][i][0], a1 = av[h][i][1];
+                    const uint32_t lo[4] = {a0.x, a1.x, a0.y, a1.y}, hi[4] = {a0.z, a1.z, a0.w, a1.w};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        mma_bf16(acc[i][j], lo, xv[h][j].x, xv[h][j].y);
+                        mma_bf16(acc[i][j], hi, xv[h][j].z, xv[h][j].w);
+                    }
                 }
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        const uint4 a0 = av[h][i][0], a1 = av[h][i][1];
-                        const uint32_t lo[4] = {a0.x, a1.x, a0.y, a1.y}, hi[4] = {a0.z, a1.z, a0.w, a1.w};
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            mma_bf16(acc[i][j], lo, xv[h][j].x, xv[h][j].y);
-                            mma_bf16(acc[i][j], hi, xv[h][j].z, xv[h][j].w);
-                        }
-                    }
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) red[warp][j * 8 + t * 2 + (e & 1)][i * 16 + g + (e >> 1) * 8] = acc[i][j][e];
-            __syncthreads();
-            // over the warps of this block, then over the blocks of the cluster, both in order
-            for (int i = tid; i < count * MT * 16; i += LR_THREADS) {
-                const int r = i / (MT * 16), c = i - r * (MT * 16);
-                float sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < LR_WARPS; ++k)
-                    if (k < k_warps) sum += red[k * row_warps + r / 16][r % 16][c];
-                red[r / 16][r % 16][c] = sum;              // read by this thread alone so far
-            }
-            if (p.parts > 1) cluster_sync_all();
-            else __syncthreads();
-            for (int i = tid + blockIdx.x * LR_THREADS; i < count * MT * 16; i += LR_THREADS * p.parts) {
-                const int r = i / (MT * 16), c = i - r * (MT * 16), tile = tile0 + c / 16;
-                if (tile >= tiles) continue;
-                float sum = 0.0f;
-                if (p.parts > 1) {
-                    const uint32_t at = smem_u32(&red[r / 16][r % 16][c]);
-                    for (int k0 = 0; k0 < p.parts; k0 += 8) {
-                        float v[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) v[k] = k0 + k < p.parts ? ld_cluster_f32(map_to_rank(at, k0 + k)) : 0.0f;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) sum += v[k];
-                    }
-                } else sum = red[r / 16][r % 16][c];
-                const int shard = tile / per_shard, rank = (tile - shard * per_shard) * 16 + c % 16;
-                sum *= p.scales[id * p.n_shards + shard];
-                const int64_t to = (int64_t)(row0 + groups.list[at + r]) * (p.n_shards * p.ranks) + shard * p.ranks + rank;
-                const __nv_bfloat16 big = __float2bfloat16_rn(sum);
-                p.big[to] = big;
-                p.small[to] = __float2bfloat16_rn(sum - __bfloat162float(big));
-            }
-            if (p.parts > 1) cluster_sync_all();            // nobody reads this block's sums any more
-            else __syncthreads();
         }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) red[warp][j * 8 + t * 2 + (e & 1)][i * 16 + g + (e >> 1) * 8] = acc[i][j][e];
+        __syncthreads();
+        // over the warps of this block, then over the blocks of the cluster, both in order
+        for (int i = tid; i < count * MT * 16; i += LR_THREADS) {
+            const int r = i / (MT * 16), c = i - r * (MT * 16);
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < LR_WARPS; ++k)
+                if (k < k_warps) sum += red[k * row_warps + r / 16][r % 16][c];
+            red[r / 16][r % 16][c] = sum;              // read by this thread alone so far
+        }
+        if (p.parts > 1) cluster_sync_all();
+        else __syncthreads();
+        for (int i = tid + blockIdx.x * LR_THREADS; i < count * MT * 16; i += LR_THREADS * p.parts) {
+            const int r = i / (MT * 16), c = i - r * (MT * 16), tile = tile0 + c / 16;
+            if (tile >= tiles) continue;
+            float sum = 0.0f;
+            if (p.parts > 1) {
+                const uint32_t at = smem_u32(&red[r / 16][r % 16][c]);
+                for (int k0 = 0; k0 < p.parts; k0 += 8) {
+                    float v[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = k0 + k < p.parts ? ld_cluster_f32(map_to_rank(at, k0 + k)) : 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) sum += v[k];
+                }
+            } else sum = red[r / 16][r % 16][c];
+            const int shard = tile / per_shard, rank = (tile - shard * per_shard) * 16 + c % 16;
+            sum *= p.scales[id * p.n_shards + shard];
+            const int64_t to = (int64_t)(row0 + groups.list[at + r]) * (p.n_shards * p.ranks) + shard * p.ranks + rank;
+            const __nv_bfloat16 big = __float2bfloat16_rn(sum);
+            p.big[to] = big;
+            p.small[to] = __float2bfloat16_rn(sum - __bfloat162float(big));
+        }
+        if (p.parts > 1) cluster_sync_all();            // nobody reads this block's sums any more
+        else __syncthreads();
     }
 }
 
@@ -308,11 +308,12 @@ __device__ __forceinline__ int shard_of(const LowRankParams &p, int64_t block, i
     return shard;
 }
 
-// Decode: a warp by itself has 32 columns of 4 rows (the MMA's others idle): every row may have an adapter of its own, and four of them are not a long way behind one another.
-constexpr int LR_OUTER_WARPS = 4, LR_FEW = 4;
-template <int KS>
+// Decode: a warp by itself has 32 columns of TILE rows.  Where every row may have an adapter of its own TILE is 4 (the MMA's other rows idle, but no more than four adapters stand one behind
+// the other), with a small bank 16.
+constexpr int LR_OUTER_WARPS = 4;
+template <int KS, int TILE>
 __global__ void __launch_bounds__(LR_OUTER_WARPS * 32) low_rank_few_kernel(const __grid_constant__ LowRankParams p) {
-    const int lane = threadIdx.x & 31, g = lane / 4, t = lane % 4, row0 = blockIdx.y * LR_FEW, last = min(row0 + LR_FEW, p.M) - 1;
+    const int lane = threadIdx.x & 31, g = lane / 4, t = lane % 4, row0 = blockIdx.y * TILE, last = min(row0 + TILE, p.M) - 1;
     int64_t col0;
     int ncols;
     const int shard = shard_of(p, blockIdx.x, LR_OUTER_WARPS * 32, col0, ncols);
@@ -324,32 +325,41 @@ __global__ void __launch_bounds__(LR_OUTER_WARPS * 32) low_rank_few_kernel(const
     pdl_trigger();
     if (ncols <= 0) return;
     const int mine = adapter_of(p, min(row0 + (lane & 15), last));
-    uint4 w[2];
-    w[1] = make_uint4(0, 0, 0, 0);
-    const __nv_bfloat16 *src = p.base + min(row0 + g, last) * p.ld_base + col0 + n;
-    if (full) w[0] = *(const uint4 *)src;
-    else {
-        uint16_t e[8];
+    constexpr int HALVES = TILE > 8 ? 2 : 1;                       // rows g, and g + 8
+    uint4 w[2] = {};
+    int64_t at[2] = {};
 #pragma unroll
-        for (int x = 0; x < 8; ++x) e[x] = n + x < ncols ? __bfloat16_as_ushort(src[x]) : 0;
-        memcpy(&w[0], e, 16);
+    for (int j = 0; j < HALVES; ++j) {
+        const int64_t row = min(row0 + g + 8 * j, last);
+        const __nv_bfloat16 *src = p.base + row * p.ld_base + col0 + n;
+        at[j] = row * (p.n_shards * p.ranks) + shard * p.ranks;
+        if (full) w[j] = *(const uint4 *)src;
+        else {
+            uint16_t e[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) e[x] = n + x < ncols ? __bfloat16_as_ushort(src[x]) : 0;
+            memcpy(&w[j], e, 16);
+        }
     }
+    if (HALVES == 1) at[1] = at[0];
     float res[4][4];
     unpack_rows(w, res);
     uint32_t bf[4][KS][2];
     int have = -1, of_row[2];
-    const int64_t at = (int64_t)min(row0 + g, last) * (p.n_shards * p.ranks) + shard * p.ranks;
-    outer_tile<KS>(p, mine, have, bf, col0, ncols, lane, [&](int) { return p.big + at; }, [&](int) { return p.small + at; }, res, of_row);
-    if (row0 + g > last || (of_row[0] == -1 && p.out == p.base)) return;         // in place, rows without an adapter stay as they are
-    const uint4 y = pack_row(res, 0);
-    __nv_bfloat16 *dst = p.out + (row0 + g) * p.ld_out + col0 + n;
-    if (full) *(uint4 *)dst = y;
-    else {
-        uint16_t e[8];
-        memcpy(e, &y, 16);
+    outer_tile<KS>(p, mine, have, bf, col0, ncols, lane, [&](int j) { return p.big + at[j]; }, [&](int j) { return p.small + at[j]; }, res, of_row);
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-            if (n + x < ncols) dst[x] = __ushort_as_bfloat16(e[x]);
+    for (int j = 0; j < HALVES; ++j) {
+        if (row0 + g + 8 * j > last || (of_row[j] == -1 && p.out == p.base)) continue;         // in place, rows without an adapter stay as they are
+        const uint4 y = pack_row(res, j);
+        __nv_bfloat16 *dst = p.out + (row0 + g + 8 * j) * p.ld_out + col0 + n;
+        if (full) *(uint4 *)dst = y;
+        else {
+            uint16_t e[8];
+            memcpy(e, &y, 16);
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+                if (n + x < ncols) dst[x] = __ushort_as_bfloat16(e[x]);
+        }
     }
 }
 

@@ -63,11 +63,23 @@ static int check_low_rank(const gq_low_rank_args *p, int64_t *n_total) {
 }
 static int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 static int ranks_of(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
-// adapters that a tile of rows may hold, and the parts that K is cut into: blocks for the whole GPU, 256 of K to a part at least, a cluster of sixteen at most
-static int low_rank_groups(const gq_low_rank_args *p) { return (int)std::min<int64_t>(std::min<int64_t>(p->M, LR_ROWS), p->n_adapters); }
-static int low_rank_parts(const gq_low_rank_args *p) {
-    const int64_t tiles = (p->M + LR_ROWS - 1) / LR_ROWS, blocks = tiles * (tiles == 1 ? low_rank_groups(p) : 1);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, p->K / 256), 296 / std::max<int64_t>(blocks, 1)));
+// How the inner products are cut: ranks of a block in sixteens (as many as leave every SM a block), blocks for a tile's adapters, parts of K (256 at least, a cluster of sixteen at most).
+// m1 qkv of rank 16: three blocks of one sixteen in 16 parts 2.9 us, one of three 4.6.
+struct LowRankCut {
+    int ranks, groups, parts, turns;
+};
+static LowRankCut low_rank_cut(const gq_low_rank_args *p) {
+    const int64_t tiles = (p->M + LR_ROWS - 1) / LR_ROWS;
+    const int sixteens = p->n_shards * ((p->rank + 15) / 16), most = (int)std::min<int64_t>(16, p->K / 256);
+    LowRankCut c{};
+    c.groups = tiles == 1 ? (int)std::min<int64_t>(std::min<int64_t>(p->M, LR_ROWS), p->n_adapters) : 1;
+    for (int n = 4; n >= 1; --n) {
+        c.turns = (sixteens + n - 1) / n;
+        c.ranks = (sixteens + c.turns - 1) / c.turns;
+        if (c.turns * tiles * c.groups * most >= 148) break;
+    }
+    c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, 296 / (c.turns * tiles * c.groups)));
+    return c;
 }
 extern "C" int64_t gq_low_rank_workspace_bytes(const gq_low_rank_args *p) {
     int64_t n = 0;
@@ -95,12 +107,13 @@ template <int MT> static cudaError_t low_rank_inner(const LowRankParams &q, dim3
 }
 template <int KS> static int low_rank_outer(const LowRankParams &q, void *stream) {
     using Shape = ChunkShape<KS>;
-    const bool few = q.M <= 128;
+    const bool few = q.M <= 64, own = q.n_adapters > 4;        // decode, and whether the rows of a tile may all have their own
     const int cols = few ? LR_OUTER_WARPS * 32 : Shape::COLS;
     int64_t blocks = 0;
     for (int s = 0; s < q.n_shards; ++s) blocks += (q.edges[s + 1] - q.edges[s] + cols - 1) / cols;
     if (few) {
-        GQ_CUDA(launch_pdl(low_rank_few_kernel<KS>, dim3((unsigned)blocks, (q.M + LR_FEW - 1) / LR_FEW), LR_OUTER_WARPS * 32, 0, stream, q));
+        if (own) GQ_CUDA(launch_pdl(low_rank_few_kernel<KS, 4>, dim3((unsigned)blocks, (q.M + 3) / 4), LR_OUTER_WARPS * 32, 0, stream, q));
+        else GQ_CUDA(launch_pdl(low_rank_few_kernel<KS, 16>, dim3((unsigned)blocks, (q.M + 15) / 16), LR_OUTER_WARPS * 32, 0, stream, q));
     } else {                      // as many walks down the rows as the GPU holds blocks, at least one for every block of columns
         int resident = 0;
         if (const int rc = resident_blocks<low_rank_chunk_kernel<KS>>(LR_THREADS, Shape::SMEM, &resident)) return rc;
@@ -121,18 +134,18 @@ extern "C" int gq_low_rank_add(const gq_low_rank_args *p, void *stream) {
     int *status;
     if (const int rc = status_word(&status)) return rc;
     const int64_t tiles = (p->M + LR_ROWS - 1) / LR_ROWS;
+    const LowRankCut cut = low_rank_cut(p);
     bool vec = aligned(p->base, 16) && aligned(p->out, 16) && p->ld_base % 8 == 0 && p->ld_out % 8 == 0;
     LowRankParams q{(const __nv_bfloat16 *)p->base, (const __nv_bfloat16 *)p->x, (const __nv_bfloat16 *)p->a, (const __nv_bfloat16 *)p->b, p->scales, p->ids,
                     (__nv_bfloat16 *)p->out, (__nv_bfloat16 *)p->workspace, (__nv_bfloat16 *)((uint8_t *)p->workspace + bytes / 2), status, p->ld_base, p->ldx, p->ld_out, n, {0},
-                    (int)p->M, (int)p->K, p->n_shards, p->n_adapters, p->rank, ranks_of(p->rank), low_rank_parts(p), p->ids_bytes == 8, 0};
+                    (int)p->M, (int)p->K, p->n_shards, p->n_adapters, p->rank, ranks_of(p->rank), cut.parts, p->ids_bytes == 8, cut.groups, 0};
     for (int s = 0; s < p->n_shards; ++s) {
         q.edges[s + 1] = q.edges[s] + p->n_outs[s];
         vec = vec && q.edges[s] % 8 == 0;
     }
     q.vec = vec;
-    const dim3 inner(q.parts, (unsigned)tiles, tiles == 1 ? low_rank_groups(p) : 1);
-    const int rank_tiles = p->n_shards * ((p->rank + 15) / 16);              // a warp's turn: as many as divide them, up to four
-    switch (rank_tiles <= 4 ? rank_tiles : rank_tiles % 4 && rank_tiles % 3 == 0 ? 3 : 4) {
+    const dim3 inner(cut.parts, (unsigned)tiles, cut.groups * cut.turns);
+    switch (cut.ranks) {
         case 1: GQ_CUDA(low_rank_inner<1>(q, inner, stream)); break;
         case 2: GQ_CUDA(low_rank_inner<2>(q, inner, stream)); break;
         case 3: GQ_CUDA(low_rank_inner<3>(q, inner, stream)); break;
