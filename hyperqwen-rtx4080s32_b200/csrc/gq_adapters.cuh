@@ -84,6 +84,36 @@ __device__ __forceinline__ void group_rows(const LowRankParams &p, int row0, Row
     __syncthreads();
 }
 
+// The sums of `count` rows and RANKS ranks, `of(row, rank)` in every block's shared memory, over the blocks of the cluster in order -> the workspace
+template <int RANKS, class OF> __device__ __forceinline__ void store_inner(const LowRankParams &p, const RowGroups &groups, int at, int count, int id, int row0, int tile0, OF of) {
+    const int per_shard = (p.rank + 15) / 16, tiles = p.n_shards * per_shard;
+    if (p.parts > 1) cluster_sync_all();
+    else __syncthreads();
+    for (int i = threadIdx.x + blockIdx.x * LR_THREADS; i < count * RANKS; i += LR_THREADS * p.parts) {
+        const int r = i / RANKS, c = i - r * RANKS, tile = tile0 + c / 16;
+        if (tile >= tiles) continue;
+        float sum = 0.0f;
+        if (p.parts > 1) {
+            const uint32_t from = smem_u32(of(r, c));
+            for (int k0 = 0; k0 < p.parts; k0 += 8) {
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = k0 + k < p.parts ? ld_cluster_f32(map_to_rank(from, k0 + k)) : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum += v[k];
+            }
+        } else sum = *of(r, c);
+        const int shard = tile / per_shard, rank = (tile - shard * per_shard) * 16 + c % 16;
+        sum *= p.scales[id * p.n_shards + shard];
+        const int64_t to = (int64_t)(row0 + groups.list[at + r]) * (p.n_shards * p.ranks) + shard * p.ranks + rank;
+        const __nv_bfloat16 big = __float2bfloat16_rn(sum);
+        p.big[to] = big;
+        p.small[to] = __float2bfloat16_rn(sum - __bfloat162float(big));
+    }
+    if (p.parts > 1) cluster_sync_all();            // nobody reads this block's sums any more
+    else __syncthreads();
+}
+
 // The sums over part blockIdx.x of K of a tile's inner products.  Ranks on M, rows on N.  A warp takes 16 rows and 16 MT ranks at a time; warps that are not needed for rows share the steps
 // of 32 k, and their sums are added in order through shared memory.  Lanes without a row or a rank read another's: what they compute is not looked at, and no load waits behind a branch.
 template <int MT>
@@ -159,31 +189,78 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_inner_kernel(const __grid
                 if (k < k_warps) sum += red[k * row_warps + r / 16][r % 16][c];
             red[r / 16][r % 16][c] = sum;              // read by this thread alone so far
         }
-        if (p.parts > 1) cluster_sync_all();
-        else __syncthreads();
-        for (int i = tid + blockIdx.x * LR_THREADS; i < count * MT * 16; i += LR_THREADS * p.parts) {
-            const int r = i / (MT * 16), c = i - r * (MT * 16), tile = tile0 + c / 16;
-            if (tile >= tiles) continue;
-            float sum = 0.0f;
-            if (p.parts > 1) {
-                const uint32_t at = smem_u32(&red[r / 16][r % 16][c]);
-                for (int k0 = 0; k0 < p.parts; k0 += 8) {
-                    float v[8];
+        store_inner<MT * 16>(p, groups, at, count, id, row0, tile0, [&](int r, int c) { return &red[r / 16][r % 16][c]; });
+    }
+}
+
+// The same for chunks, where a tile's rows mostly share an adapter and A is read by many: 64 rows times RANKS ranks, both through shared memory in steps of 64 k (cp.async, a ring of four;
+// rows at a pitch of 144 bytes, so that ldmatrix meets no bank twice).  Rows on M; a warp has 16 rows and half of the ranks.
+template <int RANKS> struct InnerShape {
+    static constexpr int PITCH = 144, STAGES = 4, STAGE = (LR_ROWS + RANKS) * PITCH, SMEM = STAGES * STAGE, RED = RANKS + 4;
+    static_assert(LR_ROWS * RED * 4 <= SMEM, "the sums take the ring's place");
+};
+template <int RANKS>
+__global__ void __launch_bounds__(LR_THREADS) low_rank_inner_chunk_kernel(const __grid_constant__ LowRankParams p) {
+    using Shape = InnerShape<RANKS>;
+    constexpr int PITCH = Shape::PITCH, S = Shape::STAGES, NT = RANKS / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ RowGroups groups;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane % 4, rw = warp % 4, cw = warp / 4;
+    const int row0 = blockIdx.y * LR_ROWS, blocks = p.K / 64, per_shard = (p.rank + 15) / 16, tiles = p.n_shards * per_shard, tile0 = blockIdx.z * (RANKS / 16);
+    const int k0 = (int)((int64_t)blockIdx.x * blocks / p.parts), k1 = (int)((int64_t)(blockIdx.x + 1) * blocks / p.parts);
+    pdl_wait();
+    pdl_trigger();
+    group_rows(p, row0, groups);
+    float(*red)[Shape::RED] = (float(*)[Shape::RED])smem;
+    for (int s = 0; s < groups.groups; ++s) {
+        const int id = groups.id[s], at = groups.start[s], count = groups.start[s + 1] - at;
+        if (id < 0) continue;
+        // 16 bytes of a row or rank at a time: 8 threads to a row; rows and ranks that are not there are read as the last
+        const __nv_bfloat16 *src[2 + RANKS / 32];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = k0 + k < p.parts ? ld_cluster_f32(map_to_rank(at, k0 + k)) : 0.0f;
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) sum += v[k];
-                }
-            } else sum = red[r / 16][r % 16][c];
-            const int shard = tile / per_shard, rank = (tile - shard * per_shard) * 16 + c % 16;
-            sum *= p.scales[id * p.n_shards + shard];
-            const int64_t to = (int64_t)(row0 + groups.list[at + r]) * (p.n_shards * p.ranks) + shard * p.ranks + rank;
-            const __nv_bfloat16 big = __float2bfloat16_rn(sum);
-            p.big[to] = big;
-            p.small[to] = __float2bfloat16_rn(sum - __bfloat162float(big));
+        for (int j = 0; j < 2 + RANKS / 32; ++j) {
+            const int r = tid / 8 + 32 * (j & 1), c = (tid & 7) * 8;
+            if (j < 2) src[j] = p.x + (int64_t)(row0 + groups.list[at + min(r, count - 1)]) * p.ldx + c;
+            else {
+                const int q = tid / 8 + 32 * (j - 2), tile = min(tile0 + q / 16, tiles - 1), shard = tile / per_shard, rank = min((tile - shard * per_shard) * 16 + q % 16, p.rank - 1);
+                src[j] = p.a + ((int64_t)id * p.n_shards * p.rank + shard * p.rank + rank) * p.K + c;
+            }
         }
-        if (p.parts > 1) cluster_sync_all();            // nobody reads this block's sums any more
-        else __syncthreads();
+        auto ask = [&](int k) {
+            if (k < k1) {
+                const uint32_t to = smem_u32(smem) + (k - k0) % S * Shape::STAGE + tid / 8 * PITCH + (tid & 7) * 16;
+#pragma unroll
+                for (int j = 0; j < 2 + RANKS / 32; ++j) cp_async16(to + j * 32 * PITCH, src[j] + k * 64);
+            }
+            cp_async_commit();
+        };
+        for (int i = 0; i < S - 1; ++i) ask(k0 + i);
+        float acc[NT][4] = {};
+        for (int k = k0; k < k1; ++k) {
+            cp_async_wait<S - 2>();
+            __syncthreads();
+            ask(k + S - 1);
+            const uint32_t stage = smem_u32(smem) + (k - k0) % S * Shape::STAGE;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                uint32_t xf[4];
+                ldsm4(xf, stage + (rw * 16 + (lane & 15)) * PITCH + h * 32 + (lane >> 4) * 16);
+#pragma unroll
+                for (int i = 0; i < NT; i += 2) {
+                    uint32_t af[4];
+                    ldsm4(af, stage + (LR_ROWS + cw * (RANKS / 2) + i * 8 + (lane >> 4) * 8 + (lane & 7)) * PITCH + h * 32 + ((lane >> 3) & 1) * 16);
+                    mma_bf16(acc[i], xf, af[0], af[1]);
+                    mma_bf16(acc[i + 1], xf, af[2], af[3]);
+                }
+            }
+        }
+        cp_async_wait<0>();
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) red[rw * 16 + g + (e >> 1) * 8][cw * (RANKS / 2) + i * 8 + t * 2 + (e & 1)] = acc[i][e];
+        store_inner<RANKS>(p, groups, at, count, id, row0, tile0, [&](int r, int c) { return &red[r][c]; });
     }
 }
 

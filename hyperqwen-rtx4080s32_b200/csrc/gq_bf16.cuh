@@ -17,6 +17,11 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
     return u;
 }
 
+// four 8 x 8 tiles of 16-bit values from shared memory, lane l naming a row of tile l / 8
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
 // 16 bytes from global to shared memory, asynchronously
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
 // the same, or 16 zeros

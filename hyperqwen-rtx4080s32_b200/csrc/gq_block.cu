@@ -72,13 +72,20 @@ static LowRankCut low_rank_cut(const gq_low_rank_args *p) {
     const int64_t tiles = (p->M + LR_ROWS - 1) / LR_ROWS;
     const int sixteens = p->n_shards * ((p->rank + 15) / 16), most = (int)std::min<int64_t>(16, p->K / 256);
     LowRankCut c{};
-    c.groups = tiles == 1 ? (int)std::min<int64_t>(std::min<int64_t>(p->M, LR_ROWS), p->n_adapters) : 1;
+    if (tiles > 1) {             // chunks: 32 or 64 ranks to a block, three blocks to an SM
+        c.ranks = sixteens <= 2 ? 2 : 4;
+        c.groups = 1;
+        c.turns = (sixteens + c.ranks - 1) / c.ranks;
+        c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, 444 / (c.turns * tiles)));
+        return c;
+    }
+    c.groups = (int)std::min<int64_t>(std::min<int64_t>(p->M, LR_ROWS), p->n_adapters);
     for (int n = 4; n >= 1; --n) {
         c.turns = (sixteens + n - 1) / n;
         c.ranks = (sixteens + c.turns - 1) / c.turns;
-        if (c.turns * tiles * c.groups * most >= 148) break;
+        if (c.turns * c.groups * most >= 148) break;
     }
-    c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, 296 / (c.turns * tiles * c.groups)));
+    c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, 296 / (c.turns * c.groups)));
     return c;
 }
 extern "C" int64_t gq_low_rank_workspace_bytes(const gq_low_rank_args *p) {
@@ -86,24 +93,26 @@ extern "C" int64_t gq_low_rank_workspace_bytes(const gq_low_rank_args *p) {
     if (const int rc = check_low_rank(p, &n)) return rc;
     return n == 0 ? 0 : 2 * up256(p->M * p->n_shards * ranks_of(p->rank) * 2);
 }
-template <int MT> static cudaError_t low_rank_inner(const LowRankParams &q, dim3 grid, void *stream) {
+// the inner products, a cluster to the parts of K
+template <auto KERNEL> static int low_rank_inner(const LowRankParams &q, dim3 grid, int smem, void *stream) {
+    static std::atomic<uint64_t> allowed{0};         // devices that know of the shared memory and of more than the portable cluster
+    int dev = 0;
+    GQ_CUDA(cudaGetDevice(&dev));
+    if (dev >= 64 || !(allowed.load() >> dev & 1)) {
+        if (smem) GQ_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        GQ_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        if (dev < 64) allowed.fetch_or((uint64_t)1 << dev);
+    }
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = q.parts; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid; cfg.blockDim = dim3(LR_THREADS); cfg.stream = (cudaStream_t)stream; cfg.attrs = attr; cfg.numAttrs = 2;
-    if (q.parts > 8) {            // more than the portable cluster: allowed once per device
-        static std::atomic<uint64_t> allowed{0};
-        int dev = 0;
-        if (const cudaError_t e = cudaGetDevice(&dev)) return e;
-        if (dev >= 64 || !(allowed.load() >> dev & 1)) {
-            if (const cudaError_t e = cudaFuncSetAttribute(low_rank_inner_kernel<MT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
-            if (dev < 64) allowed.fetch_or((uint64_t)1 << dev);
-        }
-    }
-    return cudaLaunchKernelEx(&cfg, low_rank_inner_kernel<MT>, q);
+    cfg.gridDim = grid; cfg.blockDim = dim3(LR_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = (cudaStream_t)stream; cfg.attrs = attr; cfg.numAttrs = 2;
+    GQ_CUDA(cudaLaunchKernelEx(&cfg, KERNEL, q));
+    GQ_LAUNCHED();
+    return GQ_OK;
 }
 template <int KS> static int low_rank_outer(const LowRankParams &q, void *stream) {
     using Shape = ChunkShape<KS>;
@@ -145,13 +154,13 @@ extern "C" int gq_low_rank_add(const gq_low_rank_args *p, void *stream) {
     }
     q.vec = vec;
     const dim3 inner(cut.parts, (unsigned)tiles, cut.groups * cut.turns);
-    switch (cut.ranks) {
-        case 1: GQ_CUDA(low_rank_inner<1>(q, inner, stream)); break;
-        case 2: GQ_CUDA(low_rank_inner<2>(q, inner, stream)); break;
-        case 3: GQ_CUDA(low_rank_inner<3>(q, inner, stream)); break;
-        default: GQ_CUDA(low_rank_inner<4>(q, inner, stream));
-    }
-    GQ_LAUNCHED();
+    int rc;
+    if (tiles > 1)
+        rc = cut.ranks == 2 ? low_rank_inner<low_rank_inner_chunk_kernel<32>>(q, inner, InnerShape<32>::SMEM, stream) : low_rank_inner<low_rank_inner_chunk_kernel<64>>(q, inner, InnerShape<64>::SMEM, stream);
+    else
+        rc = cut.ranks == 1 ? low_rank_inner<low_rank_inner_kernel<1>>(q, inner, 0, stream) : cut.ranks == 2 ? low_rank_inner<low_rank_inner_kernel<2>>(q, inner, 0, stream)
+             : cut.ranks == 3 ? low_rank_inner<low_rank_inner_kernel<3>>(q, inner, 0, stream) : low_rank_inner<low_rank_inner_kernel<4>>(q, inner, 0, stream);
+    if (rc) return rc;
     switch (q.ranks) {
         case 16: return low_rank_outer<1>(q, stream);
         case 32: return low_rank_outer<2>(q, stream);
