@@ -206,13 +206,13 @@ __global__ void __launch_bounds__(LR_THREADS) low_rank_inner_chunk_kernel(const 
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ RowGroups groups;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane % 4, rw = warp % 4, cw = warp / 4;
-    const int row0 = blockIdx.y * LR_ROWS, blocks = p.K / 64, per_shard = (p.rank + 15) / 16, tiles = p.n_shards * per_shard, tile0 = blockIdx.z * (RANKS / 16);
+    const int row0 = blockIdx.y * LR_ROWS, blocks = p.K / 64, per_shard = (p.rank + 15) / 16, tiles = p.n_shards * per_shard, tile0 = blockIdx.z / p.group_blocks * (RANKS / 16);
     const int k0 = (int)((int64_t)blockIdx.x * blocks / p.parts), k1 = (int)((int64_t)(blockIdx.x + 1) * blocks / p.parts);
     pdl_wait();
     pdl_trigger();
     group_rows(p, row0, groups);
     float(*red)[Shape::RED] = (float(*)[Shape::RED])smem;
-    for (int s = 0; s < groups.groups; ++s) {
+    for (int s = blockIdx.z % p.group_blocks; s < groups.groups; s += p.group_blocks) {
         const int id = groups.id[s], at = groups.start[s], count = groups.start[s + 1] - at;
         if (id < 0) continue;
         // 16 bytes of a row or rank at a time: 8 threads to a row; rows and ranks that are not there are read as the last

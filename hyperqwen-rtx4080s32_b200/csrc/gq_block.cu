@@ -63,29 +63,33 @@ static int check_low_rank(const gq_low_rank_args *p, int64_t *n_total) {
 }
 static int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 static int ranks_of(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
-// How the inner products are cut: ranks of a block in sixteens (as many as leave every SM a block), blocks for a tile's adapters, parts of K (256 at least, a cluster of sixteen at most).
-// m1 qkv of rank 16: three blocks of one sixteen in 16 parts 2.9 us, one of three 4.6.
+// How the inner products are cut: sixteens of ranks to a block, blocks that share a tile's adapters, parts of K (256 at least; the blocks of a cluster), blocks for all ranks.
+// Clusters are powers of two, of sixteen only while there are few: thirteen parts of 2,051 rows beside gate_up took 8 us more than eight, sixteen for each of seven adapters of
+// rank 32 beside qkv 4 us more than eight and fewer ranks to a block; one row beside qkv is 0.3 us faster with sixteen.
 struct LowRankCut {
     int ranks, groups, parts, turns;
 };
 static LowRankCut low_rank_cut(const gq_low_rank_args *p) {
     const int64_t tiles = (p->M + LR_ROWS - 1) / LR_ROWS;
-    const int sixteens = p->n_shards * ((p->rank + 15) / 16), most = (int)std::min<int64_t>(16, p->K / 256);
+    const int sixteens = p->n_shards * ((p->rank + 15) / 16);
     LowRankCut c{};
-    if (tiles > 1) {             // chunks: 32 or 64 ranks to a block, three blocks to an SM
+    int64_t most;
+    if (tiles > 1) {             // chunks: 32 or 64 ranks to a block, three blocks to an SM; two for a tile in which requests meet
         c.ranks = sixteens <= 2 ? 2 : 4;
-        c.groups = 1;
+        c.groups = p->n_adapters > 1 ? 2 : 1;
         c.turns = (sixteens + c.ranks - 1) / c.ranks;
-        c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, 444 / (c.turns * tiles)));
-        return c;
+        most = std::min<int64_t>(16, 444 / (c.turns * tiles));
+    } else {                     // decode: every adapter a block of its own, as many ranks to it as leave the GPU full
+        c.groups = (int)std::min<int64_t>(std::min<int64_t>(p->M, LR_ROWS), p->n_adapters);
+        for (int n = 4; n >= 1; --n) {
+            c.turns = (sixteens + n - 1) / n;
+            c.ranks = (sixteens + c.turns - 1) / c.turns;
+            if (c.turns * c.groups * 8 >= 148) break;
+        }
+        most = c.turns * c.groups * 8 < 74 ? 16 : std::min<int64_t>(8, 296 / (c.turns * c.groups));
     }
-    c.groups = (int)std::min<int64_t>(std::min<int64_t>(p->M, LR_ROWS), p->n_adapters);
-    for (int n = 4; n >= 1; --n) {
-        c.turns = (sixteens + n - 1) / n;
-        c.ranks = (sixteens + c.turns - 1) / c.turns;
-        if (c.turns * c.groups * most >= 148) break;
-    }
-    c.parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, 296 / (c.turns * c.groups)));
+    most = std::min<int64_t>(most, p->K / 256);
+    for (c.parts = 1; c.parts * 2 <= most; c.parts *= 2) {}
     return c;
 }
 extern "C" int64_t gq_low_rank_workspace_bytes(const gq_low_rank_args *p) {
