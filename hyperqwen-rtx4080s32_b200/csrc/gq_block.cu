@@ -20,8 +20,14 @@ cudaError_t gq::block_status_clear(cudaStream_t s) {
 }
 
 static bool aligned(const void *p, int bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+// the word's address on the current device, asked for once
 static int status_word(int **p) {
+    static std::atomic<int *> known[64];
+    int dev = 0;
+    GQ_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && (*p = known[dev].load(std::memory_order_acquire))) return GQ_OK;
     GQ_CUDA(cudaGetSymbolAddress((void **)p, g_block_status));
+    if (dev < 64) known[dev].store(*p, std::memory_order_release);
     return GQ_OK;
 }
 

@@ -245,3 +245,78 @@ def test_a_gradient_is_refused():
         adapters.call(s)
     with torch.no_grad():
         adapters.check(adapters.call(s), {**s, "x": s["x"].detach()})
+
+
+def test_calls_of_nothing():
+    s = adapters.make(3, 256, (24, 8), 8, 2)
+    none = {**s, "x": s["x"][:0], "base": s["base"][:0], "ids": s["ids"][:0]}
+    assert adapters.call(none).shape == (0, 32)
+    assert adapters.call({**s, "base": s["base"][:, :0], "b": s["b"][:, :0], "n_outs": [0, 0]}).shape == (3, 0)
+    inv, _ = ops.rotary_frequencies(16)
+    cache = PagedKVCache(2, 16, 1, 64)
+    qkv = adapters.bf16(0, 4 * 64, seed=1)
+    at = torch.zeros(0, dtype=torch.int64, device="cuda")
+    assert ops.qk_norm_rope(qkv, at, inv, 2, 1, 64)[1].shape == (0, 1, 64)
+    assert ops.qk_norm_rope_store(qkv, at, inv, 2, 1, 64, cache.k, cache.v, at).shape == (0, 2, 64)
+    table, lens = torch.zeros(0, 4, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int32, device="cuda")
+    assert ops.paged_attention(adapters.bf16(0, 2, 64, seed=1), cache.k, cache.v, table, lens).shape == (0, 2, 64)
+    q = adapters.bf16(3, 2, 64, seed=2)
+    no_keys = ops.paged_attention(q, cache.k, cache.v, torch.zeros(3, 0, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda"))
+    assert bool((no_keys == 0).all()) and ops.device_status() == 0
+    for pages, width in ((cache.k[:0], 4), (cache.k, 0)):          # keys, but no cache or no table
+        got = ops.paged_attention(q, pages, pages, torch.zeros(3, width, dtype=torch.int32, device="cuda"), torch.tensor([0, 5, 0], dtype=torch.int32, device="cuda"))
+        assert bool(got[1].isnan().all()) and bool((got[[0, 2]] == 0).all())
+        assert ops.device_status() == 2
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    """In a process of its own: every operator's first call is inside a capture; replayed, it gives what the next, eager one gives."""
+    import os
+    import subprocess
+    import sys
+
+    program = """
+import torch
+import test_gpu_adapters as adapters, test_gpu_paged as paged
+from hyperqwen_rtx4080s32_b200 import ops
+few, many = adapters.make(3, 512, (64, 32), 16, 2), adapters.make(200, 512, (64, 32), 16, 2)
+p, more, _ = paged.make([300, 40], [1, 1], 8, 2, 128, 16)
+inv, _ = ops.rotary_frequencies(64)
+qkv, pos = adapters.bf16(6, 8 * 64, seed=3), torch.arange(6, device="cuda")
+calls = [lambda: adapters.call(few), lambda: adapters.call(many), lambda: ops.paged_attention(**p), lambda: ops.qk_norm_rope(qkv, pos, inv, 4, 2, 64)[0]]
+torch.cuda.synchronize()
+for call in calls:
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=side):
+        out = call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, call())
+print("captured")
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([here, os.path.dirname(here), os.environ.get("PYTHONPATH", "")]))
+    run = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, env=env, timeout=300)
+    assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]
+
+
+def test_memory_that_is_written_and_read_is_refused():
+    s = adapters.make(4, 256, (256,), 8, 1)
+    both = torch.zeros(6, 256, dtype=torch.bfloat16, device="cuda")
+    for base, out in ((both[:4], both[1:5]), (both[1:5], both[:4])):
+        with pytest.raises(ops.GqError, match="base itself"):
+            adapters.call({**s, "base": base}, out=out)
+    for name in ("x", "b"):
+        with pytest.raises(ops.GqError, match="input other than base"):
+            adapters.call(s, out=s[name].view(-1)[:1024].view(4, 256))
+    p, more, _ = paged.make([20, 30], [1, 1], 4, 2, 64, 16)
+    for out in (p["q"], p["v_pages"].transpose(1, 2).view(-1)[:512].view(2, 4, 64)):
+        with pytest.raises(ops.GqError, match="shares no memory"):
+            ops.paged_attention(**p, out=out)
+    cache = PagedKVCache(2, 16, 2, 64)
+    inv, _ = ops.rotary_frequencies(64)
+    pos = torch.zeros(2, dtype=torch.int64, device="cuda")
+    with pytest.raises(ops.GqError, match="share no memory"):
+        ops.qk_norm_rope_store(cache.v.transpose(1, 2).view(-1)[:1024].view(2, 512), pos, inv, 4, 2, 64, cache.k, cache.v, pos)
+    with pytest.raises(ops.GqError, match="CUDA"):
+        adapters.call({**s, "scales": s["scales"].cpu()})
