@@ -1,10 +1,16 @@
 // Low-rank adapters beside a shared projection: out = base + scale * B (A x) for each row's own adapter.
 //
-// Rows are taken in tiles of 64; a block sorts its tile's rows by adapter, and every adapter that occurs multiplies its own rows only, so no row's sums ever hold another adapter's numbers and
-// rows of one adapter need not stand together.  Two launches: the inner products A x, K split over the blocks of a cluster, left in the workspace, and the outer products B (A x) with the addition.
-// Both read bf16 operands from global memory straight into the fragments of mma.sync m16n8k16: any order of k serves as long as both operands have the same, so a lane takes 8
-// neighbours (16 bytes) where the instruction names scattered ones.  Bound by bytes: in decode those of the adapters (latency below a few MB), in prefill those of base and out;
-// the ranks are too small for tcgen05's 128 rows to be filled.
+// Two launches: the inner products A x (K split over the blocks of a cluster, their sums left in the workspace as two bf16 parts) and the outer products B (A x) with the addition.  No row's sums
+// ever hold another adapter's numbers, and rows of one adapter need not stand together: the inner products sort a tile's 64 rows by adapter and multiply each adapter's own; the outer ones multiply
+// a tile of 16 rows (or 4) once for every adapter in it and keep that one's rows.  In decode both read bf16 operands from global memory straight into the fragments of mma.sync m16n8k16: any order
+// of k serves as long as both operands have the same, so a lane takes 8 neighbours (16 bytes) where the instruction names scattered ones.  In chunks of prompts both go through shared memory.
+// Bound by bytes, in decode those of the adapters (below a few MB latency is all), in chunks those of base and out.
+//
+// Measured (graph of calls): one row beside qkv, rank 16, 6.2 us (two launches, two rounds of memory, a cluster's sums); 27 rows of 8 adapters of rank 32 beside gate_up 11.8 (18 MB, floor 2.8); 64 rows of 16
+// of rank 64 beside down 24 (49 MB, floor 7.6): what the inner blocks ask for comes in three rounds of 2 us, and a cluster waits for its last; 2,051 rows of rank 16 beside gate_up 84 (312 MB, floor 48), of
+// rank 128 beside qkv 96 (floor 16): there the inner products run at 160 TFLOP/s, and mma.sync of 64 x 64 tiles is what bounds them.
+// Tried: sums of the parts by the outer blocks (m64 7 us less in the inner, 8 more in the outer kernel); decode through the chunk kernels (m64 24 to 36); the base straight to registers with two to
+// four tiles ahead (m2051 outer 86 to 110); 64 rows x 256 or 32 x 512 columns in shared memory with two blocks to an SM (79 and 77 against 67 with four blocks of 32 x 256).
 #pragma once
 #include "gq_bf16.cuh"
 

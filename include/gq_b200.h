@@ -362,7 +362,7 @@ int gq_read_status(const void *workspace_dev, int64_t workspace_bytes, void *str
 
 /* The largest device status code any kernel of this library has reported on the current device since the word was
  * last cleared (synchronises the stream; clear != 0 resets it after reading): 0, or a positive GQ_DEV_* code (those above; 2 also
- * for an id outside the table given to gq_dequant_rows).  Every
+ * for an id outside the table given to gq_dequant_rows, and for what the operators beside the layers find outside a bank, a cache or a page table).  Every
  * kernel that sets a workspace's status word sets this one too, so a caller that frees its workspace after each call,
  * or uses the entry point without a workspace argument, still sees a timeout.  Meant to be called between steps.
  * Reference: none (the reference's kernels have no waits that can run out). */
