@@ -147,7 +147,7 @@ extern "C" int gq_low_rank_add(const gq_low_rank_args *p, void *stream) {
     if (const int rc = check_low_rank(p, &n)) return rc;
     if (p->M == 0 || n == 0) return GQ_OK;
     if (!p->base || !p->x || !p->a || !p->b || !p->scales || !p->ids || !p->out || (p->ids_bytes != 4 && p->ids_bytes != 8)) return GQ_ERR_ARG;
-    if (!aligned(p->x, 16) || !aligned(p->a, 16) || !aligned(p->b, 16) || p->ldx % 8 || p->ldx < p->K || p->ld_base < n || p->ld_out < n) return GQ_ERR_ARG;
+    if (!aligned(p->x, 16) || !aligned(p->a, 16) || !aligned(p->b, 16) || p->ldx % 8 || p->ldx < p->K || p->ld_base < n || p->ld_out < n || (p->out == p->base && p->M > 1 && p->ld_out != p->ld_base)) return GQ_ERR_ARG;
     const int64_t bytes = gq_low_rank_workspace_bytes(p);
     if (p->workspace_bytes < bytes || !p->workspace || !aligned(p->workspace, 256)) return GQ_ERR_WORKSPACE;
     int *status;

@@ -118,15 +118,16 @@ class LoadedModel:
             if name.startswith("layers."):
                 lin.quant_method.add_adapters(lin, n_adapters, rank)
 
-    def attention(self, layer: int, *, head_dim: int | None = None, **rotary):
+    def attention(self, layer: int, *, head_dim: int | None = None, interleaved: bool = False, **rotary):
         """The attention half of a block (attention.GGUFAttention) from its qkv_proj, o_proj and head norms.  What the file says about heads, rotation and eps is
-        taken from it; `head_dim` and the arguments of ops.rotary_frequencies (rotary_dim, base, scaling, factor, original_context) go before."""
+        taken from it; `head_dim` and the arguments of ops.rotary_frequencies (rotary_dim, base, scaling, factor, original_context) go before.  A token has one
+        position (text); `interleaved` where the architecture turns neighbours, which the file does not say."""
         from . import ops
         from .attention import GGUFAttention
 
         def norm(which):
             t = self.other.get(f"model.language_model.layers.{layer}.self_attn.{which}_norm.weight")
-            return None if t is None else torch.from_numpy(np.array(t.data, copy=True)).to(device=device, dtype=torch.bfloat16)
+            return None if t is None else _values(t).to(device=device, dtype=torch.bfloat16)
 
         qkv, o, meta = self.linears[f"layers.{layer}.self_attn.qkv_proj"], self.linears[f"layers.{layer}.self_attn.o_proj"], self.meta
         device = next(iter(qkv.gguf_groups.values()))[0].device
@@ -137,7 +138,8 @@ class LoadedModel:
         known = {"rotary_dim": meta.get("rope.dimension_count", head_dim), "base": meta.get("rope.freq_base", 10000.0), "scaling": meta.get("rope.scaling.type"),
                  "factor": meta.get("rope.scaling.factor", 1.0), "original_context": meta.get("rope.scaling.original_context_length")}
         inv_freq, amplitude = ops.rotary_frequencies(**{**known, **rotary}, device=device)
-        return GGUFAttention(qkv, o, int(head_dim), inv_freq, amplitude=amplitude, q_norm=q_norm, k_norm=k_norm, eps=float(meta.get("attention.layer_norm_rms_epsilon", 1e-6)))
+        return GGUFAttention(qkv, o, int(head_dim), inv_freq, amplitude=amplitude, q_norm=q_norm, k_norm=k_norm, eps=float(meta.get("attention.layer_norm_rms_epsilon", 1e-6)),
+                             interleaved=interleaved)
 
 
 def load_gguf(path: str, device="cuda", strict: bool = True) -> LoadedModel:
@@ -186,6 +188,12 @@ def load_gguf(path: str, device="cuda", strict: bool = True) -> LoadedModel:
     return out
 
 
+def _values(t: GGUFTensor) -> torch.Tensor:
+    """A copy of an F32, F16 or BF16 tensor (the reader gives the last as bytes)."""
+    data = torch.from_numpy(np.array(t.data, copy=True))
+    return (data.view(torch.bfloat16) if t.ggml_type == 30 else data).reshape(t.shape)
+
+
 def _metadata(reader) -> dict[str, object]:
     """The file's single numbers and texts; "qwen35.rope.freq_base" is listed as "rope.freq_base" too."""
     out: dict[str, object] = {}
@@ -213,9 +221,7 @@ def load_adapter(path: str, model: LoadedModel, slot: int, scale: float = 1.0) -
         name, _, which = t.name.rpartition(".lora_")
         if which not in ("a", "b") or t.ggml_type not in (0, 1, 30):
             raise ValueError(f"{t.name}: not one of a pair of matrices in F32, F16 or BF16")
-        data = np.array(t.data, copy=True)
-        value = torch.from_numpy(data) if t.ggml_type != 30 else torch.from_numpy(data).view(torch.bfloat16)
-        parts.setdefault(name, {})[which] = value.reshape(t.shape)
+        parts.setdefault(name, {})[which] = _values(t)
     found = []
     for name, pair in parts.items():
         mapped = map_tensor_name(name)

@@ -187,13 +187,15 @@ def test_a_block_and_its_adapter_from_files(tmp_path):
     r, mats = 6, []
     for n, (no, kk) in pairs.items():
         mats += [(f"blk.3.{n}.weight.lora_a", rng.standard_normal((r, kk)).astype(np.float32) / 20, None), (f"blk.3.{n}.weight.lora_b", rng.standard_normal((no, r)).astype(np.float16), None)]
+    half = torch.from_numpy(mats[-1][1]).to(torch.bfloat16)                # one of them as BF16, which the file holds as bytes
+    mats[-1] = (mats[-1][0], half.view(torch.uint8).numpy(), 30)
     _write(extra, mats, general__type="adapter", adapter__type="lora", adapter__lora__alpha=12.0)
     with pytest.raises(ValueError, match="add_adapters"):
         loader.load_adapter(extra, model, 0)
     model.add_adapters(2, 8)
     assert loader.load_adapter(extra, model, 1, scale=0.5) == ["layers.3.mlp.gate_up_proj", "layers.3.self_attn.o_proj", "layers.3.self_attn.qkv_proj"]
     x = synth.activations(5, k, device="cuda")
-    raw = {n: a for n, a, _ in mats}
+    raw = {n: a if t is None else half.float().numpy() for n, a, t in mats}
     for key, shards in (("layers.3.self_attn.qkv_proj", (("attn_q", 0, 1024), ("attn_k", 1024, 128), ("attn_v", 1152, 128))), ("layers.3.mlp.gate_up_proj", (("ffn_gate", 0, 768), ("ffn_up", 768, 768)))):
         lin = model.linears[key]
         got, base = lin(x, adapters=torch.tensor([1, 0, -1, 1, 1], device="cuda")), lin(x)
