@@ -278,7 +278,8 @@ PyObject *dequantize_rows(py::handle rawh, int64_t type, py::handle idsh, bool b
 }
 
 // ---- the operators beside the quantized layers ---------------------------------------------------------
-// Arguments are checked here in full (shapes and types first, then devices and memory), then handed to the C ABI on the current stream of their device.
+// Arguments are checked here in full (shapes and types first, then devices and memory), then handed to the C ABI on the current stream of their device.  ops.py comes here directly on a
+// plain thread only; inside a mode, a tracer or a transform it calls the registered op, which the dispatcher brings here.
 
 [[noreturn]] void refuse(const char *op, const std::string &why) {
     PyErr_SetString(g_error, (std::string(op) + ": " + why).c_str());
@@ -308,7 +309,6 @@ class Checked {
             if (all_[i]->get_device() != all_[0]->get_device()) refuse(op_, "takes tensors of one device");
             if (all_[i]->requires_grad() && at::GradMode::is_enabled()) refuse(op_, "has no backward pass: call it under torch.no_grad(), or detach its inputs");
         }
-        if (!plain_thread()) refuse(op_, "was called inside a torch mode or function transform");
     }
   private:
     const char *op_;
@@ -546,6 +546,7 @@ PYBIND11_MODULE(_gq_torch, m) {
     m.def("dequantize_rows", [](py::handle raw, int64_t type, py::handle ids, bool bf16) {
         return py::reinterpret_steal<py::object>(dequantize_rows(raw, type, ids, bf16));
     });
+    m.def("plain_thread", &plain_thread);
     m.def("low_rank_add", &low_rank_add);
     m.def("qk_norm_rope", &qk_norm_rope);
     m.def("paged_attention", &paged_attention);

@@ -573,6 +573,19 @@ class NativeRun:
 MAX_RANK = 128
 
 
+def _aside() -> bool:
+    """Whether a mode, a tracer or a transform has to see the call: it is then made through torch.ops, as the layers' is."""
+    return torch.compiler.is_compiling() or not native().plain_thread()
+
+
+def _into(op: str, out: torch.Tensor | None, result: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return result
+    if out.shape != result.shape or out.dtype != result.dtype or out.device != result.device:      # copy_ would broadcast and convert
+        raise GqError(f"{op}: out is {result.dtype} {list(result.shape)} on {result.device}, got {out.dtype} {list(out.shape)} on {out.device}")
+    return out.copy_(result)
+
+
 def low_rank_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, ids: torch.Tensor,
                  n_outs: Sequence[int], *, out: torch.Tensor | None = None) -> torch.Tensor:
     """Low-rank adapters of many requests beside one (merged) layer: base [M, N] plus, for every row m with an adapter i = ids[m],
@@ -583,9 +596,8 @@ def low_rank_add(base: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.
     ids[m] = -1: the row has no adapter and is base's.  Any other id outside the bank makes its row NaN and device_status 2.  `out` may be base
     (in place); it is new memory if left out.  Sums in 32 bits, one rounding; a row's sums hold nothing of other rows' adapters."""
     n_outs = [int(n) for n in n_outs]
-    if torch.compiler.is_compiling():
-        sums = torch.ops.gq_b200.low_rank_add(base, x, a, b, scales, ids, n_outs)
-        return sums if out is None else out.copy_(sums)
+    if _aside():
+        return _into("low_rank_add", out, torch.ops.gq_b200.low_rank_add(base, x, a, b, scales, ids, n_outs))
     return native().low_rank_add(base, x, a, b, scales, ids, n_outs, out)
 
 
@@ -622,7 +634,7 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Ten
     The first 2 * len(inv_freq) dimensions of a head turn, as pairs half of them apart or, `interleaved`, side by side; inv_freq (float64) and amplitude as
     rotary_frequencies makes them; angles are reduced in 64 bits.  positions int32 or int64 [T].  `gated`: every query head is followed
     by an output gate of head_dim values, which stays where it is (paged_attention takes it)."""
-    if torch.compiler.is_compiling():
+    if _aside():
         return torch.ops.gq_b200.qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated)
     return native().qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated, None, None, None)
 
@@ -635,7 +647,7 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
 
     k_pages, v_pages bf16 [pages, rows, n_kv_heads, head_dim] by strides; token t goes to slot slots[t] (int32 or int64) = page * rows + row.  A negative
     slot stores nothing (padding); one beyond the cache stores nothing and makes device_status 2.  Of two tokens with one slot either may be kept."""
-    if torch.compiler.is_compiling():
+    if _aside():
         return torch.ops.gq_b200.qk_norm_rope_store(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated,
                                                     k_pages, v_pages, slots)
     return native().qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated,
@@ -654,9 +666,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     scale: head_dim ** -0.5 if left out.  gate (q's shape, any strides over tokens and heads): the result is multiplied by sigmoid(gate).
     A page outside the cache or a length beyond the table: NaN in the rows that see it, and device_status 2.  Probabilities, sums and the join of the
     cache's parts in 32 bits, one rounding; the order of the sums does not depend on timing."""
-    if torch.compiler.is_compiling():
-        o = torch.ops.gq_b200.paged_attention(q, k_pages, v_pages, page_table, lens, q_starts, scale, gate, out)
-        return o if out is None else out.copy_(o)
+    if _aside():
+        return _into("paged_attention", out, torch.ops.gq_b200.paged_attention(q, k_pages, v_pages, page_table, lens, q_starts, scale, gate, out))
     return native().paged_attention(q, k_pages, v_pages, page_table, lens, q_starts, scale, gate, out)
 
 

@@ -322,3 +322,44 @@ def test_memory_that_is_written_and_read_is_refused():
         ops.qk_norm_rope_store(cache.v.transpose(1, 2).view(-1)[:1024].view(2, 512), pos, inv, 4, 2, 64, cache.k, cache.v, pos)
     with pytest.raises(ops.GqError, match="CUDA"):
         adapters.call({**s, "scales": s["scales"].cpu()})
+
+
+def test_modes_and_tracers_see_the_calls():
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Names(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.seen = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    s = adapters.make(5, 256, (24, 8), 8, 2)
+    p, _, _ = paged.make([30, 20], [1, 1], 4, 2, 64, 16)
+    inv, _ = ops.rotary_frequencies(64)
+    qkv, pos = adapters.bf16(6, 8 * 64, seed=3), torch.arange(6, device="cuda")
+    cache = PagedKVCache(2, 16, 2, 64)
+    calls = [lambda: adapters.call(s), lambda: adapters.call({**s, "base": s["base"].clone()}, out=torch.empty_like(s["base"])), lambda: ops.paged_attention(**p),
+             lambda: ops.paged_attention(**p, out=torch.empty_like(p["q"])), lambda: ops.qk_norm_rope(qkv, pos, inv, 4, 2, 64)[1], lambda: ops.qk_norm_rope_store(qkv, pos, inv, 4, 2, 64, cache.k, cache.v, pos)]
+    for call in calls:
+        want = call()
+        with torch.device("cuda"):
+            assert torch.equal(call(), want)
+        with torch.autocast("cuda", dtype=torch.bfloat16), torch.inference_mode():
+            assert torch.equal(call(), want)
+        with Names() as names:
+            got = call()
+        assert torch.equal(got, want) and any("gq_b200" in n for n in names.seen)
+    traced = torch.jit.trace(lambda q: ops.paged_attention(q, *[p[n] for n in ("k_pages", "v_pages", "page_table", "lens")]), (p["q"],), check_trace=False)
+    other = p["q"] * 0.5
+    assert torch.equal(traced(other), ops.paged_attention(**{**p, "q": other}))
+    wrong = [lambda: adapters.call(s, out=torch.empty(2, *s["base"].shape, dtype=torch.bfloat16, device="cuda")), lambda: adapters.call(s, out=torch.empty_like(s["base"]).float()),
+             lambda: adapters.call(s, out=torch.empty_like(s["base"], device="cpu")), lambda: adapters.call({**s, "x": s["x"].clone().requires_grad_()}),
+             lambda: ops.paged_attention(**{**p, "q": p["q"].clone().requires_grad_()}), lambda: ops.paged_attention(**p, out=torch.empty(2, *p["q"].shape, dtype=torch.bfloat16, device="cuda"))]
+    for call in wrong:
+        with pytest.raises(ops.GqError):
+            call()
+        with torch.device("cuda"), Names(), pytest.raises(ops.GqError):
+            call()
