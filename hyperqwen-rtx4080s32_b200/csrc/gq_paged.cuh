@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(32 * KG * DG) paged_attention_kernel(const __g
 }
 
 // The segments that several blocks worked on: block c joins the one that starts in block c's range and ends behind it, each row by as many warps as there are, four parts of
-// a warp in flight.  All but the parts themselves is found before the wait for the blocks that write them.
+// a warp in flight.  All but the parts themselves is found before the wait for the kernel that writes them.
 constexpr int JOIN_WARPS = 16;
 template <int D, int ROWS, int UNIT>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) join_parts_kernel(const __grid_constant__ PagedParams p) {
@@ -586,20 +586,25 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_parts_kernel(const __gri
     __shared__ float2 box_stats[JOIN_WARPS];
     const gq_attention_args &a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
-    int64_t end;            // the block of the segment's last unit
+    int64_t end = 0;        // the block of the segment's last unit
+    bool joins;
     Cursor c;
     {
         const Line line = count_units<ROWS, UNIT>(p, lane);
         const Cut cut = cut_line(p, line.total);
         const int64_t w0 = cut.start(blockIdx.x), w1 = cut.start(blockIdx.x + 1);
-        if (w0 == w1) return;
-        locate<ROWS, UNIT>(p, line, w1 - 1, lane, c);
-        const int64_t first = w1 - 1 - c.unit;
-        if (first < w0 || first + c.units == w1) return;
-        end = min(cut.block_of(first + c.units - 1), cut.blocks - 1);
+        joins = w0 != w1;
+        if (joins) {
+            locate<ROWS, UNIT>(p, line, w1 - 1, lane, c);
+            const int64_t first = w1 - 1 - c.unit;
+            joins = first >= w0 && first + c.units != w1;
+            if (joins) end = min(cut.block_of(first + c.units - 1), cut.blocks - 1);
+        }
     }
-    const int rows = min(ROWS, c.v.n * p.group - c.tile * ROWS), sets = max(JOIN_WARPS / rows, 1), set = warp / min(rows, JOIN_WARPS);
+    // Blocks without a segment wait too: what is launched behind this kernel waits for this one alone, so it has to end behind the one in front.
     pdl_wait();
+    if (!joins) return;
+    const int rows = min(ROWS, c.v.n * p.group - c.tile * ROWS), sets = max(JOIN_WARPS / rows, 1), set = warp / min(rows, JOIN_WARPS);
     for (int r0 = 0; r0 < rows; r0 += JOIN_WARPS) {
         const int r = r0 + (rows < JOIN_WARPS ? warp % rows : warp);
         const bool mine = r < rows && set < sets;
