@@ -408,7 +408,8 @@ void take_pages(const Checked &c, const at::Tensor &t, int64_t kv_heads, int64_t
     }
 }
 
-py::object qk_norm_rope(const at::Tensor &qkv0, const at::Tensor &positions0, const at::Tensor &inv_freq, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+// Both forms: with a cache given (all of k_pages, v_pages, slots) keys and values go there and q comes back, without one q and k
+py::object norm_heads(const at::Tensor &qkv0, const at::Tensor &positions0, const at::Tensor &inv_freq, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
                         c10::optional<at::Tensor> q_norm, c10::optional<at::Tensor> k_norm, double eps, double amplitude, bool interleaved, bool gated,
                         c10::optional<at::Tensor> k_pages, c10::optional<at::Tensor> v_pages, c10::optional<at::Tensor> slots0) {
     const bool store = k_pages.has_value();
@@ -468,6 +469,17 @@ py::object qk_norm_rope(const at::Tensor &qkv0, const at::Tensor &positions0, co
     }
     status.check();
     return store ? py::cast(q) : py::object(py::make_tuple(q, k));
+}
+
+py::object qk_norm_rope(const at::Tensor &qkv, const at::Tensor &positions, const at::Tensor &inv_freq, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, c10::optional<at::Tensor> q_norm,
+                        c10::optional<at::Tensor> k_norm, double eps, double amplitude, bool interleaved, bool gated) {
+    return norm_heads(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated, c10::nullopt, c10::nullopt, c10::nullopt);
+}
+py::object qk_norm_rope_store(const at::Tensor &qkv, const at::Tensor &positions, const at::Tensor &inv_freq, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, c10::optional<at::Tensor> q_norm,
+                              c10::optional<at::Tensor> k_norm, double eps, double amplitude, bool interleaved, bool gated, c10::optional<at::Tensor> k_pages, c10::optional<at::Tensor> v_pages,
+                              c10::optional<at::Tensor> slots) {
+    Checked("qk_norm_rope_store").need(k_pages.has_value() && v_pages.has_value() && slots.has_value(), "k_pages, v_pages and slots are all given");
+    return norm_heads(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated, k_pages, v_pages, slots);
 }
 
 at::Tensor paged_attention(const at::Tensor &q0, const at::Tensor &k_pages, const at::Tensor &v_pages, const at::Tensor &table0, const at::Tensor &lens0,
@@ -549,6 +561,7 @@ PYBIND11_MODULE(_gq_torch, m) {
     m.def("plain_thread", &plain_thread);
     m.def("low_rank_add", &low_rank_add);
     m.def("qk_norm_rope", &qk_norm_rope);
+    m.def("qk_norm_rope_store", &qk_norm_rope_store);
     m.def("paged_attention", &paged_attention);
     py::class_<Run>(m, "Run")
         .def(py::init<at::Tensor, std::vector<at::Tensor>, std::vector<int64_t>, std::vector<int64_t>, std::vector<int64_t>, int64_t, std::vector<int64_t>,

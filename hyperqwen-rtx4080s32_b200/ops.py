@@ -636,7 +636,7 @@ def qk_norm_rope(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Ten
     by an output gate of head_dim values, which stays where it is (paged_attention takes it)."""
     if _aside():
         return torch.ops.gq_b200.qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated)
-    return native().qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated, None, None, None)
+    return native().qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated)
 
 
 def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
@@ -650,8 +650,8 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
     if _aside():
         return torch.ops.gq_b200.qk_norm_rope_store(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated,
                                                     k_pages, v_pages, slots)
-    return native().qk_norm_rope(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated,
-                                 k_pages, v_pages, slots)
+    return native().qk_norm_rope_store(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated,
+                                       k_pages, v_pages, slots)
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, *,
@@ -693,8 +693,8 @@ _OP_LIB.define("qk_norm_rope_store(Tensor qkv, Tensor positions, Tensor inv_freq
                "float eps, float amplitude, bool interleaved, bool gated, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor slots) -> Tensor")
 _OP_LIB.define("paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor lens, Tensor? q_starts, float? scale, Tensor? gate, Tensor? kept) -> Tensor")
 _OP_LIB.impl("low_rank_add", lambda *args: native().low_rank_add(*args, None), "CUDA")
-_OP_LIB.impl("qk_norm_rope", lambda *args: native().qk_norm_rope(*args, None, None, None), "CUDA")
-_OP_LIB.impl("qk_norm_rope_store", lambda *args: native().qk_norm_rope(*args), "CUDA")
+_OP_LIB.impl("qk_norm_rope", lambda *args: native().qk_norm_rope(*args), "CUDA")
+_OP_LIB.impl("qk_norm_rope_store", lambda *args: native().qk_norm_rope_store(*args), "CUDA")
 _OP_LIB.impl("paged_attention", lambda *args: native().paged_attention(*args[:-1], None if args[-1] is None else args[-1].clone(memory_format=torch.contiguous_format)), "CUDA")
 torch.library.register_fake("gq_b200::low_rank_add")(lambda base, *_: base.new_empty(base.shape))
 torch.library.register_fake("gq_b200::qk_norm_rope")(lambda qkv, positions, inv_freq, hq, hk, d, *_: (qkv.new_empty((qkv.shape[0], hq, d)), qkv.new_empty((qkv.shape[0], hk, d))))

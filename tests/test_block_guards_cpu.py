@@ -3,7 +3,13 @@ import os
 import re
 
 import pytest
+import torch
 
+from hyperqwen_rtx4080s32_b200 import ops
+
+import test_block_ops_cpu as refusals
+
+E, h = ops.GqError, refusals.h
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "hyperqwen-rtx4080s32_b200", "csrc")
 
 
@@ -32,3 +38,9 @@ def test_every_kernel_waits_for_the_one_in_front_on_every_path(header):
         ahead = body[:body.index("pdl_wait();")]
         assert "return" not in ahead, f"{name} returns before it has waited"
         assert ahead.count("{") - ahead.count("}") == 1 and ahead.rstrip()[-1] in ";}", f"{name} waits in a branch"
+
+
+@pytest.mark.parametrize("missing", [("k_pages",), ("v_pages",), ("slots",), ("k_pages", "slots"), ("k_pages", "v_pages", "slots")], ids=str)
+def test_a_store_without_a_part_of_its_cache_is_refused(missing):
+    with pytest.raises(E, match="all given"):
+        refusals.heads(store=True, **{name: None for name in missing})
