@@ -345,16 +345,26 @@ class LowRankAdapters:
         self.b = torch.zeros((n_adapters, n, self.rank), dtype=torch.bfloat16, device=dev)
         self.scales = torch.zeros((n_adapters, len(self.order)), dtype=torch.float32, device=dev)
 
-    def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0, shard_id=None) -> None:
-        """The adapter of one shard (the only one, if shard_id is None): a [r, K], b [n_out, r] of any float type, its products times `scale`."""
+    def check_slot(self, slot: int) -> None:
+        if not 0 <= slot < self.a.shape[0]:
+            raise ops.GqError(f"no slot {slot} among {self.a.shape[0]}")
+
+    def check(self, slot: int, a: torch.Tensor, b: torch.Tensor, shard_id=None) -> int:
+        """Raises GqError where load would; the shard's place among the layer's."""
+        self.check_slot(slot)
         if shard_id is None and len(self.order) == 1:
             shard_id = self.order[0]
-        if shard_id not in self.order or not 0 <= slot < self.a.shape[0]:
-            raise ops.GqError(f"no shard {shard_id!r} among {self.order}, or no slot {slot} among {self.a.shape[0]}")
+        if shard_id not in self.order:
+            raise ops.GqError(f"no shard {shard_id!r} among {self.order}")
         j = self.order.index(shard_id)
-        r, first = a.shape[0], sum(self.n_outs[:j])
-        if a.dim() != 2 or b.dim() != 2 or a.shape[1] != self.k or b.shape[1] != r or b.shape[0] != self.n_outs[j] or not 1 <= r <= self.rank:
+        if a.dim() != 2 or b.dim() != 2 or a.shape[1] != self.k or b.shape != (self.n_outs[j], a.shape[0]) or not 1 <= a.shape[0] <= self.rank:
             raise ops.GqError(f"an adapter of this shard is [r, {self.k}] and [{self.n_outs[j]}, r] with r up to {self.rank}, got {tuple(a.shape)} and {tuple(b.shape)}")
+        return j
+
+    def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0, shard_id=None) -> None:
+        """The adapter of one shard (the only one, if shard_id is None): a [r, K], b [n_out, r] of any float type, its products times `scale`."""
+        j = self.check(slot, a, b, shard_id)
+        r, first = a.shape[0], sum(self.n_outs[:j])
         mine, rows = self.a[slot, j * self.rank:(j + 1) * self.rank], self.b[slot, first:first + self.n_outs[j]]
         mine[:r], mine[r:] = a.to(self.a), 0
         rows[:, :r], rows[:, r:] = b.to(self.b), 0
@@ -362,6 +372,7 @@ class LowRankAdapters:
 
     def clear(self, slot: int) -> None:
         """Empties a slot."""
+        self.check_slot(slot)
         self.scales[slot] = 0
         self.a[slot] = 0
         self.b[slot] = 0

@@ -209,7 +209,8 @@ def _metadata(reader) -> dict[str, object]:
 def load_adapter(path: str, model: LoadedModel, slot: int, scale: float = 1.0) -> list[str]:
     """Reads a GGUF adapter file (general.type "adapter", adapter.type "lora": a pair X.lora_a [r, K], X.lora_b [n_out, r] for every adapted weight X, and
     adapter.lora.alpha) into `slot` of the banks that model.add_adapters made, which is emptied first; its products count alpha / r * scale.
-    Returns the layers that have it.  A weight that is no linear layer of the model raises ValueError, before anything is changed."""
+    Returns the layers that have it.  Nothing is changed where the file does not fit: a weight that is no linear layer of the model raises ValueError, a slot or
+    matrices that are not a bank's GqError."""
     from gguf import GGUFReader
 
     reader = GGUFReader(path)
@@ -232,10 +233,13 @@ def load_adapter(path: str, model: LoadedModel, slot: int, scale: float = 1.0) -
         bank = getattr(lin, "gguf_adapters", None)
         if bank is None or pair["a"].shape[0] > bank.rank:
             raise ValueError(f"{name}: model.add_adapters(rank >= {pair['a'].shape[0]}) comes first")
+        bank.check(slot, pair["a"], pair["b"], mapped.shard_id)
         found.append((key, bank, pair, mapped.shard_id))
-    for lin in model.linears.values():
-        if getattr(lin, "gguf_adapters", None) is not None:
-            lin.gguf_adapters.clear(slot)
+    banks = [lin.gguf_adapters for lin in model.linears.values() if getattr(lin, "gguf_adapters", None) is not None]
+    for bank in banks:
+        bank.check_slot(slot)
+    for bank in banks:
+        bank.clear(slot)
     alpha = float(meta.get("adapter.lora.alpha", 0.0))
     for _, bank, pair, shard_id in found:
         r = pair["a"].shape[0]

@@ -2,10 +2,12 @@
 import os
 import re
 
+import numpy as np
 import pytest
 import torch
 
-from hyperqwen_rtx4080s32_b200 import ops
+from hyperqwen_rtx4080s32_b200 import loader, ops
+from hyperqwen_rtx4080s32_b200.linear import LowRankAdapters
 
 import test_block_ops_cpu as refusals
 
@@ -44,3 +46,78 @@ def test_every_kernel_waits_for_the_one_in_front_on_every_path(header):
 def test_a_store_without_a_part_of_its_cache_is_refused(missing):
     with pytest.raises(E, match="all given"):
         refusals.heads(store=True, **{name: None for name in missing})
+
+
+K = 256
+
+
+def write_gguf(path, tensors, arch="qwen35", **meta):
+    from gguf import GGUFWriter
+
+    w = GGUFWriter(str(path), arch)
+    for key, v in meta.items():
+        key = key.replace("__", ".")
+        (w.add_string if isinstance(v, str) else w.add_float32 if isinstance(v, float) else w.add_uint32)(key, v)
+    for name, arr in tensors:
+        w.add_tensor(name, arr)
+    w.write_header_to_file()
+    w.write_kv_data_to_file()
+    w.write_tensors_to_file()
+    w.close()
+    return str(path)
+
+
+def loaded_layer(n_outs, ids, k=K):
+    """What LowRankAdapters looks at of a layer, in host memory."""
+    lin = torch.nn.Module()
+    lin.weight = torch.nn.Module()
+    lin.weight.shard_id = list(ids)
+    lin.gguf_tiles = {sid: None for sid in ids}
+    lin.gguf_tiles_rows = dict(zip(ids, n_outs))
+    lin.gguf_groups = {ids[0]: (torch.zeros(1, dtype=torch.uint8), None, None, list(ids), k // 256, 0)}
+    return lin
+
+
+def model_with_banks(slots=3, rank=8):
+    model = loader.LoadedModel()
+    for key, n_outs, ids in (("layers.3.self_attn.qkv_proj", (48, 16, 16), ("q", "k", "v")), ("layers.3.self_attn.o_proj", (24,), (None,))):
+        lin = model.linears[key] = loaded_layer(n_outs, ids)
+        bank = lin.gguf_adapters = LowRankAdapters(lin, slots, rank)
+        for t in (bank.a, bank.b, bank.scales):
+            t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(t.numel())))
+    return model
+
+
+def pair(name, r, n_out, k=K):
+    return [(f"{name}.lora_a", np.ones((r, k), np.float32)), (f"{name}.lora_b", np.ones((n_out, r), np.float32))]
+
+
+GOOD = pair("blk.3.attn_q.weight", 4, 48)
+
+
+@pytest.mark.parametrize("slot,tensors", [
+    (0, GOOD + pair("blk.3.attn_output.weight", 4, 24, k=512)), (0, GOOD + pair("blk.3.attn_output.weight", 4, 32)), (0, GOOD + pair("blk.3.attn_k.weight", 4, 48)),
+    (0, GOOD + [pair("blk.3.attn_v.weight", 4, 16)[0], pair("blk.3.attn_v.weight", 5, 16)[1]]), (0, GOOD + [("blk.3.attn_v.weight.lora_a", np.ones(K, np.float32)), pair("blk.3.attn_v.weight", 1, 16)[1]]),
+    (-1, GOOD), (3, GOOD), (-1, []), (3, [])], ids=["K", "rows", "another shard's rows", "two ranks", "a row", "slot -1", "slot 3", "nothing into slot -1", "nothing into slot 3"])
+def test_an_adapter_that_does_not_fit_changes_nothing(tmp_path, slot, tensors):
+    model = model_with_banks()
+    banks = [lin.gguf_adapters for lin in model.linears.values()]
+    before = [t.clone() for b in banks for t in (b.a, b.b, b.scales)]
+    path = write_gguf(tmp_path / "adapter.gguf", tensors, general__type="adapter", adapter__type="lora", adapter__lora__alpha=8.0)
+    with pytest.raises((E, ValueError)):
+        loader.load_adapter(path, model, slot)
+    assert all(torch.equal(t, old) for t, old in zip([t for b in banks for t in (b.a, b.b, b.scales)], before))
+
+
+def test_an_adapter_that_fits_fills_its_slot_alone(tmp_path):
+    model = model_with_banks()
+    bank, other = (lin.gguf_adapters for lin in model.linears.values())
+    before = [bank.a.clone(), bank.b.clone()]
+    path = write_gguf(tmp_path / "adapter.gguf", GOOD, general__type="adapter", adapter__type="lora", adapter__lora__alpha=8.0)
+    assert loader.load_adapter(path, model, 1, scale=0.5) == ["layers.3.self_attn.qkv_proj"]
+    assert bool((bank.a[1, :4] == 1).all()) and not bool(bank.a[1, 4:].any()) and bool((bank.b[1, :48, :4] == 1).all()) and not bool(bank.b[1, 48:].any()) and not bool(bank.b[1, :, 4:].any())
+    assert bank.scales[1].tolist() == [1.0, 0.0, 0.0] and not bool(other.a[1].any()) and not bool(other.scales[1].any())
+    assert torch.equal(bank.a[[0, 2]], before[0][[0, 2]]) and torch.equal(bank.b[[0, 2]], before[1][[0, 2]])
+    for slot in (-1, 3):
+        with pytest.raises(E, match="no slot"):
+            bank.clear(slot)
