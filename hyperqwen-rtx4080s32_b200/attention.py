@@ -35,15 +35,17 @@ class PagedKVCache:
 
 class GGUFAttention(torch.nn.Module):
     """`qkv` and `o` are the merged projection (shards "q", "k", "v") and the output projection; where the q shard has twice the heads' rows, each
-    head is followed by an output gate.  q_norm, k_norm: bf16 [head_dim] or None.  inv_freq, amplitude: ops.rotary_frequencies."""
+    head is followed by an output gate.  head_dim is 64, 128 or 256.  q_norm, k_norm: bf16 [head_dim] or None.  inv_freq, amplitude: ops.rotary_frequencies."""
 
     def __init__(self, qkv: GGUFLinear, o: GGUFLinear, head_dim: int, inv_freq: torch.Tensor, *, amplitude: float = 1.0, q_norm: torch.Tensor | None = None,
                  k_norm: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False):
         super().__init__()
         if len(qkv.output_partition_sizes) != 3:
             raise GqError("qkv has the shards q, k and v")
+        if head_dim not in ops.ATTENTION_HEAD_DIMS:            # paged_attention would refuse it, behind the store into the cache
+            raise GqError(f"attention takes heads of {ops.ATTENTION_HEAD_DIMS}, got {head_dim}")
         rows_q, rows_k, rows_v = qkv.output_partition_sizes
-        if o.input_size % head_dim or rows_k % head_dim or rows_k != rows_v or rows_q not in (o.input_size, 2 * o.input_size):
+        if o.input_size % head_dim or not rows_k or rows_k % head_dim or rows_k != rows_v or o.input_size % rows_k or rows_q not in (o.input_size, 2 * o.input_size):
             raise GqError(f"heads of {head_dim} do not fit q / k / v rows of {rows_q} / {rows_k} / {rows_v} and an output projection of {o.input_size} columns")
         self.qkv, self.o = qkv, o
         self.head_dim, self.n_heads, self.n_kv_heads = head_dim, o.input_size // head_dim, rows_k // head_dim

@@ -571,6 +571,7 @@ class NativeRun:
 # in full before anything is launched (GqError).  What only the device can see (an id, a slot, a page outside its range) sets device_status to 2.
 
 MAX_RANK = 128
+ATTENTION_HEAD_DIMS = (64, 128, 256)
 
 
 def _aside() -> bool:

@@ -7,7 +7,8 @@ import pytest
 import torch
 
 from hyperqwen_rtx4080s32_b200 import loader, ops
-from hyperqwen_rtx4080s32_b200.linear import LowRankAdapters
+from hyperqwen_rtx4080s32_b200.attention import GGUFAttention
+from hyperqwen_rtx4080s32_b200.linear import GGUFLinear, LowRankAdapters
 
 import test_block_ops_cpu as refusals
 
@@ -121,3 +122,15 @@ def test_an_adapter_that_fits_fills_its_slot_alone(tmp_path):
     for slot in (-1, 3):
         with pytest.raises(E, match="no slot"):
             bank.clear(slot)
+
+
+def test_heads_that_the_attention_does_not_take_are_refused_when_the_block_is_made():
+    inv = torch.zeros(4, dtype=torch.float64)
+    for d in (64, 128, 256):
+        assert GGUFAttention(GGUFLinear(512, [6 * d, 2 * d, 2 * d]), GGUFLinear(6 * d, [512]), d, inv).n_heads == 6
+    for d in (96, 32, 16, 512, 8):
+        with pytest.raises(E, match="attention takes heads of"):
+            GGUFAttention(GGUFLinear(512, [8 * d, 2 * d, 2 * d]), GGUFLinear(8 * d, [512]), d, inv)
+    for n_heads, n_kv in ((5, 2), (2, 4), (4, 0)):
+        with pytest.raises(E, match="do not fit"):
+            GGUFAttention(GGUFLinear(512, [n_heads * 64, n_kv * 64, n_kv * 64]), GGUFLinear(n_heads * 64, [512]), 64, inv)
