@@ -303,6 +303,8 @@ class Checked {
     }
     void add(const at::Tensor &t) { if (count_ < 16) all_[count_++] = &t; }
     void devices() const {
+        for (int i = 0; i < count_; ++i)
+            if (all_[i]->_fw_grad(0).defined()) refuse(op_, "has no forward derivative: call it with the primals of its inputs");
         for (int i = 0; i < count_; ++i) {
             if (!all_[i]->is_cuda()) refuse(op_, "takes CUDA tensors (there is no CPU path)");
             if (!plain_tensor(*all_[i])) refuse(op_, "takes tensors that are what their memory says (no negative views, wrappers or transforms)");

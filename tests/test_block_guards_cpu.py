@@ -134,3 +134,12 @@ def test_heads_that_the_attention_does_not_take_are_refused_when_the_block_is_ma
     for n_heads, n_kv in ((5, 2), (2, 4), (4, 0)):
         with pytest.raises(E, match="do not fit"):
             GGUFAttention(GGUFLinear(512, [n_heads * 64, n_kv * 64, n_kv * 64]), GGUFLinear(n_heads * 64, [512]), 64, inv)
+
+
+@pytest.mark.parametrize("call,names", [(refusals.adapters, dict(x=(3, 256), base=(3, 24), b=(2, 24, 8))), (refusals.heads, dict(qkv=(5, 128))), (refusals.attend, dict(q=(4, 6, 64), v_pages=(3, 16, 2, 64)))], ids=["adapters", "heads", "attention"])
+def test_a_forward_tangent_is_refused(call, names):
+    import torch.autograd.forward_ad as fwd
+
+    for name, shape in names.items():
+        with fwd.dual_level(), pytest.raises(E, match="forward derivative"):
+            call(**{name: fwd.make_dual(h(*shape), h(*shape))})
