@@ -112,9 +112,12 @@ template <int RANKS, class OF> __device__ __forceinline__ void store_inner(const
         const int shard = tile / per_shard, rank = (tile - shard * per_shard) * 16 + c % 16;
         sum *= p.scales[id * p.n_shards + shard];
         const int64_t to = (int64_t)(row0 + groups.list[at + r]) * (p.n_shards * p.ranks) + shard * p.ranks + rank;
-        const __nv_bfloat16 big = __float2bfloat16_rn(sum);
+        // an infinity has nothing left over (inf - inf would make NaN of it), and a finite sum beyond bf16's range is its largest value and a rest
+        constexpr float TOP = 3.3895313892515355e38f;
+        const bool infinite = isinf(sum);
+        const __nv_bfloat16 big = __float2bfloat16_rn(!infinite && fabsf(sum) > TOP ? copysignf(TOP, sum) : sum);
         p.big[to] = big;
-        p.small[to] = __float2bfloat16_rn(sum - __bfloat162float(big));
+        p.small[to] = infinite ? __float2bfloat16_rn(0.0f) : __float2bfloat16_rn(sum - __bfloat162float(big));
     }
     if (p.parts > 1) cluster_sync_all();            // nobody reads this block's sums any more
     else __syncthreads();

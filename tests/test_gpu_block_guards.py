@@ -1,0 +1,47 @@
+"""Values and calls at the edge of what the operators beside the layers take: infinities, gates that hold NaN, caches of nothing."""
+import pytest
+import torch
+
+from hyperqwen_rtx4080s32_b200 import ops
+
+import test_gpu_adapters as adapters
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+@pytest.mark.parametrize("m,rank,bank", [(1, 8, 1), (5, 16, 3), (30, 64, 6), (150, 16, 2), (150, 128, 5)])
+def test_inner_values_beyond_bf16_are_not_made_nan(m, rank, bank):
+    """Row 0: an infinite activation against positive weights.  Last row: inner values of 3.4e38, which 32 bits hold and bf16 alone does not, against columns
+    small enough for the result.  Both against the definition: signed infinities, and a value within the usual bound."""
+    s = adapters.make(m, 256, (48, 37), rank, bank, seed=m)
+    s["ids"][0] = s["ids"][m - 1] = bank - 1
+    s["scales"].fill_(1.0)
+    a, b = s["a"][bank - 1], s["b"][bank - 1]
+    a.copy_(a.abs() + 2.0 ** -6)
+    b[:20] = b[:20].abs() + 2.0 ** -6             # columns that become +inf, -inf, and (mixed signs) NaN
+    b[20:40] = -b[20:40].abs() - 2.0 ** -6
+    b[40:44, 0], b[40:44, 1:] = 1.0, -1.0
+    s["x"][0, 77] = INF
+    got = adapters.call(s)
+    assert bool((got[0, :20] == INF).all()) and bool((got[0, 20:40] == -INF).all()) and bool(got[0, 40:44].isnan().all())
+    s["x"][0, 77] = -INF
+    got = adapters.call(s)
+    assert bool((got[0, :20] == -INF).all()) and bool((got[0, 20:40] == INF).all())
+    if m > 1:
+        rest = torch.arange(1, m, device="cuda")
+        s["x"][0, 77] = 0
+        want, bound = adapters.want_and_bound(s)
+        assert bool(((got.double() - want).abs() <= bound)[rest].all())
+    # inner values between bf16's largest (0x1.fep127) and 32 bits': products of 0x1.fcp127 and 0x1.8p120, a sum that 32 bits hold exactly
+    row = m - 1
+    s["x"][row].zero_()
+    s["x"][row, 3], s["x"][row, 200] = 2.0 ** 127, 2.0 ** 120
+    a.zero_()
+    a[:, 3], a[:, 200] = 1.984375, 1.5
+    b.mul_(2.0 ** -110)
+    b[40:44] = 0
+    got = adapters.call(s)
+    assert bool(got[row].isfinite().all())
+    want, bound = adapters.want_and_bound(s)
+    assert bool(((got.double() - want).abs() <= bound)[row].all()) and float(want[row].abs().max()) > 0
