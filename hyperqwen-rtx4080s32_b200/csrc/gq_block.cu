@@ -183,7 +183,7 @@ extern "C" int gq_low_rank_add(const gq_low_rank_args *p, void *stream) {
 
 extern "C" int gq_head_norm_rope(const gq_head_norm_args *p, void *stream) {
     if (!p) return GQ_ERR_ARG;
-    const bool store = p->k_pages || p->v_pages;
+    const bool store = p->k_pages || p->v_pages || (p->slots && !p->k_out);       // a cache of no pages has no memory
     if (p->T < 0 || p->T > INT32_MAX || p->n_heads < 1 || p->n_kv_heads < 1 || p->head_dim < 8 || p->head_dim % 8 || p->rotary_dim < 0 || p->rotary_dim % 2 ||
         p->rotary_dim > p->head_dim) return GQ_ERR_SHAPE;
     if (p->head_dim > 512 || (int64_t)p->n_heads + 2 * (int64_t)p->n_kv_heads > 65535) return GQ_ERR_LIMIT;
@@ -193,21 +193,23 @@ extern "C" int gq_head_norm_rope(const gq_head_norm_args *p, void *stream) {
     if (!p->qkv || !p->q_out || !p->positions || (p->rotary_dim && !p->inv_freq) || (p->positions_bytes != 4 && p->positions_bytes != 8) || p->ld_qkv < width) return GQ_ERR_ARG;
     if (!aligned(p->qkv, 16) || p->ld_qkv % 8 || !aligned(p->q_out, 16) || !aligned(p->q_norm, 16) || !aligned(p->k_norm, 16)) return GQ_ERR_ARG;
     if (store) {
-        if (!p->k_pages || !p->v_pages || !p->slots || (p->slots_bytes != 4 && p->slots_bytes != 8) || p->k_out || !aligned(p->k_pages, 16) || !aligned(p->v_pages, 16)) return GQ_ERR_ARG;
+        if ((p->n_pages && (!p->k_pages || !p->v_pages)) || !p->slots || (p->slots_bytes != 4 && p->slots_bytes != 8) || p->k_out || !aligned(p->k_pages, 16) || !aligned(p->v_pages, 16)) return GQ_ERR_ARG;
         for (int i = 0; i < 3; ++i)
             if (p->k_strides[i] % 8 || p->v_strides[i] % 8) return GQ_ERR_ARG;
     } else if (!p->k_out || !aligned(p->k_out, 16)) return GQ_ERR_ARG;
     int *status;
     if (const int rc = status_word(&status)) return rc;
+    gq_head_norm_args a = *p;
+    if (!store) a.slots = nullptr;                                           // what the kernels look at
     if (p->head_dim % 16 || (!p->interleaved && p->rotary_dim % 16)) {
-        GQ_CUDA(launch_pdl(head_norm_any_kernel, dim3((unsigned)p->T, p->n_heads + (store ? 2 : 1) * p->n_kv_heads), 64, 0, stream, *p, status));
+        GQ_CUDA(launch_pdl(head_norm_any_kernel, dim3((unsigned)p->T, p->n_heads + (store ? 2 : 1) * p->n_kv_heads), 64, 0, stream, a, status));
     } else {
         int group = 1;                                                       // lanes of a head, a power of two
         while (group * 16 < p->head_dim) group *= 2;
         const int batch = p->T >= 2048 ? HEAD_BATCH : 1;                     // few tokens: a block each
         const unsigned blocks = (unsigned)((p->T + batch - 1) / batch);
-        if (p->interleaved) GQ_CUDA(launch_pdl(head_norm_kernel<true>, dim3(blocks), HEAD_THREADS, 0, stream, *p, batch, group, status));
-        else GQ_CUDA(launch_pdl(head_norm_kernel<false>, dim3(blocks), HEAD_THREADS, 0, stream, *p, batch, group, status));
+        if (p->interleaved) GQ_CUDA(launch_pdl(head_norm_kernel<true>, dim3(blocks), HEAD_THREADS, 0, stream, a, batch, group, status));
+        else GQ_CUDA(launch_pdl(head_norm_kernel<false>, dim3(blocks), HEAD_THREADS, 0, stream, a, batch, group, status));
     }
     GQ_LAUNCHED();
     return GQ_OK;

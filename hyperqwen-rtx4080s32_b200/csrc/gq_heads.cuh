@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(HEAD_THREADS) head_norm_kernel(const __grid_co
     __shared__ int64_t k_at[HEAD_BATCH], v_at[HEAD_BATCH];     // where a token's keys and values go, -1: nowhere
     const int D = p.head_dim, lanes = D / 16, half = p.rotary_dim / 2, turn_lanes = (half + 7) / 8, wide = p.gated ? 2 * D : D;
     const int l = threadIdx.x & (group - 1), sub = (int)threadIdx.x / group, per_turn = HEAD_THREADS / group;       // lane of the head, head of this turn
-    const bool store = p.k_pages != nullptr, live = l < lanes, norms = p.q_norm || p.k_norm;
+    const bool store = p.slots != nullptr, live = l < lanes, norms = p.q_norm || p.k_norm;
     const int heads = p.n_heads + p.n_kv_heads;
     const int64_t t0 = (int64_t)blockIdx.x * batch;
     const int tokens = (int)min((int64_t)batch, p.T - t0), items = tokens * heads;
@@ -191,7 +191,7 @@ __global__ void head_norm_any_kernel(const gq_head_norm_args p, int *status) {
     const __nv_bfloat16 *src = (const __nv_bfloat16 *)p.qkv + t * p.ld_qkv +
                                (is_q ? (int64_t)h * wide : (int64_t)p.n_heads * wide + (int64_t)(is_k ? h : h + p.n_kv_heads) * D);
     __nv_bfloat16 *dst = is_q ? (__nv_bfloat16 *)p.q_out + (t * p.n_heads + h) * D : (__nv_bfloat16 *)p.k_out + (t * p.n_kv_heads + h) * D;
-    if (!is_q && p.k_pages) {
+    if (!is_q && p.slots) {
         const int64_t slot = p.slots_bytes == 8 ? ((const int64_t *)p.slots)[t] : ((const int32_t *)p.slots)[t];
         if (slot < 0) return;
         const int64_t page = slot / p.page_size, row = slot % p.page_size;

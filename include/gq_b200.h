@@ -318,9 +318,9 @@ typedef struct gq_head_norm_args {
     const double *inv_freq;      /* [rotary_dim / 2], radians per position */
     const void *q_norm, *k_norm; /* bf16 [head_dim] or null */
     void *q_out;                 /* bf16 [T, n_heads, head_dim], contiguous */
-    void *k_out;                 /* the same for keys, or null where pages are given */
-    void *k_pages, *v_pages;     /* bf16 [n_pages, page_size, n_kv_heads, head_dim] by strides, or null */
-    const void *slots;           /* int32 or int64 [T]: page * page_size + row */
+    void *k_out;                 /* the same for keys, or null: keys and values are stored */
+    void *k_pages, *v_pages;     /* bf16 [n_pages, page_size, n_kv_heads, head_dim] by strides; null where keys are not stored, or n_pages is 0 */
+    const void *slots;           /* int32 or int64 [T]: page * page_size + row; null where keys are not stored */
     int64_t T, ld_qkv, n_pages;
     int64_t k_strides[3], v_strides[3];     /* elements between pages, rows, heads */
     int32_t n_heads, n_kv_heads, head_dim, rotary_dim, page_size, positions_bytes, slots_bytes, interleaved, gated;

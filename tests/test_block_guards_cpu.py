@@ -1,4 +1,5 @@
 """Guards of the operators beside the layers that need no GPU: the order of programmatic launches, refusals, files and banks."""
+import ctypes
 import os
 import re
 
@@ -6,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from hyperqwen_rtx4080s32_b200 import loader, ops
+from hyperqwen_rtx4080s32_b200 import _lib, loader, ops
 from hyperqwen_rtx4080s32_b200.attention import GGUFAttention
 from hyperqwen_rtx4080s32_b200.linear import GGUFLinear, LowRankAdapters
 
@@ -143,3 +144,24 @@ def test_a_forward_tangent_is_refused(call, names):
     for name, shape in names.items():
         with fwd.dual_level(), pytest.raises(E, match="forward derivative"):
             call(**{name: fwd.make_dual(h(*shape), h(*shape))})
+
+
+class HeadNormArgs(ctypes.Structure):
+    """gq_head_norm_args of include/gq_b200.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("qkv", "positions", "inv_freq", "q_norm", "k_norm", "q_out", "k_out", "k_pages", "v_pages", "slots")] + [
+        (n, ctypes.c_int64) for n in ("T", "ld_qkv", "n_pages")] + [("k_strides", ctypes.c_int64 * 3), ("v_strides", ctypes.c_int64 * 3)] + [
+        (n, ctypes.c_int32) for n in ("n_heads", "n_kv_heads", "head_dim", "rotary_dim", "page_size", "positions_bytes", "slots_bytes", "interleaved", "gated")] + [("eps", ctypes.c_float), ("amplitude", ctypes.c_float)]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are none: what is accepted has to end at the missing device")
+@pytest.mark.parametrize("pages,slots,k_out,n_pages,accepted", [
+    (False, True, False, 0, True), (False, True, False, 3, False), (True, True, False, 3, True), (True, False, False, 3, False), (True, True, True, 3, False), (False, False, True, 0, True),
+    (False, True, True, 0, True), (False, False, False, 0, False)], ids=str)
+def test_what_says_that_keys_are_stored(pages, slots, k_out, n_pages, accepted):
+    """Pages, or slots without an output for keys: a cache of no pages has null pointers and is stored into all the same (no slot is inside it)."""
+    a = HeadNormArgs(T=2, ld_qkv=256, n_pages=n_pages, n_heads=2, n_kv_heads=1, head_dim=64, page_size=16, positions_bytes=8, slots_bytes=8)
+    a.qkv = a.q_out = a.positions = 1 << 20
+    if pages:
+        a.k_pages = a.v_pages = 1 << 20
+    a.slots, a.k_out = (1 << 20) if slots else None, (1 << 20) if k_out else None
+    assert (_lib.lib().gq_head_norm_rope(ctypes.byref(a), None) == -3) == (not accepted)

@@ -5,6 +5,7 @@ import torch
 from hyperqwen_rtx4080s32_b200 import ops
 
 import test_gpu_adapters as adapters
+import test_gpu_heads as heads
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -45,3 +46,15 @@ def test_inner_values_beyond_bf16_are_not_made_nan(m, rank, bank):
     assert bool(got[row].isfinite().all())
     want, bound = adapters.want_and_bound(s)
     assert bool(((got.double() - want).abs() <= bound)[row].all()) and float(want[row].abs().max()) > 0
+
+
+@pytest.mark.parametrize("d", [64, 72])
+def test_a_cache_of_no_pages(d):
+    s, how = heads.make(5, 4, 2, d, 24 if d == 72 else 32, seed=2)
+    want = ops.qk_norm_rope(**s, **how)[0]
+    none = torch.zeros(0, 16, 2, d, dtype=torch.bfloat16, device="cuda")
+    slots = torch.full((5,), -1, device="cuda")
+    assert torch.equal(ops.qk_norm_rope_store(**s, k_pages=none, v_pages=none.clone(), slots=slots, **how), want) and ops.device_status() == 0
+    slots[2] = 0
+    assert torch.equal(ops.qk_norm_rope_store(**s, k_pages=none, v_pages=none.clone(), slots=slots, **how), want)
+    assert ops.device_status() == 2 and ops.device_status() == 0
