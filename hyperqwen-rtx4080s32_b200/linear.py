@@ -252,11 +252,12 @@ class GGUFLinearMethod:
             ops.native().finish(packed)
 
     def check_status(self, device=None) -> None:
-        """Raise if any kernel of the path has reported a bounded wait that ran out on the device since the last
-        check (the result of that call was incomplete).  Synchronises; meant for the engine to call between steps."""
+        """Raise if any kernel of the path, or of the operators beside it, has reported a bounded wait that ran out or an argument that only the device sees to be
+        wrong since the last check (the result of that call is incomplete).  Synchronises; meant for the engine to call between steps."""
         code = ops.device_status(device, clear=True)
         if code:
-            raise RuntimeError(f"gq_b200: a kernel reported device status {code} (1: a bounded wait ran out; 2: bad shape, a tile's type that contradicts the call, or an id outside an embedding table) since the last check")
+            raise RuntimeError(f"gq_b200: a kernel reported device status {code} (1: a bounded wait ran out; 2: bad shape, a tile's type that contradicts the call, an id outside an embedding table or a bank of adapters, a slot or page outside a cache, "
+                               "or a length beyond a page table) since the last check")
 
     # ---- a6 ----
     def apply(self, layer: torch.nn.Module, x: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:

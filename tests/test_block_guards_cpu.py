@@ -9,7 +9,7 @@ import torch
 
 from hyperqwen_rtx4080s32_b200 import _lib, loader, ops
 from hyperqwen_rtx4080s32_b200.attention import GGUFAttention
-from hyperqwen_rtx4080s32_b200.linear import GGUFLinear, LowRankAdapters
+from hyperqwen_rtx4080s32_b200.linear import GGUFLinear, GGUFLinearMethod, LowRankAdapters
 
 import test_block_ops_cpu as refusals
 
@@ -165,3 +165,14 @@ def test_what_says_that_keys_are_stored(pages, slots, k_out, n_pages, accepted):
         a.k_pages = a.v_pages = 1 << 20
     a.slots, a.k_out = (1 << 20) if slots else None, (1 << 20) if k_out else None
     assert (_lib.lib().gq_head_norm_rope(ctypes.byref(a), None) == -3) == (not accepted)
+
+
+def test_the_status_message_names_what_the_word_reports(monkeypatch):
+    lin = GGUFLinear(256, [64])
+    assert isinstance(lin.quant_method, GGUFLinearMethod)
+    monkeypatch.setattr(ops, "device_status", lambda device=None, clear=True: 2)
+    with pytest.raises(RuntimeError, match="status 2") as raised:
+        lin.quant_method.check_status()
+    assert all(cause in str(raised.value) for cause in ("shape", "type", "embedding", "adapters", "slot", "page outside a cache", "page table"))
+    monkeypatch.setattr(ops, "device_status", lambda device=None, clear=True: 0)
+    lin.quant_method.check_status()
