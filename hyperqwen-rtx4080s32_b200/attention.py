@@ -27,9 +27,16 @@ class PagedKVCache:
         self.k, self.v = memory[0].transpose(1, 2), memory[1].transpose(1, 2)
 
     def slots(self, page_table: torch.Tensor, sequences: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
-        """The slots (int64) of tokens at `positions` of `sequences`, rows of page_table; a negative position has none (-1)."""
-        at = positions.clamp(min=0).long()
-        slots = page_table[sequences.long(), at // self.page_size].long() * self.page_size + at % self.page_size
+        """The slots (int64) of tokens at `positions` of `sequences`, rows of page_table; a negative position has none (-1).  Where the table has no page for a token, or
+        one outside the cache, the slot is beyond the cache: the store leaves it out and reports it (device_status 2)."""
+        at, seq = positions.clamp(min=0).long(), sequences.long()
+        page, (n_seqs, width), n_pages = at // self.page_size, page_table.shape, self.k.shape[0]
+        beyond = n_pages * self.page_size
+        if page_table.numel() == 0:
+            return torch.where(positions < 0, -1, beyond).expand(torch.broadcast_shapes(positions.shape, sequences.shape))
+        there = (page < width) & (seq >= 0) & (seq < n_seqs)
+        pages = page_table[seq.clamp(0, n_seqs - 1), page.clamp(max=width - 1)].long()       # an index outside the table would end the process's context
+        slots = torch.where(there & (pages >= 0) & (pages < n_pages), pages * self.page_size + at % self.page_size, beyond)
         return torch.where(positions < 0, -1, slots)
 
 

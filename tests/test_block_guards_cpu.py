@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from hyperqwen_rtx4080s32_b200 import _lib, loader, ops
-from hyperqwen_rtx4080s32_b200.attention import GGUFAttention
+from hyperqwen_rtx4080s32_b200.attention import GGUFAttention, PagedKVCache
 from hyperqwen_rtx4080s32_b200.linear import GGUFLinear, GGUFLinearMethod, LowRankAdapters
 
 import test_block_ops_cpu as refusals
@@ -176,3 +176,13 @@ def test_the_status_message_names_what_the_word_reports(monkeypatch):
     assert all(cause in str(raised.value) for cause in ("shape", "type", "embedding", "adapters", "slot", "page outside a cache", "page table"))
     monkeypatch.setattr(ops, "device_status", lambda device=None, clear=True: 0)
     lin.quant_method.check_status()
+
+
+def test_slots_where_the_table_has_no_page():
+    cache = PagedKVCache(7, 4, 2, 8, device="cpu")
+    table = torch.tensor([[5, 1], [6, -1], [7, 0]], dtype=torch.int32)
+    seqs, positions = torch.tensor([0, 0, 1, 1, 2, 2, 3, -1, 3, 0]), torch.tensor([7, 8, 3, 4, 0, 4, 0, 0, -1, 1 << 40])
+    assert cache.slots(table, seqs, positions).tolist() == [7, 28, 27, 28, 28, 0, 28, 28, -1, 28]
+    for empty in (table[:0], table[:, :0]):
+        got = cache.slots(empty, torch.tensor([0, 0]), torch.tensor([0, -1]))
+        assert got.dtype == torch.int64 and got.tolist() == [28, -1]
