@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(32 * KG * DG) paged_attention_kernel(const __g
                         for (int x = 0; x < 2; ++x) {
                             const int d = dim_of(i) + 8 * x;
                             float v = sum_o[q][i][2 * x + j] * inv;
-                            if (gate) v /= 1.0f + ex2(-1.4426950408889634f * __bfloat162float(gate[d]));
+                            if (gate && inv != 0.0f) v /= 1.0f + ex2(-1.4426950408889634f * __bfloat162float(gate[d]));        // no key: zeros, whatever the gate
                             dst[d] = __float2bfloat16_rn(v);
                         }
                 } else {
@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) join_parts_kernel(const __gri
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float v = o[i] * inv;
-                if (gate) v /= 1.0f + ex2(-1.4426950408889634f * __bfloat162float(gate[i * 32]));
+                if (gate && inv != 0.0f) v /= 1.0f + ex2(-1.4426950408889634f * __bfloat162float(gate[i * 32]));
                 dst[i * 32] = __float2bfloat16_rn(v);
             }
         }

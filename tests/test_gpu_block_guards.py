@@ -6,6 +6,7 @@ from hyperqwen_rtx4080s32_b200 import ops
 
 import test_gpu_adapters as adapters
 import test_gpu_heads as heads
+import test_gpu_paged as paged
 
 pytestmark = pytest.mark.gpu
 INF = float("inf")
@@ -58,3 +59,17 @@ def test_a_cache_of_no_pages(d):
     slots[2] = 0
     assert torch.equal(ops.qk_norm_rope_store(**s, k_pages=none, v_pages=none.clone(), slots=slots, **how), want)
     assert ops.device_status() == 2 and ops.device_status() == 0
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("value", [float("nan"), INF, -INF])
+def test_a_gate_of_a_token_that_sees_nothing(d, value):
+    """Tokens in front of the first key share a tile with tokens that see one, stand in tiles without a key, or in sequences without any."""
+    lens, news = [1, 0, 2, 40, 300], [2, 3, 60, 42, 1]
+    s, more, starts = paged.make(lens, news, 6, 2, d, 16, gated=True, seed=d)
+    clean = ops.paged_attention(**s, **more)
+    blind = torch.cat([torch.arange(n) < n - length for length, n in zip(lens, news)]).cuda()
+    assert int(blind.sum()) == 64
+    more["gate"][blind] = value
+    got = ops.paged_attention(**s, **more)
+    assert bool((got[blind] == 0).all()) and torch.equal(got, clean)
