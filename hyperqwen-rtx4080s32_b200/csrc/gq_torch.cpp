@@ -17,13 +17,17 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/util/SmallVector.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/core/grad_mode.h>
+#include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <string>
+#include <utility>
 #include <vector>
 #include "../../include/gq_b200.h"
 
@@ -324,6 +328,38 @@ inline int64_t extent(const at::Tensor &t) {
     for (int64_t i = 0; i < t.dim(); ++i) { if (t.size(i) == 0) return 0; n += (t.size(i) - 1) * t.stride(i); }
     return n;
 }
+using Dims = c10::SmallVector<std::pair<int64_t, int64_t>, 4>;          // stride, size
+// A tensor's dimensions of more than one element, the longest stride first; false if two of its elements may be one (a stride shorter than what lies inside it)
+bool nested(const at::Tensor &t, Dims &dims) {
+    for (int64_t i = 0; i < t.dim(); ++i)
+        if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+    std::sort(dims.rbegin(), dims.rend());
+    int64_t inside = 1;
+    for (size_t i = dims.size(); i-- > 0;) {
+        if (dims[i].first < inside) return false;
+        inside += (dims[i].second - 1) * dims[i].first;
+    }
+    return true;
+}
+bool own_memory(const at::Tensor &t) {
+    Dims dims;
+    return t.numel() == 0 || nested(t, dims);
+}
+// whether some difference of two indexes of these dimensions is `off` elements
+bool apart_by(const Dims &dims, size_t i, int64_t off) {
+    if (i == dims.size()) return off == 0;
+    const int64_t down = off / dims[i].first - (off % dims[i].first < 0);
+    for (int64_t d : {down, down + 1})           // what is left has to be less than a stride
+        if (std::abs(d) < dims[i].second && apart_by(dims, i + 1, off - d * dims[i].first)) return true;
+    return false;
+}
+// whether two caches of one shape share an element; exact where their strides are the same, else whether they start at one place
+bool same_cells(const at::Tensor &u, const at::Tensor &v) {
+    if (u.numel() == 0 || u.data_ptr() == v.data_ptr()) return u.numel() != 0;
+    Dims du, dv;
+    if (!nested(u, du) || !nested(v, dv) || du != dv) return false;
+    return apart_by(du, 0, ((const char *)v.data_ptr() - (const char *)u.data_ptr()) / u.element_size());
+}
 // whether two tensors' ranges of memory meet; of rows with unit stride, whether the rows do
 bool meet(const at::Tensor &u, const at::Tensor &v) {
     const char *a = (const char *)u.data_ptr(), *b = (const char *)v.data_ptr();
@@ -434,6 +470,8 @@ py::object norm_heads(const at::Tensor &qkv0, const at::Tensor &positions0, cons
         take_pages(c, *k_pages, n_kv_heads, head_dim, "k_pages is bf16 [pages, rows, kv heads, head_dim]", p.k_strides);
         take_pages(c, *v_pages, n_kv_heads, head_dim, "v_pages is bf16 [pages, rows, kv heads, head_dim]", p.v_strides);
         c.need(k_pages->size(0) == v_pages->size(0) && k_pages->size(1) == v_pages->size(1), "k_pages and v_pages hold the same pages");
+        c.need(own_memory(*k_pages) && own_memory(*v_pages), "the pages' rows and heads each have memory of their own");
+        c.need(!same_cells(*k_pages, *v_pages), "keys and values have pages of their own");
         c.need(slots0->dim() == 1 && slots0->size(0) == t && integers(*slots0), "slots is int32 or int64 [T]");
     }
     for (const at::Tensor *x : {&qkv0, &positions0, &inv_freq}) c.add(*x);
@@ -442,8 +480,11 @@ py::object norm_heads(const at::Tensor &qkv0, const at::Tensor &positions0, cons
     c.devices();
     if (store) {
         c.need(on16(*k_pages) && on16(*v_pages), "the pages start at multiples of 16 bytes");
-        for (auto *pages : {&*k_pages, &*v_pages})
+        for (auto *pages : {&*k_pages, &*v_pages}) {
             for (const at::Tensor *x : std::initializer_list<const at::Tensor *>{&qkv0, &positions0, &inv_freq, &*slots0}) c.need(!meet(*pages, *x), "the pages share no memory with the other arguments");
+            for (auto *w : {&q_norm, &k_norm})
+                if (w->has_value()) c.need(!meet(*pages, **w), "the pages share no memory with the other arguments");
+        }
     }
     Status status;
     at::Tensor q, k;
@@ -507,7 +548,7 @@ at::Tensor paged_attention(const at::Tensor &q0, const at::Tensor &k_pages, cons
             c.need((*x)->numel() == 0 || (*x)->stride(2) == 1, "gate and out have unit stride along head_dim");
         }
     if (out0.has_value())
-        c.need((t <= 1 || out0->stride(0) >= dim) && (heads <= 1 || out0->stride(1) >= dim), "out's rows and heads have memory of their own");
+        c.need((t <= 1 || out0->stride(0) >= dim) && (heads <= 1 || out0->stride(1) >= dim) && own_memory(*out0), "out's rows and heads have memory of their own");
     for (const at::Tensor *x : {&q0, &k_pages, &v_pages, &table0, &lens0}) c.add(*x);
     for (auto *x : {&q_starts0, &gate0, &out0})
         if (x->has_value()) c.add(**x);

@@ -186,3 +186,32 @@ def test_slots_where_the_table_has_no_page():
     for empty in (table[:0], table[:, :0]):
         got = cache.slots(empty, torch.tensor([0, 0]), torch.tensor([0, -1]))
         assert got.dtype == torch.int64 and got.tolist() == [28, -1]
+
+
+def test_outputs_and_caches_whose_own_parts_share_memory_are_refused():
+    buf = h(4096)
+    for strides in ((64, 64, 1), (64, 128, 1), (128, 64, 1), (320, 64, 1)):       # heads or tokens that begin inside another's
+        with pytest.raises(E, match="of their own"):
+            refusals.attend(out=buf.as_strided((4, 6, 64), strides))
+    for strides in ((384, 64, 1), (64, 256, 1), (72, 300, 1)):
+        with pytest.raises(E, match="CUDA"):
+            refusals.attend(out=buf.as_strided((4, 6, 64), strides))
+    for strides in ((32, 32, 16, 1), (128, 16, 16, 1), (64, 32, 16, 1)):
+        with pytest.raises(E, match="of their own"):
+            refusals.heads(store=True, k_pages=buf.as_strided((3, 4, 2, 16), strides))
+
+
+def test_keys_and_values_in_one_memory_are_refused_and_side_by_side_are_not():
+    one = h(3, 4, 2, 16)
+    buf, both = h(4, 4, 2, 16), h(3, 2, 4, 2, 16)
+    for k, v in ((one, one), (buf[:3], buf[1:]), (buf[1:], buf[:3])):
+        with pytest.raises(E, match="pages of their own"):
+            refusals.heads(store=True, k_pages=k, v_pages=v)
+    flat, by_head, turns = h(3, 4, 4, 16), h(3, 2, 8, 16), h(6, 4, 2, 16)
+    for k, v in ((both[:, 0], both[:, 1]), (both[:, 1], both[:, 0]), (flat[:, :, :2], flat[:, :, 2:]), (flat[:, :, ::2], flat[:, :, 1::2]), (by_head[:, :, :4].transpose(1, 2), by_head[:, :, 4:].transpose(1, 2)),
+                 (turns[::2], turns[1::2]), (one, one.clone())):
+        with pytest.raises(E, match="CUDA"):
+            refusals.heads(store=True, k_pages=k, v_pages=v)
+    rows = h(800)
+    with pytest.raises(E, match="pages of their own"):                   # a row further: most rows are shared
+        refusals.heads(store=True, k_pages=rows.as_strided((3, 4, 2, 16), (128, 32, 16, 1)), v_pages=rows.as_strided((3, 4, 2, 16), (128, 32, 16, 1), 32))
