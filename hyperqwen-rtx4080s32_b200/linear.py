@@ -98,6 +98,13 @@ class GGUFConfig:
         return GGUFLinearMethod(self)
 
 
+def _rows_of_residual(pre) -> None:
+    """The residual of an op in front as rows, as the layer sees its activation."""
+    if getattr(pre, "residual", None) is not None:
+        pre.residual = pre.residual.reshape(-1, pre.residual.shape[-1])
+        pre.residual_out = pre.residual_out.reshape(-1, pre.residual_out.shape[-1])
+
+
 class GGUFLinearMethod:
     """Linear method for GGUF on B200."""
 
@@ -268,9 +275,8 @@ class GGUFLinearMethod:
         into the launch for up to 16 rows.  An addition to the reference's method, whose apply takes the finished
         activation (gguf-tiles-all-types.patch:203-262)."""
         native = layer.__dict__.get("gguf_native")
-        if pre is not None and getattr(pre, "residual", None) is not None:
-            pre.residual = pre.residual.reshape(-1, pre.residual.shape[-1])
-            pre.residual_out = pre.residual_out.reshape(-1, pre.residual_out.shape[-1])
+        if pre is not None:
+            _rows_of_residual(pre)
         if native is not None:
             out = native(layer.gguf_groups, x, pre)
             if out is not None:
@@ -315,9 +321,13 @@ class GGUFLinearMethod:
             raise RuntimeError("the layer has no bank of adapters: add_adapters was not called")
         if ops.in_fused_allreduce():
             raise ops.GqError("adapters are added before the sum over the ranks: call the layer outside fused_allreduce and all-reduce its output")
+        lead = x.shape[:-1]
+        x = x.reshape(-1, x.shape[-1])
         if pre is not None:
+            _rows_of_residual(pre)
             x = pre.unfused(x)
-        return bank.add_(self.apply(layer, x, bias), x, ids)
+        out = bank.add_(self.apply(layer, x, bias), x, ids)
+        return out.reshape(*lead, out.shape[-1])
 
 
 # ---- low-rank adapters beside a layer ------------------------------------------------------------------

@@ -215,3 +215,22 @@ def test_keys_and_values_in_one_memory_are_refused_and_side_by_side_are_not():
     rows = h(800)
     with pytest.raises(E, match="pages of their own"):                   # a row further: most rows are shared
         refusals.heads(store=True, k_pages=rows.as_strided((3, 4, 2, 16), (128, 32, 16, 1)), v_pages=rows.as_strided((3, 4, 2, 16), (128, 32, 16, 1), 32))
+
+
+@pytest.mark.parametrize("x_shape,residual_shape", [((2, 3, K), (2, 3, K)), ((2, 3, K), (6, K)), ((6, K), (6, K)), ((6, K), (2, 3, K))], ids=str)
+def test_a_residual_of_any_shape_in_front_of_a_layer_with_adapters(monkeypatch, x_shape, residual_shape):
+    """As in front of the layer alone: the rows are what counts, and residual_out comes back as rows."""
+    lin, seen = loaded_layer((24,), (None,)), []
+    method = GGUFLinear(K, [24]).quant_method
+    bank = lin.gguf_adapters = LowRankAdapters(lin, 2, 8)
+    monkeypatch.setattr(method, "apply", lambda layer, x, bias=None: x[..., :24].clone())
+    monkeypatch.setattr(bank, "add_", lambda y, x, ids: seen.append((x, ids)) or y)
+    g = torch.Generator().manual_seed(1)
+    x, residual = (torch.randn(s, generator=g).to(torch.bfloat16) for s in (x_shape, residual_shape))
+    pre = ops.PreAddRMSNorm(torch.ones(K, dtype=torch.bfloat16), residual=residual)
+    ids = torch.zeros(x_shape[:-1], dtype=torch.int64)
+    out = method.apply_with_adapters(lin, x, ids, pre)
+    plain = ops.PreAddRMSNorm(torch.ones(K, dtype=torch.bfloat16), residual=residual.reshape(-1, K))
+    want = plain.unfused(x.reshape(-1, K))
+    assert out.shape == (*x_shape[:-1], 24) and torch.equal(out.reshape(-1, 24), want[:, :24]) and torch.equal(seen[0][0].reshape(-1, K), want)
+    assert torch.equal(pre.residual_out.reshape(-1, K), plain.residual_out) and pre.residual_out.shape == (6, K)
