@@ -118,10 +118,24 @@ class LoadedModel:
             if name.startswith("layers."):
                 lin.quant_method.add_adapters(lin, n_adapters, rank)
 
+    def _beyond_the_block(self, own_scaling: bool) -> list[str]:
+        """What the file says about its attention that GGUFAttention does not do: it would be left out without a word."""
+        meta = self.meta
+        neutral = {"attention.sliding_window": 0, "attention.scale": 0.0, "attn_logit_softcapping": 0.0, "attention.max_alibi_bias": 0.0, "attention.clamp_kqv": 0.0, "attention.causal": True}
+        found = [k for k, v in neutral.items() if meta.get(k, v) != v]
+        if not own_scaling:
+            neutral = {"attn_factor": 1.0, "yarn_attn_factor": 1.0, "yarn_ext_factor": 1.0, "yarn_log_multiplier": 0.0, "alpha": 0.0}
+            found += [f"rope.scaling.{k}" for k, v in neutral.items() if meta.get(f"rope.scaling.{k}", v) != v]
+            found += [n for n in self.unmapped if re.search(r"(^|\.)rope_(freqs|factors_long|factors_short)\.weight$", n)]
+            if "rope.scaling.type" not in meta and meta.get("rope.scaling.factor", 1.0) not in (0.0, 1.0):
+                found.append("rope.scaling.factor without a type")
+        return found
+
     def attention(self, layer: int, *, head_dim: int | None = None, interleaved: bool = False, **rotary):
         """The attention half of a block (attention.GGUFAttention) from its qkv_proj, o_proj and head norms.  What the file says about heads, rotation and eps is
-        taken from it; `head_dim` and the arguments of ops.rotary_frequencies (rotary_dim, base, scaling, factor, original_context) go before.  A token has one
-        position (text); `interleaved` where the architecture turns neighbours, which the file does not say."""
+        taken from it; `head_dim` and the arguments of ops.rotary_frequencies (rotary_dim, base, scaling, factor, original_context, beta_fast, beta_slow) go before.  A token has
+        one position (text); `interleaved` where the architecture turns neighbours, which the file does not say.  A file that says what this attention does not do (a sliding
+        window, rotation factors of its own, ...) raises ValueError; with `scaling` given, what it says about scaling is not looked at."""
         from . import ops
         from .attention import GGUFAttention
 
@@ -136,7 +150,11 @@ class LoadedModel:
         if not head_dim:
             raise ValueError("neither the file nor the call says how wide a head is")
         known = {"rotary_dim": meta.get("rope.dimension_count", head_dim), "base": meta.get("rope.freq_base", 10000.0), "scaling": meta.get("rope.scaling.type"),
-                 "factor": meta.get("rope.scaling.factor", 1.0), "original_context": meta.get("rope.scaling.original_context_length")}
+                 "factor": meta.get("rope.scaling.factor", 1.0), "original_context": meta.get("rope.scaling.original_context_length"),
+                 "beta_fast": meta.get("rope.scaling.yarn_beta_fast", 32.0), "beta_slow": meta.get("rope.scaling.yarn_beta_slow", 1.0)}
+        unknown = self._beyond_the_block("scaling" in rotary)
+        if unknown:
+            raise ValueError(f"layer {layer}: the file says what this attention does not do ({', '.join(unknown)}); attention.GGUFAttention takes frequencies and an amplitude of your own")
         inv_freq, amplitude = ops.rotary_frequencies(**{**known, **rotary}, device=device)
         return GGUFAttention(qkv, o, int(head_dim), inv_freq, amplitude=amplitude, q_norm=q_norm, k_norm=k_norm, eps=float(meta.get("attention.layer_norm_rms_epsilon", 1e-6)),
                              interleaved=interleaved)

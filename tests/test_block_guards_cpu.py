@@ -234,3 +234,40 @@ def test_a_residual_of_any_shape_in_front_of_a_layer_with_adapters(monkeypatch, 
     want = plain.unfused(x.reshape(-1, K))
     assert out.shape == (*x_shape[:-1], 24) and torch.equal(out.reshape(-1, 24), want[:, :24]) and torch.equal(seen[0][0].reshape(-1, K), want)
     assert torch.equal(pre.residual_out.reshape(-1, K), plain.residual_out) and pre.residual_out.shape == (6, K)
+
+
+def block_model(d=64, unmapped=(), **meta):
+    """A loaded model of one attention block in host memory, its file's numbers under `meta` (rope__scaling__type for "rope.scaling.type")."""
+    model = loader.LoadedModel(meta={k.replace("__", "."): v for k, v in meta.items()}, unmapped=list(unmapped))
+    for key, lin in (("layers.3.self_attn.qkv_proj", GGUFLinear(512, [8 * d, 2 * d, 2 * d])), ("layers.3.self_attn.o_proj", GGUFLinear(8 * d, [512]))):
+        lin.gguf_groups = {"q": (torch.zeros(1, dtype=torch.uint8),)}
+        model.linears[key] = lin
+    return model
+
+
+def test_the_files_scaling_is_taken_whole():
+    meta = dict(rope__freq_base=1e6, rope__scaling__type="yarn", rope__scaling__factor=4.0, rope__scaling__original_context_length=4096, attention__key_length=64)
+    want = ops.rotary_frequencies(64, 1e6, scaling="yarn", factor=4.0, original_context=4096, beta_fast=16.0, beta_slow=2.0, device="cpu")
+    got = block_model(rope__scaling__yarn_beta_fast=16.0, rope__scaling__yarn_beta_slow=2.0, rope__scaling__yarn_ext_factor=1.0, **meta).attention(3)
+    assert torch.equal(got.inv_freq, want[0]) and got.amplitude == want[1]
+    usual = block_model(**meta).attention(3)
+    assert torch.equal(usual.inv_freq, ops.rotary_frequencies(64, 1e6, scaling="yarn", factor=4.0, original_context=4096, device="cpu")[0]) and not torch.equal(usual.inv_freq, got.inv_freq)
+    assert torch.equal(block_model(**meta).attention(3, beta_fast=16.0, beta_slow=2.0).inv_freq, want[0])
+
+
+@pytest.mark.parametrize("meta,unmapped", [
+    (dict(rope__scaling__attn_factor=1.2), ()), (dict(rope__scaling__yarn_attn_factor=0.9), ()), (dict(rope__scaling__yarn_ext_factor=0.5), ()), (dict(rope__scaling__yarn_log_multiplier=0.1), ()),
+    (dict(rope__scaling__alpha=1000.0), ()), (dict(rope__scaling__factor=8.0), ()), ({}, ("rope_freqs.weight",)), ({}, ("blk.3.rope_factors_long.weight",))], ids=str)
+def test_scaling_that_is_not_known_is_refused(meta, unmapped):
+    model = block_model(attention__key_length=64, unmapped=unmapped, **meta)
+    with pytest.raises(ValueError, match="does not do"):
+        model.attention(3)
+    assert torch.equal(model.attention(3, scaling="linear", factor=2.0).inv_freq, ops.rotary_frequencies(64, scaling="linear", factor=2.0, device="cpu")[0])
+
+
+@pytest.mark.parametrize("meta", [dict(attention__sliding_window=4096), dict(attention__scale=0.1), dict(attn_logit_softcapping=50.0), dict(attention__max_alibi_bias=8.0), dict(attention__clamp_kqv=8.0),
+                                  dict(attention__causal=False)], ids=str)
+def test_an_attention_of_another_kind_is_refused(meta):
+    with pytest.raises(ValueError, match="does not do"):
+        block_model(attention__key_length=64, **meta).attention(3, scaling="none")
+    assert block_model(attention__key_length=64, attention__sliding_window=0, attention__causal=True).attention(3).n_heads == 8
