@@ -607,15 +607,17 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, scaling: str |
     """(inv_freq float64 [rotary_dim / 2], amplitude) for qk_norm_rope, made once per model: radians per position of each rotated pair.
     `scaling`, the kinds a GGUF file names: None or "none"; "linear", positions divided by `factor`; "yarn", pairs that turn less than beta_slow times over
     `original_context` tokens divided by `factor`, those above beta_fast kept, a ramp between, and values times 0.1 ln(factor) + 1."""
-    if rotary_dim < 0 or rotary_dim % 2 or base <= 0 or factor <= 0:
+    if not (rotary_dim >= 0 and rotary_dim % 2 == 0 and 0 < base < math.inf and 0 < factor < math.inf):
         raise GqError(f"rotary_dim is even, base and factor are positive; got {rotary_dim}, {base}, {factor}")
     inv = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / max(1, rotary_dim))
     amplitude = 1.0
     if scaling == "linear":
         inv = inv / factor
     elif scaling == "yarn":
-        if not original_context or original_context <= 0:
+        if not original_context or not 0 < original_context < math.inf:
             raise GqError("yarn needs the context the model was trained on")
+        if not (base > 1 and 0 < beta_slow <= beta_fast < math.inf):
+            raise GqError(f"yarn needs a base above 1 and turns 0 < beta_slow <= beta_fast; got {base}, {beta_slow}, {beta_fast}")
         pair = lambda turns: rotary_dim * math.log(original_context / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
         low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rotary_dim - 1)
         kept = 1 - ((torch.arange(inv.numel(), dtype=torch.float64) - low) / max(high - low, 0.001)).clamp(0, 1)

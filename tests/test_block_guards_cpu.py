@@ -271,3 +271,10 @@ def test_an_attention_of_another_kind_is_refused(meta):
     with pytest.raises(ValueError, match="does not do"):
         block_model(attention__key_length=64, **meta).attention(3, scaling="none")
     assert block_model(attention__key_length=64, attention__sliding_window=0, attention__causal=True).attention(3).n_heads == 8
+
+
+@pytest.mark.parametrize("bad", [dict(base=1.0), dict(base=0.5), dict(beta_slow=0.0), dict(beta_fast=0.0), dict(beta_slow=-1.0), dict(beta_slow=40.0), dict(beta_fast=float("inf")), dict(base=float("nan")), dict(factor=float("nan")),
+                                 dict(factor=float("inf")), dict(base=float("inf")), dict(original_context=float("nan")), dict(original_context=-4)], ids=str)
+def test_rotations_that_are_none_are_refused(bad):
+    with pytest.raises(E):
+        ops.rotary_frequencies(**{**dict(rotary_dim=64, base=1e4, scaling="yarn", factor=4.0, original_context=4096), **bad}, device="cpu")
