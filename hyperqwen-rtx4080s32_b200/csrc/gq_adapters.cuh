@@ -7,8 +7,9 @@
 // Bound by bytes, in decode those of the adapters (below a few MB latency is all), in chunks those of base and out.
 //
 // Measured (graph of calls): one row beside qkv, rank 16, 6.2 us (two launches, two rounds of memory, a cluster's sums); 27 rows of 8 adapters of rank 32 beside gate_up 11.8 (18 MB, floor 2.8); 64 rows of 16
-// of rank 64 beside down 24 (49 MB, floor 7.6; 36 where A is not in the L2): the inner blocks wait for loads and for one another at 15 % of DRAM's rate, and why so long is not known; 2,051 rows of rank 16 beside gate_up 84 (312 MB, floor 48), of
-// rank 128 beside qkv 96 (floor 16): there the inner products run at 160 TFLOP/s, and mma.sync of 64 x 64 tiles is what bounds them.
+// of rank 64 beside down 24 (49 MB, floor 7.6; 37 where A is not in the L2): the inner warps go through four or five whole latencies one behind the other, two barriers of the cluster for every adapter, at 15 % of DRAM's rate, and the outer
+// tiles of 4 rows load one adapter's columns behind another's; 2,051 rows of rank 16 beside gate_up 83 (312 MB, floor 48), of
+// rank 128 beside qkv 95 (floor 16): there the inner products run at 160 TFLOP/s, and mma.sync of 64 x 64 tiles is what bounds them.
 // Tried: all of a block's part of A asked of the L2 at once (m64 36 to 36 us, one row 6.2 to 6.5); sums of the parts by the outer blocks (m64 7 us less in the inner, 8 more in the outer kernel); decode through the chunk kernels (m64 24 to 36); the base straight to registers with two to
 // four tiles ahead (m2051 outer 86 to 110); 64 rows x 256 or 32 x 512 columns in shared memory with two blocks to an SM (79 and 77 against 67 with four blocks of 32 x 256).
 #pragma once

@@ -70,7 +70,7 @@ static int check_low_rank(const gq_low_rank_args *p, int64_t *n_total) {
 static int64_t up256(int64_t v) { return (v + 255) & ~(int64_t)255; }
 static int ranks_of(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 // How the inner products are cut: sixteens of ranks to a block, blocks that share a tile's adapters, parts of K (256 at least; the blocks of a cluster), blocks for all ranks.
-// Clusters are powers of two, of sixteen only while there are few: thirteen parts of 2,051 rows beside gate_up took 8 us more than eight, sixteen for each of seven adapters of
+// 148, 74, 296 and 444 are one, a half, two and three blocks to each of a B200's SMs.  Clusters are powers of two, of sixteen only while there are few: thirteen parts of 2,051 rows beside gate_up took 8 us more than eight, sixteen for each of seven adapters of
 // rank 32 beside qkv 4 us more than eight and fewer ranks to a block; one row beside qkv is 0.3 us faster with sixteen.
 struct LowRankCut {
     int ranks, groups, parts, turns;
@@ -206,7 +206,9 @@ extern "C" int gq_head_norm_rope(const gq_head_norm_args *p, void *stream) {
     } else {
         int group = 1;                                                       // lanes of a head, a power of two
         while (group * 16 < p->head_dim) group *= 2;
-        const int batch = p->T >= 2048 ? HEAD_BATCH : 1;                     // few tokens: a block each
+        // Tokens to a block.  One each while that fills the GPU about once, then four, whose start (positions, turns, weights) is one.  As one / as four to a block, 40 / 8 heads of 128 with the store:
+        // 256 tokens 4.2 / 7.7 us, 1,024 8.7 / 9.0, 1,536 12.2 / 13.1, 2,047 15.6 / 13.9, 4,096 32.6 / 27.6, 8,192 62 / 51; 24 / 4 gated heads of 256 1,536 13.0 / 14.9, 2,047 16.5 / 15.8, 8,192 66 / 57.
+        const int batch = p->T >= 2048 ? HEAD_BATCH : 1;
         const unsigned blocks = (unsigned)((p->T + batch - 1) / batch);
         if (p->interleaved) GQ_CUDA(launch_pdl(head_norm_kernel<true>, dim3(blocks), HEAD_THREADS, 0, stream, a, batch, group, status));
         else GQ_CUDA(launch_pdl(head_norm_kernel<false>, dim3(blocks), HEAD_THREADS, 0, stream, a, batch, group, status));
@@ -226,6 +228,8 @@ static int check_attention(const gq_attention_args *p) {
     return GQ_OK;
 }
 // Rows of a tile, in eights: those of a sequence's tokens under one kv head, as far as the batch's average tells.  (16 x 4 tokens of 5 heads: 52 us as a warp for every 8 rows, 45 as three eights of one.)
+// One width serves a whole batch, so a long chunk among decodes costs both: 1,024 tokens of one sequence and 63 decodes over 1,000 to 7,000 keys take 638 us in one call, 278 and 176 in two; with 16 tokens for
+// 1,024 184 in one, 24 and 176 in two (heads 40 / 8 of 128).
 static int row_eights(const gq_attention_args *p) {
     const int64_t tokens = p->n_seqs ? (p->T + p->n_seqs - 1) / p->n_seqs : 1, rows = tokens * (p->n_heads / p->n_kv_heads);
     return rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 ? 3 : 4;

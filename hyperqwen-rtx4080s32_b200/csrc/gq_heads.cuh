@@ -39,7 +39,7 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // norm is a few shuffles and a rotation needs no exchange.  Sine and cosine are the same for all heads of a token: a block takes `batch` tokens, computes their turns into shared memory
 // (in 64 bits up to the fraction of a turn) while its first loads are under way, then walks the tokens' heads; values are copied behind them.  The bytes of the rows, queries and keys in and
 // out, are the floor; what is near it is the issue rate, hence the paired arithmetic, weights as floats in shared memory and no division in the walk.
-// Measured (graph of calls): 8 tokens 3.4 us (one round of memory, the turns, one round); 2,051 tokens of 24 / 4 gated heads of 256 with the store 15.4 (67 MB, floor 10.3); 8,192 of 40 / 8 heads of
+// Measured (graph of calls): 8 tokens 3.6 us (one round of memory, the turns, one round); 2,051 tokens of 24 / 4 gated heads of 256 with the store 15.5 (67 MB, floor 10.3); 8,192 of 40 / 8 heads of
 // 128 37.5 = 5.4 TB/s (floor 30.9).  Blocks that stay and compute the next batch's turns ahead were slower (8,192 tokens 50 to 60 us before the arithmetic was paired).
 constexpr int HEAD_THREADS = 256, HEAD_BATCH = 4;
 template <bool INTERLEAVED>
@@ -179,7 +179,8 @@ __global__ void __launch_bounds__(HEAD_THREADS) head_norm_kernel(const __grid_co
     }
 }
 
-// Heads that do not fall into pairs of 16-byte pieces (head_dim or a half-turned part that is no multiple of 16): one block to a token's head, a value at a time
+// Heads that do not fall into pairs of 16-byte pieces (head_dim or a half-turned part that is no multiple of 16): one block to a token's head, a value at a time, the turn of its pair computed for each in 64 bits,
+// which is what the time is.  2,000 tokens of 40 / 8 heads of 96 with 24 dimensions turned 64 us (floor 6.1; with 32 turned, in the kernel above, 13.7), 8 tokens 3.0.
 __global__ void head_norm_any_kernel(const gq_head_norm_args p, int *status) {
     __shared__ float u[512];
     __shared__ float part[32];

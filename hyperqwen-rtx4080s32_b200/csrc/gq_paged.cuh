@@ -11,12 +11,14 @@
 // A block is KG key groups.  A key group streams 16 keys at a time through a ring of S stages of its own in shared memory (cp.async, 16 bytes a lane; rows at a pitch of 2 head_dim + 16 bytes, so that
 // ldmatrix meets no bank twice) and multiplies them by all rows of the tile, 8 NQ of them: scores as k q^T and outputs as v^T p^T (mma.sync m16n8k16, keys and dimensions on M), since the rows are
 // what there are few of.  A key is read from shared memory once.  Heads of 256 are split over DG = 2 warps, which exchange their halves of the scores.  p enters as two bf16 parts (p and what its
-// rounding left): one part would add an error as large as the output's own rounding, and leaving the second out gained 3 % at 8 x 8,192 keys and nothing elsewhere.  tcgen05 has nothing to give
-// here: a tile would use 5 to 32 of its 128 rows, and the loads are the bound.
+// rounding left): one part would add an error as large as the output's own rounding, and leaving the second out gained 3 % at 8 x 8,192 keys and nothing elsewhere.  With one token of a few heads the
+// loads are the bound, whatever multiplies.  With several tokens or chunks of prompts they are not, and the same transposed products would suit tcgen05 (128 keys or dimensions on M, the rows on N, scores and
+// outputs in tensor memory); that has not been built.
 //
-// Measured (graph of calls, heads 40 / 8 of 128, bf16): 64 sequences of up to 16,384 keys 231 us = 6.1 TB/s of cache, 0.93 of a copy's rate; 131,072 keys of one 98 us, 5.5 TB/s: the SMs do not get
-// their bytes equally fast (80 us in the middle, 97 the slowest), and the join takes 5.  8 of up to 8,192 20 us, 517 keys of one 7.6, of which a launch, the way to the first key and a join are 6.
-// 16 x 4 tokens of 24 / 4 heads of 256 107 us = 3.3 TB/s: two warps to a scheduler, each with a chain of 72 products, an exchange and the probabilities of 24 rows for every 16 keys.
+// Measured (graph of calls, heads 40 / 8 of 128, bf16): 64 sequences of up to 16,384 keys 231 us = 6.1 TB/s of cache, 0.93 of a copy's rate; 131,072 keys of one 97 us, 5.5 TB/s: the SMs do not get
+// their bytes equally fast (80 us in the middle, 97 the slowest), and the join takes 5.  8 of up to 8,192 21 us, 517 keys of one 7.6, of which a launch, the way to the first key and a join are 6.
+// Chunks of prompts: 2,048 tokens 750 us = 57 TFLOP/s, 512 behind 7,680 keys 745 us = 112 TFLOP/s, 8,192 tokens 7.3 ms: tiles of 32 rows read the keys again and again, and every block walks all
+// tiles in front of its first.  16 x 4 tokens of 24 / 4 heads of 256 109 us = 3.2 TB/s: two warps to a scheduler, each with a chain of 72 products, an exchange and the probabilities of 24 rows for every 16 keys.
 // Tried: a bulk copy for each row of 256 bytes, 18 cycles of the copy engine each (64 x 16,384 keys 280 to 362 us); rows on M, 8 to 16 of 16 of them empty (280 to 244 us); two or three
 // parts to a resident block, for the slow SMs' sake (131,072 keys 99 to 102 and 107 us: as many more parts to join); a warp for every 8 rows of a shared stage (gated 113 to 115 us).
 #pragma once

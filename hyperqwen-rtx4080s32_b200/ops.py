@@ -649,7 +649,8 @@ def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, inv_freq: tor
     """qk_norm_rope, with keys and values written to the pages of a cache in the same pass; returns q.
 
     k_pages, v_pages bf16 [pages, rows, n_kv_heads, head_dim] by strides; token t goes to slot slots[t] (int32 or int64) = page * rows + row.  A negative
-    slot stores nothing (padding); one beyond the cache stores nothing and makes device_status 2.  Of two tokens with one slot either may be kept."""
+    slot stores nothing (padding); one beyond the cache stores nothing and makes device_status 2.  Of two tokens with one slot, either one's key and either one's value may be
+    kept, head by head.  Keys and values have memory of their own, each row and head of them too."""
     if _aside():
         return torch.ops.gq_b200.qk_norm_rope_store(qkv, positions, inv_freq, n_heads, n_kv_heads, head_dim, q_norm, k_norm, eps, amplitude, interleaved, gated,
                                                     k_pages, v_pages, slots)
@@ -665,8 +666,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     page_table[s, j // rows] (int32 [sequences, pages]); the i-th of its n tokens sees the keys up to lens[s] - n + i.  A token that sees none: zeros.
 
     k_pages, v_pages bf16 [pages, rows, kv_heads, head_dim] by strides, head_dim 64, 128 or 256, heads a multiple of kv_heads.  q_starts (int32 [sequences + 1]):
-    the first token of each sequence, for batches of uneven numbers of tokens; rows behind the last sequence stay as they are in `out` (zeros without one).
-    scale: head_dim ** -0.5 if left out.  gate (q's shape, any strides over tokens and heads): the result is multiplied by sigmoid(gate).
+    the first token of each sequence, for batches of uneven numbers of tokens (a long chunk and many decodes are faster as two calls); rows behind the last sequence stay as they are in `out` (zeros without one).
+    scale: head_dim ** -0.5 if left out.  gate (q's shape, any strides over tokens and heads): the result is multiplied by sigmoid(gate).  An infinite value that a token
+    sees may become NaN in it.
     A page outside the cache or a length beyond the table: NaN in the rows that see it, and device_status 2.  Probabilities, sums and the join of the
     cache's parts in 32 bits, one rounding; the order of the sums does not depend on timing."""
     if _aside():

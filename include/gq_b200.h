@@ -280,7 +280,7 @@ int gq_gemm_prefill(const void *x_dev, int64_t M, int64_t K, int64_t ldx, const 
  * before all of them have been checked (< 0: nothing was launched).  Reference: none — the reference leaves these steps to the engine
  * around its linear method. */
 
-/* Low-rank adapters of many requests beside one (merged) layer, any number of rows:
+/* Low-rank adapters of many requests beside one (merged) layer, up to 4,194,240 rows:
  *   out[m, n] = base[m, n] + scales[i, s] * sum_r b[i, n, r] * (sum_k a[i, s * rank + r, k] * x[m, k]),  i = ids[m], s the shard of column n
  * ids[m] = -1: no adapter, out[m] = base[m].  Any other id outside the bank: out[m] is NaN and the device status becomes 2.  Rows of other
  * adapters never enter a row's sums.  K is a multiple of 256, rank a multiple of 8 up to GQ_MAX_RANK, one to GQ_MAX_DEVICE_SHARDS shards.  a, b and x
@@ -308,10 +308,10 @@ int gq_low_rank_add(const gq_low_rank_args *args, void *stream);
  *   u = x * rsqrt(mean(x^2) + eps) * weight       (weight null: u = x)
  *   (u_i, u_j) -> amplitude * (u_i cos f - u_j sin f, u_j cos f + u_i sin f),  f = position * inv_freq[p], for the pairs p of the first
  *   rotary_dim dimensions: (p, p + rotary_dim / 2), or (2 p, 2 p + 1) if interleaved; the others are left as u.
- * The angle is reduced in 64 bits, so positions may be large.  qkv holds n_heads heads of queries (each followed by a gate of the same
+ * The angle is reduced in 64 bits, so positions may be large; sine and cosine are within 2^-22.  qkv holds n_heads heads of queries (each followed by a gate of the same
  * size if gated: it is left alone), n_kv_heads of keys, n_kv_heads of values.  head_dim is a multiple of 8 up to 512, rotary_dim even (0: no rotation).
- * A negative slot stores nothing; one beyond the cache stores nothing and sets device status 2.  Two tokens of one slot: either may be kept.
- * The outputs and the pages share no memory with qkv; rows of qkv, rows and heads of pages, outputs and weights start at multiples of 16 bytes. */
+ * A negative slot stores nothing; one beyond the cache stores nothing and sets device status 2.  Two tokens of one slot: for each head's key and each
+ * head's value there either one may be kept.  The outputs and the pages share no memory with one another or an input; rows of qkv, rows and heads of pages, outputs and weights start at multiples of 16 bytes. */
 typedef struct gq_head_norm_args {
     const void *qkv;             /* bf16 [T, n_heads * head_dim * (gated ? 2 : 1) + 2 * n_kv_heads * head_dim], row stride ld_qkv */
     const void *positions;       /* int32 or int64 [T] */
@@ -330,7 +330,7 @@ int gq_head_norm_rope(const gq_head_norm_args *args, void *stream);
 
 /* Attention of the newest tokens of n_seqs sequences over a paged key-value cache that holds them already:
  *   o = sum_j softmax_j(scale * q . k_j) v_j over the keys j <= lens[s] - n + i of sequence s for the i-th of its n tokens,  o *= sigmoid(gate)
- * A token that sees no key: zeros.  Tokens of sequence s are q_starts[s] .. q_starts[s + 1] - 1 (null: T / n_seqs each); rows behind the last
+ * A token that sees no key: zeros, whatever its gate.  An infinite value that a token sees may become NaN.  Tokens of sequence s are q_starts[s] .. q_starts[s + 1] - 1 (null: T / n_seqs each); rows behind the last
  * sequence are left as they were.  Key j stands in row j % page_size of page page_table[s, j / page_size].  A page outside the cache, or a length beyond the table: the
  * rows that see it are NaN and the device status becomes 2.  head_dim 64, 128 or 256; n_heads a multiple of n_kv_heads; every row, head and page starts
  * at a multiple of 16 bytes (gate, and out: of 2).  out shares no memory with an input.  Up to 2^24 tokens, and tables of up to 2^30 keys. */
