@@ -377,8 +377,8 @@ class LowRankAdapters:
         j = self.check(slot, a, b, shard_id)
         r, first = a.shape[0], sum(self.n_outs[:j])
         mine, rows = self.a[slot, j * self.rank:(j + 1) * self.rank], self.b[slot, first:first + self.n_outs[j]]
-        mine[:r], mine[r:] = a.to(self.a), 0
-        rows[:, :r], rows[:, r:] = b.to(self.b), 0
+        mine[:r], mine[r:] = a.detach().to(self.a), 0              # trained matrices are parameters; the bank is not
+        rows[:, :r], rows[:, r:] = b.detach().to(self.b), 0
         self.scales[slot, j] = float(scale)
 
     def clear(self, slot: int) -> None:

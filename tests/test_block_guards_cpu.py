@@ -278,3 +278,11 @@ def test_an_attention_of_another_kind_is_refused(meta):
 def test_rotations_that_are_none_are_refused(bad):
     with pytest.raises(E):
         ops.rotary_frequencies(**{**dict(rotary_dim=64, base=1e4, scaling="yarn", factor=4.0, original_context=4096), **bad}, device="cpu")
+
+
+def test_trained_parameters_are_loaded_as_values():
+    bank = LowRankAdapters(loaded_layer((24,), (None,)), 2, 8)
+    a, b = (torch.nn.Parameter(torch.ones(s)) for s in ((4, K), (24, 4)))
+    bank.load(1, a, b, torch.tensor(0.5))
+    assert not any(t.requires_grad for t in (bank.a, bank.b, bank.scales)) and a.requires_grad
+    assert bool((bank.a[1, :4] == 1).all()) and bool((bank.b[1, :, :4] == 1).all()) and bank.scales[1, 0] == 0.5
