@@ -195,7 +195,7 @@ extern "C" int gq_head_norm_rope(const gq_head_norm_args *p, void *stream) {
     if (store) {
         if ((p->n_pages && (!p->k_pages || !p->v_pages)) || !p->slots || (p->slots_bytes != 4 && p->slots_bytes != 8) || p->k_out || !aligned(p->k_pages, 16) || !aligned(p->v_pages, 16)) return GQ_ERR_ARG;
         for (int i = 0; i < 3; ++i)
-            if (p->k_strides[i] % 8 || p->v_strides[i] % 8) return GQ_ERR_ARG;
+            if (p->k_strides[i] < 0 || p->v_strides[i] < 0 || p->k_strides[i] % 8 || p->v_strides[i] % 8) return GQ_ERR_ARG;
     } else if (!p->k_out || !aligned(p->k_out, 16)) return GQ_ERR_ARG;
     int *status;
     if (const int rc = status_word(&status)) return rc;
@@ -288,7 +288,7 @@ extern "C" int gq_paged_attention(const gq_attention_args *p, void *stream) {
     if (!p->q || !p->lens || !p->out || p->ld_table < p->table_width || (p->n_pages && (!p->k_pages || !p->v_pages)) || (p->table_width && !p->page_table)) return GQ_ERR_ARG;
     if (!aligned(p->q, 16) || !aligned(p->k_pages, 16) || !aligned(p->v_pages, 16)) return GQ_ERR_ARG;
     for (int i = 0; i < 3; ++i)
-        if (p->k_strides[i] % 8 || p->v_strides[i] % 8 || (i < 2 && p->q_strides[i] % 8)) return GQ_ERR_ARG;
+        if (p->k_strides[i] < 0 || p->v_strides[i] < 0 || p->k_strides[i] % 8 || p->v_strides[i] % 8 || (i < 2 && p->q_strides[i] % 8)) return GQ_ERR_ARG;
     int *status;
     if (const int rc = status_word(&status)) return rc;
     int64_t bytes;

@@ -322,7 +322,7 @@ typedef struct gq_head_norm_args {
     void *k_pages, *v_pages;     /* bf16 [n_pages, page_size, n_kv_heads, head_dim] by strides; null where keys are not stored, or n_pages is 0 */
     const void *slots;           /* int32 or int64 [T]: page * page_size + row; null where keys are not stored */
     int64_t T, ld_qkv, n_pages;
-    int64_t k_strides[3], v_strides[3];     /* elements between pages, rows, heads */
+    int64_t k_strides[3], v_strides[3];     /* elements between pages, rows, heads; none is negative */
     int32_t n_heads, n_kv_heads, head_dim, rotary_dim, page_size, positions_bytes, slots_bytes, interleaved, gated;
     float eps, amplitude;
 } gq_head_norm_args;
@@ -344,7 +344,7 @@ typedef struct gq_attention_args {
     void *out;                   /* as q, by strides of its own */
     int64_t T, n_seqs, table_width, ld_table, n_pages;
     int64_t q_strides[2], gate_strides[2], out_strides[2];      /* elements between tokens, heads */
-    int64_t k_strides[3], v_strides[3];                         /* elements between pages, rows, heads */
+    int64_t k_strides[3], v_strides[3];                         /* elements between pages, rows, heads; none is negative */
     int32_t n_heads, n_kv_heads, head_dim, page_size;
     float scale;
     void *workspace;             /* gq_attention_workspace_bytes(args) bytes, 256-byte aligned; null if that is 0 */

@@ -286,3 +286,24 @@ def test_trained_parameters_are_loaded_as_values():
     bank.load(1, a, b, torch.tensor(0.5))
     assert not any(t.requires_grad for t in (bank.a, bank.b, bank.scales)) and a.requires_grad
     assert bool((bank.a[1, :4] == 1).all()) and bool((bank.b[1, :, :4] == 1).all()) and bank.scales[1, 0] == 0.5
+
+
+class AttentionArgs(ctypes.Structure):
+    """gq_attention_args of include/gq_b200.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k_pages", "v_pages", "page_table", "lens", "q_starts", "gate", "out")] + [(n, ctypes.c_int64) for n in ("T", "n_seqs", "table_width", "ld_table", "n_pages")] + [
+        (n, ctypes.c_int64 * 2) for n in ("q_strides", "gate_strides", "out_strides")] + [(n, ctypes.c_int64 * 3) for n in ("k_strides", "v_strides")] + [
+        (n, ctypes.c_int32) for n in ("n_heads", "n_kv_heads", "head_dim", "page_size")] + [("scale", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64)]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are none: what is accepted has to end at the missing device")
+@pytest.mark.parametrize("which", ["k_strides", "v_strides"])
+@pytest.mark.parametrize("strides,accepted", [((2048, 64, 1024), True), ((0, 64, 0), True), ((-2048, 64, 1024), False), ((2048, -64, 1024), False), ((2048, 64, -1024), False), ((2048, 60, 1024), False)], ids=str)
+def test_strides_of_pages_at_the_c_entries(which, strides, accepted):
+    """A negative stride between rows would be taken as 32 unsigned bits, and one that leads below the first page as a slot that is none."""
+    at = 1 << 20
+    a = AttentionArgs(q=at, k_pages=at, v_pages=at, page_table=at, lens=at, out=at, T=2, n_seqs=2, table_width=4, ld_table=4, n_pages=8, n_heads=2, n_kv_heads=2, head_dim=64, page_size=16, scale=1.0)
+    b = HeadNormArgs(qkv=at, q_out=at, positions=at, slots=at, k_pages=at, v_pages=at, T=2, ld_qkv=384, n_pages=8, n_heads=2, n_kv_heads=2, head_dim=64, page_size=16, positions_bytes=8, slots_bytes=8)
+    for args, entry in ((a, "gq_paged_attention"), (b, "gq_head_norm_rope")):
+        args.k_strides[:] = args.v_strides[:] = (2048, 64, 1024)
+        getattr(args, which)[:] = strides
+        assert (getattr(_lib.lib(), entry)(ctypes.byref(args), None) == -3) == (not accepted)
